@@ -1,0 +1,69 @@
+// 8-bit block-scaled matrices: the held form shared by quant8.hip, gemm8.hip and rows8.hip.
+//
+// A matrix [R, C] is held as codes [R][up128(C)] bytes (zero behind C) and scale bytes [up128(C) / 128][up128(R)]: the byte
+// e + 127 is the scale 2^e of a row's block of 128 columns, rows contiguous.  Powers of two because (a) the scaling is then
+// exact, so a code is the input rounded ONCE and is defined bit for bit, (b) the matrix instruction takes the scale as an
+// operand (E8M0) and applies it for nothing, (c) 2^e x code is exact in bf16.  One granularity for every operand: a 128 x 128
+// weight tile repeats its byte for 128 rows (1/128 byte an element).
+#pragma once
+#include "common.h"
+
+constexpr int B8 = 128;                              // block: columns that share a scale
+constexpr int B8_MIN_EXP = -112;                     // smallest scale exponent: 2^-e and code x 2^e stay normal fp32 numbers
+
+__host__ __device__ static inline long up128(long n) { return (n + 127) / 128 * 128; }
+
+// Scale exponent of a block from the bits of its largest finite magnitude: the smallest e >= -112 with amax <= largest * 2^e.
+// largest = 1.75 * 2^8 (e4m3) or 1.75 * 2^15 (e5m2), so e follows from amax's exponent and whether its mantissa exceeds 1.75.
+template <int FMT> __device__ __forceinline__ int block_exponent(uint32_t amax_bits) {
+    const int e = (int)(amax_bits >> 23) - 127 - (FMT ? 15 : 8) + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return e < B8_MIN_EXP ? B8_MIN_EXP : e;          // (zero and subnormal fp32 maxima land here too)
+}
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// |x| as bits, 0 for inf and NaN: they take no part in the scale (and become NaN, or e5m2's infinity, as codes)
+__device__ __forceinline__ uint32_t finite_abs_bits(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+// four values, already scaled into the format's range -> four codes (nearest, ties to even)
+template <int FMT> __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
+    int r = 0;
+    if constexpr (FMT) {
+        r = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, r, false);
+        r = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, r, true);
+    } else {
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, r, false);
+        r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+    }
+    return (uint32_t)r;
+}
+// four codes -> four values (unscaled, exact)
+typedef float b8_f32x2 __attribute__((ext_vector_type(2)));
+typedef float b8_f32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ b8_f32x4 unpack_codes(int fmt, uint32_t u) {
+    const b8_f32x2 lo = fmt ? __builtin_amdgcn_cvt_pk_f32_bf8((int)u, false) : __builtin_amdgcn_cvt_pk_f32_fp8((int)u, false);
+    const b8_f32x2 hi = fmt ? __builtin_amdgcn_cvt_pk_f32_bf8((int)u, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)u, true);
+    return b8_f32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+// element types of unpacked tensors (CLT_DT_*): fp32, bf16, fp16
+template <int DT> struct Elem { typedef uint16_t type; };
+template <> struct Elem<CLT_DT_F32> { typedef float type; };
+template <int DT> __device__ __forceinline__ float elem_to_f32(typename Elem<DT>::type v) {
+    if constexpr (DT == CLT_DT_F32) return v;
+    else if constexpr (DT == CLT_DT_BF16) return bf16_to_f32(v);
+    else return f16_to_f32(v);
+}
+// two fp32 -> one dword of 16-bit results, nearest even (fp16: overflow gives inf; the loss scaler's flag is not touched here)
+template <int DT> __device__ __forceinline__ uint32_t pack_out16(float lo, float hi) {
+    if constexpr (DT == CLT_DT_BF16) return pack_bf16x2(lo, hi);
+    else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const b8_f32x2 v = {lo, hi};
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+    }
+}
+template <int DT> __device__ __forceinline__ typename Elem<DT>::type f32_to_elem(float v) {
+    if constexpr (DT == CLT_DT_F32) return v;
+    else return (uint16_t)pack_out16<DT>(v, 0.0f);
+}

@@ -1,0 +1,244 @@
+"""8-bit block-scaled operators (include/clt_hip.h, "8-bit block-scaled matrices"): packing and restoring activations and
+weights, products of packed matrices, and the linear map of a few or many tokens on kept packed weights.
+
+A matrix [R, C] is held as 8-bit floats with one power-of-two scale for every row and block of 128 columns (`Block8`).
+Tensors may be fp32, bf16 or fp16, of any size (zero rows included) and with any strides as long as the last dimension is
+dense; everything runs on the tensors' device and on that device's current stream, allocates only through torch's caching
+allocator and can be captured into a graph.  Non-HIP tensors raise: there is no fallback."""
+from __future__ import annotations
+
+import contextlib
+from typing import Optional, Tuple
+
+import torch
+
+from ._lib import CltError, lib
+
+BLOCK = 128
+FORMATS = {"e4m3": 0, "e5m2": 1}
+_DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _up(n: int) -> int:
+    return (n + BLOCK - 1) // BLOCK * BLOCK
+
+
+def _call(name, *args):
+    rc = getattr(lib, name)(*args)
+    if rc:
+        raise CltError(name, rc)
+
+
+def _on(device):
+    """The tensors' device made current for a launch (a no-op when it is already)."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _fmt(fmt: str) -> int:
+    if fmt not in FORMATS:
+        raise ValueError(f"8-bit format must be one of {sorted(FORMATS)}, got {fmt!r}")
+    return FORMATS[fmt]
+
+
+def _dense(x: torch.Tensor, dims=(2, 3)) -> torch.Tensor:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError("crosslayer_transcoder_amd ops need CUDA (HIP) tensors; there is no CPU fallback")
+    if x.dtype not in _DT:
+        raise TypeError(f"expected float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() not in dims:
+        raise ValueError(f"expected {' or '.join(map(str, dims))} dimensions, got shape {tuple(x.shape)}")
+    return x if x.shape[-1] <= 1 or x.stride(-1) == 1 else x.contiguous()
+
+
+class Block8:
+    """A batch of matrices [L, rows, cols] in 8 bits.  data: uint8 [L, rows, >= cols rounded up to 128], rows 16-byte aligned,
+    codes of `fmt` ("e4m3" / "e5m2"), ZERO behind column `cols` up to the next multiple of 128; scale: uint8 [L, >= blocks of 128
+    columns, >= rows], byte e + 127 for the scale 2^e of a row's block.  The pack functions below make it; one may be built
+    from kept tensors (a checkpoint of packed weights) as well."""
+    __slots__ = ("data", "scale", "rows", "cols", "fmt")
+
+    def __init__(self, data: torch.Tensor, scale: torch.Tensor, rows: int, cols: int, fmt: str = "e4m3"):
+        _fmt(fmt)
+        if data.dtype != torch.uint8 or scale.dtype != torch.uint8:
+            raise TypeError("codes and scale bytes are uint8 tensors")
+        if data.device != scale.device:
+            raise ValueError("codes and scale bytes are on different devices")
+        if data.dim() != 3 or scale.dim() != 3 or data.shape[0] != scale.shape[0]:
+            raise ValueError("codes [L, rows, bytes] and scale bytes [L, blocks, rows] have three dimensions")
+        if rows < 0 or cols < 0 or data.shape[1] != rows or data.shape[2] < _up(cols) or scale.shape[1] < _up(cols) // BLOCK or scale.shape[2] < rows:
+            raise ValueError(f"codes {tuple(data.shape)} / scale bytes {tuple(scale.shape)} do not hold a [{rows}, {cols}] matrix")
+        if data.numel() and (data.stride(2) != 1 or scale.stride(2) != 1 or data.stride(1) % 16 or data.stride(0) % 16 or data.data_ptr() % 16):
+            raise ValueError("packed rows are dense and start at multiples of 16 bytes")
+        self.data, self.scale, self.rows, self.cols, self.fmt = data, scale, rows, cols, fmt
+
+    @property
+    def batch(self) -> int:
+        return self.data.shape[0]
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def first_rows(self, n: int) -> "Block8":
+        """View of the first n rows."""
+        if not 0 <= n <= self.rows:
+            raise ValueError(f"{n} of {self.rows} rows")
+        return Block8(self.data[:, :n], self.scale, n, self.cols, self.fmt)
+
+    def first_columns(self, n: int) -> "Block8":
+        """View of the first n columns, n a multiple of 128 (a block belongs to one contraction)."""
+        if not 0 <= n <= self.cols or (n % BLOCK and n != self.cols):
+            raise ValueError(f"first {n} of {self.cols} columns: a multiple of {BLOCK} is needed")
+        return Block8(self.data, self.scale, self.rows, n, self.fmt)
+
+    def of_batch(self, l: int) -> "Block8":
+        """View of one matrix of the batch."""
+        return Block8(self.data[l:l + 1], self.scale[l:l + 1], self.rows, self.cols, self.fmt)
+
+    def nbytes(self) -> int:
+        return self.data.numel() + self.scale.numel()
+
+    def __repr__(self):
+        return f"Block8({self.fmt}, batch={self.batch}, rows={self.rows}, cols={self.cols})"
+
+
+def _empty(x, rows, cols):
+    """Unwritten codes and scale bytes of a [L, rows, cols] matrix (every byte of both is written by clt_pack8)."""
+    L = x.shape[0]
+    return (torch.empty((L, rows, _up(cols)), dtype=torch.uint8, device=x.device),
+            torch.empty((L, _up(cols) // BLOCK, _up(rows)), dtype=torch.uint8, device=x.device))
+
+
+def pack8_raw(x: torch.Tensor, fmt: int, along: bool, across: bool, tiles: bool = False, sums: bool = False):
+    """clt_pack8 on x [L, R, C] -> (q, s, qt, st, column sums), None where not asked for."""
+    L, R, C = x.shape
+    q, s = _empty(x, R, C) if along else (None, None)
+    qt, st = _empty(x, C, R) if across else (None, None)
+    if L == 0 or R == 0 or C == 0:
+        return q, s, qt, st, (torch.zeros((L, C), dtype=torch.float32, device=x.device) if sums else None)
+    cs = ws = None
+    nws = 0
+    if sums:
+        nws = lib.clt_pack8_sums_workspace_bytes(L, R, C)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+        cs = torch.empty((L, C), dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        _call("clt_pack8", x.data_ptr(), _DT[x.dtype], x.stride(1), x.stride(0), L, R, C, fmt, int(tiles),
+              q.data_ptr() if along else None, s.data_ptr() if along else None, qt.data_ptr() if across else None,
+              st.data_ptr() if across else None, cs.data_ptr() if sums else None, ws.data_ptr() if sums else None, nws, _stream(x.device))
+    return q, s, qt, st, cs
+
+
+def _as3(x):
+    x = _dense(x)
+    return x.unsqueeze(0) if x.dim() == 2 else x
+
+
+def quantize8(x: torch.Tensor, fmt: str = "e4m3") -> Block8:
+    """x [R, C] or [L, R, C] held with blocks along its columns (the operand of a contraction over them)."""
+    x = _as3(x)
+    q, s, *_ = pack8_raw(x, _fmt(fmt), True, False)
+    return Block8(q, s, x.shape[1], x.shape[2], fmt)
+
+
+def quantize8_t(x: torch.Tensor, fmt: str = "e4m3") -> Block8:
+    """x^T [C, R] held with blocks of 128 rows of x: the 8-bit checkpoint a contraction over the rows (a weight gradient) reads."""
+    x = _as3(x)
+    _, _, q, s, _ = pack8_raw(x, _fmt(fmt), False, True)
+    return Block8(q, s, x.shape[2], x.shape[1], fmt)
+
+
+def quantize8_both(x: torch.Tensor, fmt: str = "e4m3") -> Tuple[Block8, Block8]:
+    """(quantize8(x), quantize8_t(x)) from one read of x."""
+    x = _as3(x)
+    q, s, qt, st, _ = pack8_raw(x, _fmt(fmt), True, True)
+    return Block8(q, s, x.shape[1], x.shape[2], fmt), Block8(qt, st, x.shape[2], x.shape[1], fmt)
+
+
+def quantize8_tiles(x: torch.Tensor, fmt: str = "e4m3") -> Tuple[Block8, Block8]:
+    """A weight matrix and its transpose, one scale per 128 x 128 tile: both hold the same values."""
+    x = _as3(x)
+    q, s, qt, st, _ = pack8_raw(x, _fmt(fmt), True, True, tiles=True)
+    return Block8(q, s, x.shape[1], x.shape[2], fmt), Block8(qt, st, x.shape[2], x.shape[1], fmt)
+
+
+def dequantize8(q: Block8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values held, [L, rows, cols], each rounded once to `dtype` (exact in fp32, and in bf16 for normal numbers)."""
+    if dtype not in _DT:
+        raise TypeError(f"expected float32, bfloat16 or float16, got {dtype}")
+    _hip(q)
+    out = torch.empty((q.batch, q.rows, q.cols), dtype=dtype, device=q.device)
+    if out.numel():
+        with _on(q.device):
+            _call("clt_unpack8", q.data.data_ptr(), q.scale.data_ptr(), FORMATS[q.fmt], q.batch, q.rows, q.cols, q.data.stride(1),
+                  q.scale.stride(1), q.data.stride(0), q.scale.stride(0), out.data_ptr(), _DT[dtype], _stream(q.device))
+    return out
+
+
+def _hip(q):
+    if not isinstance(q, Block8):
+        raise TypeError("expected a Block8")
+    if not q.data.is_cuda:
+        raise RuntimeError("crosslayer_transcoder_amd ops need CUDA (HIP) tensors; there is no CPU fallback")
+
+
+def _bias(bias, L, N, device):
+    if bias is None:
+        return None
+    if bias.device != device or bias.numel() != L * N or (bias.dim() > 1 and tuple(bias.shape) != (L, N)):
+        raise ValueError(f"bias must be [{L}, {N}] on the operands' device")
+    if not bias.dtype.is_floating_point:
+        raise TypeError(f"bias must be floating point, got {bias.dtype}")
+    return bias.to(torch.float32).contiguous()
+
+
+def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
+          out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
+    """out [L, M, N] (+)= a [L, M, K] @ b [L, N, K]^T + bias [L, N].  fp32 results: exact products, fp32 sums; bf16 / fp16 results:
+    the 8-bit matrix instructions (twice the rate; their loss is far below the result's rounding).  `out`: an [L, M, N] tensor or
+    view with a dense last dimension to write into (its dtype counts); accumulate: add to it (fp32 only)."""
+    _hip(a), _hip(b)
+    L, M, N, K = a.batch, a.rows, b.rows, a.cols
+    if b.batch != L or b.cols != K or b.device != a.device:
+        raise ValueError(f"operands do not match: {a} and {b}")
+    if out is None:
+        if accumulate:
+            raise ValueError("accumulate needs the tensor to add to")
+        if out_dtype not in _DT:
+            raise TypeError(f"expected float32, bfloat16 or float16, got {out_dtype}")
+        out = torch.empty((L, M, N), dtype=out_dtype, device=a.device)
+    elif out.dtype not in _DT or (accumulate and out.dtype != torch.float32):
+        raise TypeError(f"cannot {'add to' if accumulate else 'write'} {out.dtype}")
+    elif tuple(out.shape) != (L, M, N) or out.device != a.device or (N > 1 and out.stride(2) != 1) or (M > 1 and out.stride(1) < N):
+        raise ValueError(f"out must be an [{L}, {M}, {N}] tensor of non-overlapping dense rows on the operands' device")
+    bias = _bias(bias, L, N, a.device)
+    if out.numel():
+        with _on(a.device):
+            _call("clt_gemm8", a.data.data_ptr(), a.scale.data_ptr(), FORMATS[a.fmt], a.data.stride(1), a.scale.stride(1),
+                  a.data.stride(0), a.scale.stride(0), b.data.data_ptr(), b.scale.data_ptr(), FORMATS[b.fmt], b.data.stride(1),
+                  b.scale.stride(1), b.data.stride(0), b.scale.stride(0), out.data_ptr(), _DT[out.dtype], out.stride(1) if M > 1 else N,
+                  out.stride(0), bias.data_ptr() if bias is not None else None, N, M, N, K, L, int(accumulate), _stream(a.device))
+    return out
+
+
+def linear8(x: torch.Tensor, w: Block8, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """y [T, L, N] = x [T, L, K] @ w^T + bias with kept packed weights w [L, N, K] (x [T, K] -> y [T, N] when L == 1): x is packed in
+    e4m3 with blocks along K on the way.  out_dtype: x's by default."""
+    x = _dense(x)
+    _hip(w)
+    two = x.dim() == 2
+    if two:
+        x = x.unsqueeze(1)
+    T, L, K = x.shape
+    if L != w.batch or K != w.cols or x.device != w.device:
+        raise ValueError(f"x {tuple(x.shape)} does not match {w}")
+    dt = x.dtype if out_dtype is None else out_dtype
+    if dt not in _DT:
+        raise TypeError(f"expected float32, bfloat16 or float16, got {dt}")
+    y = torch.empty((T, L, w.rows), dtype=dt, device=x.device)
+    gemm8(quantize8(x.transpose(0, 1)), w, bias, out=y.transpose(0, 1))
+    return y.squeeze(1) if two else y

@@ -527,6 +527,38 @@ int clt_sparse_reduce_dots_f32(const float* dots, long stride, const uint32_t* c
 int clt_sparse_scatter_dense_f32(const uint32_t* col_start, const int32_t* tok, const float* val, int B, int ncols,
                                  float* out, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * 8-bit block-scaled matrices: operands of fast products and activations kept in 8 bits for the backward pass (beyond the
+ * reference, which holds every activation of the module forward in fp32 or 16 bits; clt.py:157-165, 241-248, 334-343).
+ *
+ * Held form of a matrix [rows, cols]: `q` codes [rows][up128(cols)] (one byte each, 0 behind cols) and `s` scale bytes
+ * [up128(cols) / 128][up128(rows)]: byte e + 127 is the scale 2^e of a row's block of 128 columns.  e is the smallest integer
+ * >= -112 with amax <= largest * 2^e, amax over the block's finite values; code = x * 2^-e rounded to nearest, ties to even.
+ * NaN stays NaN; an infinity becomes NaN (e4m3, which has none) or stays (e5m2).  q, s and their pitches: 16-byte aligned.
+ */
+#define CLT_F8_E4M3 0 /* 4 exponent bits, 3 mantissa bits, largest 448   */
+#define CLT_F8_E5M2 1 /* 5 exponent bits, 2 mantissa bits, largest 57344 */
+#define CLT_DT_F32 0
+#define CLT_DT_BF16 1
+#define CLT_DT_F16 2
+/* x [batch][rows][cols] (strides in elements, unit column stride) -> q/s (blocks along the columns) and/or qt/st (x transposed,
+ * [cols][rows], blocks of 128 rows), from one read; either pair may be NULL.  tiles != 0: one scale per 128 x 128 tile, the same
+ * for both forms (weights: the two forms hold the same values).  column_sums (or NULL): fp32 [batch][cols], summed over rows in
+ * a fixed order (workspace: clt_pack8_sums_workspace_bytes). */
+size_t clt_pack8_sums_workspace_bytes(int batch, int rows, int cols);
+int clt_pack8(const void* x, int dtype, long row_stride, long batch_stride, int batch, int rows, int cols, int format, int tiles,
+              void* q, void* s, void* qt, void* st, float* column_sums, void* workspace, size_t workspace_bytes, void* stream);
+/* out [batch][rows][cols] (contiguous, dtype CLT_DT_*) = 2^e * code, rounded once.  pitch / scale_pitch: bytes per row of q / s. */
+int clt_unpack8(const void* q, const void* s, int format, int batch, int rows, int cols, long pitch, long scale_pitch,
+                long q_batch_stride, long s_batch_stride, void* out, int dtype, void* stream);
+/* C[M][N] (+)= A[M][K] * B[N][K]^T + bias[N], batched; pitches and batch strides of A, B in bytes, of C and bias in elements.
+ * c_dtype bf16 / fp16: 8-bit matrix instructions (products aligned to ~14 bits in groups of 16, fp32 sums, one rounding);
+ * c_dtype fp32: exact products (bf16 instructions), fp32 sums; accumulate != 0 (fp32 only): C += . K = 0 gives the bias. */
+int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long ldas, long a_batch, long as_batch,
+              const void* b, const void* b_scale, int b_format, long ldb, long ldbs, long b_batch, long bs_batch,
+              void* c, int c_dtype, long ldc, long c_batch, const float* bias, long bias_batch, int M, int N, int K, int batch,
+              int accumulate, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
