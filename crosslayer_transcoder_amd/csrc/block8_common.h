@@ -67,3 +67,33 @@ template <int DT> __device__ __forceinline__ typename Elem<DT>::type f32_to_elem
     if constexpr (DT == CLT_DT_F32) return v;
     else return (uint16_t)pack_out16<DT>(v, 0.0f);
 }
+
+// ---- products (gemm8.hip, gemm8_large.hip) ----
+typedef int b8_i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8_bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b8_bf16x8 __attribute__((ext_vector_type(8)));
+struct Gemm8Args {
+    const uint8_t *a, *as, *b, *bs;          // codes and scale bytes
+    void* c; const float* bias;
+    long lda, ldas, ldb, ldbs, ldc;          // pitches: code rows, scale-byte rows (one per block of 128), C rows
+    long ba, bas, bb, bbs, bc, bbias;        // batch strides
+    int M, N, KB, tilesA, tilesB;
+    int accumulate;
+};
+
+// 256 x 256 tiles; returns 1 where the shape is the small tiles' (gemm8_large.hip)
+int clt_internal_gemm8_large(const Gemm8Args& g, int fa, int fb, int dtype, int batch, hipStream_t st);
+
+// eight codes (two dwords) x 2^e -> eight bf16
+template <int FMT> __device__ __forceinline__ b8_bf16x8 widen8(uint32_t lo, uint32_t hi, float scale) {
+    b8_bf16x2 p[4];
+    if constexpr (FMT) {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, scale, false); p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, scale, true);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, scale, false); p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, scale, true);
+    } else {
+        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false); p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false); p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    }
+    return b8_bf16x8{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
+}
+

@@ -14,32 +14,7 @@
 #include "block8_common.h"
 
 namespace {
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
-struct Gemm8Args {
-    const uint8_t *a, *as, *b, *bs;          // codes and scale bytes
-    void* c; const float* bias;
-    long lda, ldas, ldb, ldbs, ldc;          // pitches: code rows, scale-byte rows (one per block of 128), C rows
-    long ba, bas, bb, bbs, bc, bbias;        // batch strides
-    int M, N, KB, tilesA, tilesB;
-    int accumulate;
-};
-
-// eight codes (two dwords) x 2^e -> eight bf16
-template <int FMT> __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float scale) {
-    bf16x2 p[4];
-    if constexpr (FMT) {
-        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, scale, false); p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(lo, scale, true);
-        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, scale, false); p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(hi, scale, true);
-    } else {
-        p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false); p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
-        p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false); p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
-    }
-    return bf16x8{p[0][0], p[0][1], p[1][0], p[1][1], p[2][0], p[2][1], p[3][0], p[3][1]};
-}
+typedef b8_f32x4 f32x4;
 
 // Four consecutive columns of a row of C: 16- or 8-byte store where the row's alignment allows it (vec), else element by element
 template <int DT> __device__ __forceinline__ void store4(void* c, long at, f32x4 v, int valid, bool vec, int accumulate) {
@@ -116,14 +91,14 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256) void gemm8_k
         if (kb + 1 < g.KB) load(kb + 1);
         __syncthreads();
         // a lane's 32 codes of a row: 16-byte chunks fq and fq + 4 (the same k for both operands; the order inside a block is free)
-        i32x8 fa[4], fb[4];
+        b8_i32x8 fa[4], fb[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const int x = fr >> 1, rowa = (wa * 64 + n * 16 + fr) * 128, rowb = 16384 + (wb * 64 + n * 16 + fr) * 128;
             const int4 a_lo = *reinterpret_cast<const int4*>(lds + rowa + ((fq ^ x) << 4)), a_hi = *reinterpret_cast<const int4*>(lds + rowa + (((fq + 4) ^ x) << 4));
             const int4 b_lo = *reinterpret_cast<const int4*>(lds + rowb + ((fq ^ x) << 4)), b_hi = *reinterpret_cast<const int4*>(lds + rowb + (((fq + 4) ^ x) << 4));
-            fa[n] = i32x8{a_lo.x, a_lo.y, a_lo.z, a_lo.w, a_hi.x, a_hi.y, a_hi.z, a_hi.w};
-            fb[n] = i32x8{b_lo.x, b_lo.y, b_lo.z, b_lo.w, b_hi.x, b_hi.y, b_hi.z, b_hi.w};
+            fa[n] = b8_i32x8{a_lo.x, a_lo.y, a_lo.z, a_lo.w, a_hi.x, a_hi.y, a_hi.z, a_hi.w};
+            fb[n] = b8_i32x8{b_lo.x, b_lo.y, b_lo.z, b_lo.w, b_hi.x, b_hi.y, b_hi.z, b_hi.w};
         }
         if constexpr (DT != CLT_DT_F32) {
 #pragma unroll
@@ -137,7 +112,7 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256) void gemm8_k
             for (int n = 0; n < 4; ++n) { xa[n] = exp2_int(ca[n] - 127); xb[n] = exp2_int(cb[n] - 127); }
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                bf16x8 ha[4], hb[4];
+                b8_bf16x8 ha[4], hb[4];
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     ha[n] = widen8<FA>((uint32_t)fa[n][2 * s], (uint32_t)fa[n][2 * s + 1], xa[n]);
@@ -193,9 +168,11 @@ extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long 
     Gemm8Args g = {static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(a_scale), static_cast<const uint8_t*>(b),
                    static_cast<const uint8_t*>(b_scale), c, bias, lda, ldas, ldb, ldbs, ldc, a_batch, as_batch, b_batch, bs_batch,
                    c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate};
+    const hipStream_t st = as_stream(stream);
+    const int rc = clt_internal_gemm8_large(g, a_format, b_format, c_dtype, batch, st);
+    if (rc <= 0) return rc;                                  // (1: the shape is the small tiles')
     const long blocks = (long)g.tilesA * g.tilesB * batch;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
-    const hipStream_t st = as_stream(stream);
     return c_dtype == CLT_DT_F32 ? launch<CLT_DT_F32>(g, a_format, b_format, blocks, st)
            : c_dtype == CLT_DT_BF16 ? launch<CLT_DT_BF16>(g, a_format, b_format, blocks, st)
                                     : launch<CLT_DT_F16>(g, a_format, b_format, blocks, st);

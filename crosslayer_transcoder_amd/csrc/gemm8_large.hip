@@ -1,0 +1,325 @@
+// The large form of clt_gemm8 (see gemm8.hip for the operator and its two inner products): 256 x 256 tiles for shapes that fill
+// the chip with them.
+//
+// One block of 4 waves per CU, 2 x 2 waves of 128 x 128 (256 accumulators and ~200 other registers a lane: one wave per SIMD has
+// all 512).  The wave tile is what the LDS allows: a block of 128 k costs a wave 16 fragments of 32 bytes a lane = 32 KB of
+// reads for 64 matrix instructions of 32 cycles; four waves read 128 KB in those 2048 cycles, half of the LDS's rate, where 8
+// waves of 128 x 64 would need three quarters and wait for it.
+// Operands go global -> LDS by DMA, two buffers of 64 KB, one 128-byte block of k at a time; the scale bytes of the block (256 + 256)
+// and the tile's bias ride along.  The grid is persistent; nothing of the epilogue passes through LDS, so both buffers
+// already receive the next tile's first two blocks while this tile's results are stored.
+//
+// Row order.  LDS row p of a 128-row half holds matrix row (p % 16) * 8 + p / 16 (A) or c(p % 16) * 8 + p / 16 with
+// c(4 q + i) = 4 i + q (B), so fragment j of a wave is rows 8 * lane + j: (a) the scale bytes of a lane's eight fragments are eight
+// consecutive bytes — one 8-byte read per operand and block, the instruction picks its byte by op_sel; (b) a lane's
+// accumulators of the eight B fragments are eight consecutive columns of C — 16 bytes of 16-bit results, 32 of fp32 — and four
+// lanes make 64 / 128 consecutive bytes: stores need no transposition.
+#include <type_traits>
+#include "block8_common.h"
+
+namespace {
+typedef b8_f32x4 f32x4;
+typedef b8_i32x8 i32x8;
+typedef b8_bf16x8 bf16x8;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+constexpr int OPB = 256 * 128;                        // one operand's block in LDS
+constexpr int STG = 2 * OPB;
+constexpr int SCALE_BASE = 2 * STG;                   // per buffer: 256 scale bytes of A, 256 of B
+constexpr int BIAS_BASE = SCALE_BASE + 2 * 512;       // four slots of 256 floats (a tile's, while up to two more are on their way)
+constexpr int LDS_BYTES = BIAS_BASE + 4 * 1024;
+static_assert(LDS_BYTES <= 160 * 1024, "LDS");
+extern __shared__ __attribute__((aligned(1024))) unsigned char g8_smem[];
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <int N, class F> __device__ __forceinline__ void unroll(F f) {
+    if constexpr (N > 0) { unroll<N - 1>(f); f(std::integral_constant<int, N - 1>{}); }
+}
+
+// 16-byte stores of rows that are aligned to their element only
+typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+
+template <int DT, int FA, int FB>
+__global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int total) {
+    constexpr bool WIDE = DT == CLT_DT_F32;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wb = w >> 1, wa = w & 1, fr = lane & 15, fq = lane >> 4;
+    const int nwg = g.tilesA * g.tilesB, nk = g.KB;
+    struct Tile { int batch, a0, b0; };
+    // block -> tile: every XCD (block index mod 8) works on a contiguous range of tiles, walked in panels of 4 A tiles with the A tile
+    // fastest, so that the blocks an XCD runs together share operand tiles in its L2
+    auto decode = [&](int vb) {
+        Tile t;
+        t.batch = vb / nwg;
+        int lid = vb - t.batch * nwg;
+        const int xcd = lid & 7, q = nwg >> 3, r = nwg & 7;
+        lid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lid >> 3);
+        constexpr int GA = 4;
+        const int full = g.tilesA / GA, rem = g.tilesA - full * GA, per = GA * g.tilesB;
+        int ta, tb;
+        if (lid < full * per) { const int pn = lid / per, x = lid - pn * per; tb = x / GA; ta = pn * GA + (x - tb * GA); }
+        else { const int x = lid - full * per; tb = x / rem; ta = full * GA + (x - tb * rem); }
+        t.a0 = ta * 256; t.b0 = tb * 256;
+        return t;
+    };
+
+    // ---- DMA: piece i of wave w fills LDS rows (4 i + w) * 8 .. + 7; a lane supplies 16 bytes (chunk XOR-swizzled with bits 1..3 of the
+    // row).  Descriptors start at the tile's first row and end behind its last one: rows past the matrix arrive as zeros.
+    const int q8 = (w & 1) * 8 + (lane >> 3);             // LDS row mod 16
+    const int ch = (lane & 7) ^ ((q8 >> 1) & 7);
+    const int vA = (q8 * 8 + (w >> 1)) * (int)g.lda + ch * 16;
+    const int vB = ((((q8 & 3) << 2) | (q8 >> 2)) * 8 + (w >> 1)) * (int)g.ldb + ch * 16;
+    __amdgpu_buffer_rsrc_t rA, rB, rS, rBias;
+    auto rsrc = [](const void* p, long records) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)records, 0x00020000); };
+    auto aim = [&](const Tile& t) {
+        rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda, (long)min(g.M - t.a0, 256) * g.lda);
+        rB = rsrc(g.b + t.batch * g.bb + (long)t.b0 * g.ldb, (long)min(g.N - t.b0, 256) * g.ldb);
+        // scale bytes (the dwords that hold a row's byte): even waves A's, odd waves B's — twice the same bytes instead of a branch
+        const uint8_t* sp = w & 1 ? g.bs + t.batch * g.bbs + t.b0 : g.as + t.batch * g.bas + t.a0;
+        // (the range check counts the scalar offset, here the block's scale row, too: the range ends with this tile's rows in the last one)
+        rS = rsrc(sp, (long)(nk - 1) * (w & 1 ? g.ldbs : g.ldas) + min(((w & 1 ? g.N - t.b0 : g.M - t.a0) + 3) & ~3, 256));
+        if (g.bias) rBias = rsrc(g.bias + t.batch * g.bbias + t.b0, min(g.N - t.b0, 256) * 4L);
+    };
+    auto piece = [&](int buf, int kt, int i) {
+        unsigned char* base = g8_smem + buf * STG + (i * 4 + w) * 1024;
+        const int rows = (i & 3) * 2 + (i >> 2) * 128;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (lds_void*)base, 16, vA + rows * (int)g.lda, kt * 128, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (lds_void*)(base + OPB), 16, vB + rows * (int)g.ldb, kt * 128, 0, 0);
+    };
+    const int srow = (int)(w & 1 ? g.ldbs : g.ldas);
+    auto scale_piece = [&](int buf, int kt) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rS, (lds_void*)(g8_smem + SCALE_BASE + buf * 512 + (w & 1) * 256), 4, lane * 4, kt * srow, 0, 0);
+    };
+    // ---- fragment addresses: LDS row j * 16 + fr of the wave's half
+    const int x = fr >> 1;
+    const int cB = ((fr & 3) << 2) | (fr >> 2);
+    const int scA = SCALE_BASE + wa * 128 + fr * 8, scB = SCALE_BASE + 256 + wb * 128 + cB * 8;
+    const int rowA = (wa * 128 + fr) * 128, rowB = OPB + (wb * 128 + fr) * 128;
+
+    f32x4 acc[8][8];
+#pragma unroll
+    for (int m = 0; m < 8; ++m)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int NST = WIDE ? 64 : 32;                   // stores of an interior tile per lane
+
+    // ---- the stream of k-blocks: staging runs two blocks ahead of the products, across tiles
+    int vb = blockIdx.x, svb = vb, skt = 0, sslot = 0, slot = 0, buf = 0;
+    Tile t = decode(vb);
+    auto enter = [&](const Tile& e) {                     // staging enters tile svb = e
+        if (svb < total) {
+            aim(e);
+            if (g.bias && w == 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(rBias, (lds_void*)(g8_smem + BIAS_BASE + sslot * 1024), 16, lane * 16, 0, 0, 0);
+        } else { rA = rsrc(g.a, 0); rB = rsrc(g.b, 0); rS = rsrc(g.as, 0); }      // nothing left: zeros arrive in a buffer nobody reads
+    };
+    // (moved on at the head of a block, where the staging state is needed: control flow behind the matrix instructions would let the
+    // compiler sink them, which have no side effects, below everything they are meant to overlap)
+    auto advance = [&](const Tile& next) {
+        if (++skt == nk) { skt = 0; svb += (int)gridDim.x; sslot = (sslot + 1) & 3; enter(next); }
+    };
+    enter(t);
+    for (int k = 0; k < 2; ++k) {
+        if (k) advance(decode(svb + (int)gridDim.x));
+        scale_piece(k, skt);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) piece(k, skt, i);
+    }
+    Tile nt = decode(svb + (int)gridDim.x);               // the tile staging enters next (decoded off the critical path)
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    // Buffer handover: this wave's reads of the block are complete and its pieces of the next block have landed; then all waves'.
+    // Vector memory retires in order: in a tile's first block the next block's pieces are older than the previous tile's stores,
+    // which may stay outstanding (63 is the counter's limit).  One asm statement: the scheduling region around it stays whole.
+    auto handover = [](int kt) {
+        asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(0)\n1:\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_barrier" ::"s"(kt), "i"(NST < 63 ? NST : 63) : "scc", "memory");
+    };
+    const int lo = (fq ^ x) << 4;
+    int aA = rowA, aB = rowB, aSA = scA, aSB = scB;       // the block's addresses; the other buffer's by XOR
+    auto flip = [&]() { aA ^= STG; aB ^= STG; aSA ^= 512; aSB ^= 512; };
+
+    // fast path state: fragments of the current block (and, from its second half on, of the next); 32-bit path state below
+    i32x8 fa[8], fb[8];
+    i32x2 sa, sb;
+    auto ld = [&](int at, int off) {                      // chunks fq and fq + 4: any split of the block's k that both operands share
+        const i32x4 u = *reinterpret_cast<const i32x4*>(g8_smem + (at + lo) + off), v = *reinterpret_cast<const i32x4*>(g8_smem + (at + (lo ^ 64)) + off);
+        return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // 32-bit results: a block is 4 steps of 32 k; a lane's 8 codes of a row and step are 8 bytes
+    const int half = (fq & 1) << 3, cq = fq >> 1;
+    auto ldw = [&](int at, int off, int s) { return *reinterpret_cast<const i32x2*>(g8_smem + (at + ((((2 * s) + cq) ^ x) << 4) + half) + off); };
+    i32x2 rb[8];
+    bf16x8 ha[8], hb;
+    float xa[8], xb[8];
+    auto scales = [&](float* d, int at) {
+        const i32x2 u = *reinterpret_cast<const i32x2*>(g8_smem + at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] = __uint_as_float((((uint32_t)u[j >> 2] >> (8 * (j & 3))) & 0xffu) << 23);
+    };
+    if constexpr (!WIDE) {
+        sa = *reinterpret_cast<const i32x2*>(g8_smem + aSA);
+        sb = *reinterpret_cast<const i32x2*>(g8_smem + aSB);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) fa[n] = ld(aA, n * 2048);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) fb[m] = ld(aB, m * 2048);
+    } else {
+        scales(xa, aSA);
+        scales(xb, aSB);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) { const i32x2 r = ldw(aA, n * 2048, 0); ha[n] = widen8<FA>((uint32_t)r[0], (uint32_t)r[1], xa[n]); }
+#pragma unroll
+        for (int m = 0; m < 8; ++m) rb[m] = ldw(aB, m * 2048, 0);
+        hb = widen8<FB>((uint32_t)rb[0][0], (uint32_t)rb[0][1], xb[0]);
+    }
+
+    for (;;) {
+        for (int kt = 0; kt < nk; ++kt) {
+            advance(nt);
+            if constexpr (!WIDE) {
+                // 64 instructions a block.  First half: B fragments 0..3, A fragments fastest; B fragments 4..7 are read meanwhile.
+                // Handover.  Second half: A fragment by A fragment against B fragments 4..7; the block after next is staged, the
+                // next block's B fragments 0..3 are read, and every A fragment is replaced by the next block's after its last use.
+                auto mfma = [&](auto m_, auto n_) {
+                    constexpr int m = decltype(m_)::value, n = decltype(n_)::value;
+                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[m], fa[n], acc[m][n], FB, FA, m & 3, sb[m >> 2], n & 3, sa[n >> 2]);
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                unroll<4>([&](auto m) {
+                    fb[m + 4] = ld(aB, (m + 4) * 2048);
+                    __builtin_amdgcn_sched_barrier(0);
+                    unroll<8>([&](auto n) { mfma(m, n); });
+                });
+                handover(kt);
+                flip();
+                const i32x2 sa_n = *reinterpret_cast<const i32x2*>(g8_smem + aSA), sb_n = *reinterpret_cast<const i32x2*>(g8_smem + aSB);
+                scale_piece(buf, skt);
+                unroll<8>([&](auto n) {
+                    unroll<4>([&](auto j) {
+                        if constexpr (j < 2 && n < 4) piece(buf, skt, 2 * n + j);
+                        if constexpr (j == 2 && n >= 4) fb[n - 4] = ld(aB, (n - 4) * 2048);
+                        mfma(std::integral_constant<int, 4 + decltype(j)::value>{}, n);
+                    });
+                    fa[n] = ld(aA, n * 2048);
+                });
+                sa = sa_n; sb = sb_n;
+            } else {
+                // 4 steps of 8 groups (B fragment m) of 8 instructions of 16 cycles.  In a step the next step's codes are read (groups
+                // 0..3), its A fragments converted (groups 4..7) and every B fragment one group ahead of its use.
+                float xa_n[8], xb_n[8];
+                unroll<4>([&](auto s) {
+                    constexpr int S = decltype(s)::value;
+                    i32x2 ra_n[8], rb_n[8];
+                    bf16x8 ha_n[8];
+                    if constexpr (S == 3) {
+                        handover(kt);
+                        flip();
+                        scales(xa_n, aSA);
+                        scales(xb_n, aSB);
+                        scale_piece(buf, skt);
+                    }
+                    unroll<8>([&](auto m_) {
+                        constexpr int m = decltype(m_)::value;
+                        if constexpr (m < 4) {
+#pragma unroll
+                            for (int j = 2 * m; j < 2 * m + 2; ++j) { ra_n[j] = ldw(aA, j * 2048, (S + 1) & 3); rb_n[j] = ldw(aB, j * 2048, (S + 1) & 3); }
+                        } else {
+#pragma unroll
+                            for (int j = 2 * m - 8; j < 2 * m - 6; ++j) ha_n[j] = widen8<FA>((uint32_t)ra_n[j][0], (uint32_t)ra_n[j][1], S == 3 ? xa_n[j] : xa[j]);
+                        }
+                        if constexpr (S == 3) piece(buf, skt, m);
+                        bf16x8 hb_n;
+                        if constexpr (m < 7) hb_n = widen8<FB>((uint32_t)rb[m + 1][0], (uint32_t)rb[m + 1][1], xb[m + 1]);
+                        else hb_n = widen8<FB>((uint32_t)rb_n[0][0], (uint32_t)rb_n[0][1], S == 3 ? xb_n[0] : xb[0]);
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb, ha[n], acc[m][n], 0, 0, 0);
+                        hb = hb_n;
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) { ha[j] = ha_n[j]; rb[j] = rb_n[j]; }
+                });
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { xa[j] = xa_n[j]; xb[j] = xb_n[j]; }
+            }
+            buf ^= 1;
+        }
+        const Tile cur = t;
+        const int cslot = slot;
+        vb += (int)gridDim.x;
+        slot = (slot + 1) & 3;
+        const bool more = vb < total;
+        if (more) t = decode(vb);
+        nt = decode(svb + (int)gridDim.x);
+        // ---- results: for (n, i) a lane has row 8 fr + n and eight columns 8 (4 i + fq) ..
+        typedef typename Elem<DT>::type T;
+        const int r0 = wa * 128 + fr * 8, c0 = wb * 128 + fq * 8;
+        const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N && !g.accumulate;
+        T* ctile = static_cast<T*>(g.c) + cur.batch * g.bc + (long)cur.a0 * g.ldc + cur.b0;
+        const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + c0;
+        const bool has_bias = g.bias != nullptr;
+        const int rows = g.M - cur.a0 - r0, cols = g.N - cur.b0 - c0;
+        const unsigned at = (unsigned)(r0 * (int)g.ldc + c0) * (unsigned)sizeof(T);      // a lane's offset in the tile: 32 bits (host check)
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 lo = f32x4{acc[0][n][i], acc[1][n][i], acc[2][n][i], acc[3][n][i]};
+                f32x4 hi = f32x4{acc[4][n][i], acc[5][n][i], acc[6][n][i], acc[7][n][i]};
+                if (has_bias) { lo += *reinterpret_cast<const f32x4*>(bl + i * 32); hi += *reinterpret_cast<const f32x4*>(bl + i * 32 + 4); }
+                T* p = reinterpret_cast<T*>(reinterpret_cast<char*>(ctile + (long)n * g.ldc + i * 32) + at);
+                if constexpr (WIDE) {
+                    if (interior) { *reinterpret_cast<f32x4_u*>(p) = lo; *reinterpret_cast<f32x4_u*>(p + 4) = hi; }
+                    else if (n < rows)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (i * 32 + j < cols) { const float v = j < 4 ? lo[j & 3] : hi[j & 3]; p[j] = g.accumulate ? p[j] + v : v; }
+                } else {
+                    const u32x4_u u = {pack_out16<DT>(lo[0], lo[1]), pack_out16<DT>(lo[2], lo[3]), pack_out16<DT>(hi[0], hi[1]), pack_out16<DT>(hi[2], hi[3])};
+                    if (interior) *reinterpret_cast<u32x4_u*>(p) = u;
+                    else if (n < rows)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (i * 32 + j < cols) p[j] = (T)(u[j >> 1] >> (16 * (j & 1)));
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (!more) break;
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!interior) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // (not NST stores: handover could not count)
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no DMA into this block's LDS outlives it
+}
+
+template <int DT, int FA, int FB> int launch(const Gemm8Args& g, int total, hipStream_t st) {
+    const auto f = gemm8_large_kernel<DT, FA, FB>;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES) != hipSuccess) return CLT_ERR_LAUNCH;
+    f<<<dim3((unsigned)(total < 256 ? total : 256)), dim3(256), LDS_BYTES, st>>>(g, total);
+    CLT_LAUNCH_CHECK();
+    return CLT_OK;
+}
+template <int DT> int launch_fmt(const Gemm8Args& g, int fa, int fb, int total, hipStream_t st) {
+    if (fa == 0 && fb == 0) return launch<DT, 0, 0>(g, total, st);
+    if (fa == 1 && fb == 0) return launch<DT, 1, 0>(g, total, st);
+    if (fa == 0) return launch<DT, 0, 1>(g, total, st);
+    return launch<DT, 1, 1>(g, total, st);
+}
+}  // namespace
+
+int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, int batch, hipStream_t st) {
+    Gemm8Args g = g0;
+    g.tilesA = (g.M - 1) / 256 + 1; g.tilesB = (g.N - 1) / 256 + 1;
+    const long total = (long)g.tilesA * g.tilesB * batch;
+    // a chip's worth of tiles, mostly full ones
+    if (g.KB < 1 || g.M < 128 || g.N < 128 || total < 128 || total > 0x3fffffffL) return 1;
+    // 32-bit offsets inside a tile's rows and over a scale row's blocks, whole dwords of scale bytes
+    if (256 * g.lda > 0x7fffffffL || 256 * g.ldb > 0x7fffffffL || (long)g.KB * g.ldas > 0x7ffffeffL || (long)g.KB * g.ldbs > 0x7ffffeffL) return 1;
+    if (256 * g.ldc * 4 > 0x7fffffffL) return 1;
+    if (g.ldas % 4 || g.ldbs % 4 || g.bas % 4 || g.bbs % 4 || ((uintptr_t)g.as & 3) || ((uintptr_t)g.bs & 3)) return 1;
+    return dtype == CLT_DT_F32 ? launch_fmt<CLT_DT_F32>(g, fa, fb, (int)total, st)
+           : dtype == CLT_DT_BF16 ? launch_fmt<CLT_DT_BF16>(g, fa, fb, (int)total, st)
+                                  : launch_fmt<CLT_DT_F16>(g, fa, fb, (int)total, st);
+}
