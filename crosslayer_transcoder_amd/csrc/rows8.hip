@@ -1,0 +1,257 @@
+// y [T][L][N] = x [T][L][K] * w [L][N][K]^T + bias for few tokens (T <= 64) and kept 8-bit weights: the serving form of a linear
+// map.  x is packed (e4m3, blocks along K) on the way; products are exact and sums fp32 whatever the result's type (bf16 matrix
+// instructions on the values held, as clt_gemm8's fp32 form).
+//
+// Bound: HBM, the N * K weight bytes once.  A block of 8 waves owns a layer, a slice of K and R rows of w.  It packs its slice of
+// x into LDS (the values held, as bf16 — once per block, so R is made as large as the grid allows), then every wave streams 16
+// rows x 128 k (2 KB) a step, four steps ahead in registers: 64 KB in flight per block of 8 waves, which is what 8 TB/s over
+// 256 CUs needs at ~2 us of latency.  The first steps are requested before x is packed.  Tokens ride the instruction's "N" index
+// (16 of them, repeated where there are fewer), weight rows its "M" index.  Where rows alone give too few blocks, K is cut into
+// slices whose partial sums a second launch adds in order.
+#include "block8_common.h"
+
+namespace {
+typedef b8_f32x4 f32x4;
+typedef b8_bf16x8 bf16x8;
+constexpr int WAVES = 8, MAX_T = 64;
+constexpr int LDS_CAP = 136 * 1024;                  // packed slice of x at most
+
+struct Rows8Args {
+    const void* x; long x_token, x_layer;            // strides in elements
+    const uint8_t *w, *ws; long ldw, ldws, bw, bws;
+    const float* bias; long bbias;
+    void* y; long y_token, y_layer; int y_dtype;     // results, or
+    float* part;                                     // partial sums [slice][layer][token][N] when K is cut
+    int T, N, K, KB, slice_kb, slices, groups;       // groups: row groups of 16 per wave
+    int row_blocks;
+    int x_dtype, vec, y_vec;
+};
+
+extern __shared__ __attribute__((aligned(16))) unsigned char r8_smem[];
+
+template <int DT> __device__ __forceinline__ void load_x8(const void* x, long at, int n, bool vec, float v[8]) {
+    const typename Elem<DT>::type* p = static_cast<const typename Elem<DT>::type*>(x) + at;
+    if (vec && n >= 8) {
+        if constexpr (DT == CLT_DT_F32) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { v[2 * k] = elem_to_f32<DT>((uint16_t)(q[k] & 0xffffu)); v[2 * k + 1] = elem_to_f32<DT>((uint16_t)(q[k] >> 16)); }
+        }
+    } else
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = k < n ? elem_to_f32<DT>(p[k]) : 0.0f;
+}
+
+// `valid` of four consecutive results; whole: one store (valid >= 4 and the row's alignment allows it)
+__device__ __forceinline__ void store_result(void* y, int dtype, long at, f32x4 v, int valid, bool whole) {
+    if (dtype == CLT_DT_F32) {
+        float* p = static_cast<float*>(y) + at;
+        if (whole) *reinterpret_cast<f32x4*>(p) = v;
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i < valid) p[i] = v[i];
+    } else {
+        uint16_t* p = static_cast<uint16_t*>(y) + at;
+        const bool bf = dtype == CLT_DT_BF16;
+        const uint2 u = bf ? make_uint2(pack_out16<CLT_DT_BF16>(v[0], v[1]), pack_out16<CLT_DT_BF16>(v[2], v[3]))
+                           : make_uint2(pack_out16<CLT_DT_F16>(v[0], v[1]), pack_out16<CLT_DT_F16>(v[2], v[3]));
+        if (whole) *reinterpret_cast<uint2*>(p) = u;
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i < valid) p[i] = (uint16_t)((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
+    }
+}
+
+// MT: groups of 16 tokens; FMT: format of the weights
+template <int MT, int FMT> __global__ __launch_bounds__(WAVES * 64) void rows8_kernel(Rows8Args a) {
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
+    const int rbk = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks, slice = rest % a.slices, layer = rest / a.slices;
+    const int kb0 = slice * a.slice_kb, nkb = min(a.slice_kb, a.KB - kb0);
+    const int pitch = a.slice_kb * 256 + 16;             // bytes of a token's values in LDS
+    const int n0 = (rbk * WAVES + w) * a.groups * 16;
+    const int ngroups = min(a.groups, (a.N - n0 + 15) >> 4);     // (<= 0: nothing for this wave but packing)
+    const int steps = max(ngroups, 0) * nkb;
+    const uint8_t *W = a.w + layer * a.bw + (long)kb0 * 128 + fq * 32, *S = a.ws + layer * a.bws + (long)kb0 * a.ldws;
+
+    // ---- weight stream: step s is row group s / nkb, block s % nkb
+    constexpr int U = 4;
+    uint4 q[U][2];
+    int sc[U];
+    int lg = 0, lk = 0;                                  // next step to request
+    auto request = [&](int u) {
+        const int row = min(n0 + lg * 16 + fr, a.N - 1);
+        const uint4* p = reinterpret_cast<const uint4*>(W + (long)row * a.ldw + lk * 128);
+        q[u][0] = p[0];
+        q[u][1] = p[1];
+        sc[u] = S[(long)lk * a.ldws + row];
+        if (++lk == nkb) { lk = 0; ++lg; }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) if (u < steps) request(u);
+
+    // ---- pack the slice of x: 16 lanes a block of 128 of one token, 8 elements a lane
+    for (int id = tid >> 4; id < a.T * nkb; id += WAVES * 4) {
+        const int t = id / nkb, kb = id - t * nkb, k = (kb0 + kb) * 128 + fr * 8;
+        float v[8];
+        const long at = t * a.x_token + layer * a.x_layer + k;
+        if (a.x_dtype == CLT_DT_F32) load_x8<CLT_DT_F32>(a.x, at, a.K - k, a.vec, v);
+        else if (a.x_dtype == CLT_DT_BF16) load_x8<CLT_DT_BF16>(a.x, at, a.K - k, a.vec, v);
+        else load_x8<CLT_DT_F16>(a.x, at, a.K - k, a.vec, v);
+        uint32_t m = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, finite_abs_bits(v[j]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+        const int e = block_exponent<0>(m);
+        const float f = exp2_int(-e), g = exp2_int(e);
+        const uint32_t lo = pack_codes<0>(v[0] * f, v[1] * f, v[2] * f, v[3] * f), hi = pack_codes<0>(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+        *reinterpret_cast<bf16x8*>(r8_smem + t * pitch + kb * 256 + fr * 16) = widen8<0>(lo, hi, g);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (LDS only: the weight requests stay in flight)
+
+    const unsigned char* xrow[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xrow[t] = r8_smem + min(t * 16 + fr, a.T - 1) * pitch + fq * 64;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    int cg = 0, ck = 0;
+    for (int base = 0; base < steps; base += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (base + u >= steps) break;
+            const uint32_t c[8] = {q[u][0].x, q[u][0].y, q[u][0].z, q[u][0].w, q[u][1].x, q[u][1].y, q[u][1].z, q[u][1].w};
+            const float s = __uint_as_float((uint32_t)sc[u] << 23);
+            bf16x8 h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[j] = widen8<FMT>(c[2 * j], c[2 * j + 1], s);
+            if (base + u + U < steps) request(u);
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h[j], *reinterpret_cast<const bf16x8*>(xrow[t] + ck * 256 + j * 16), acc[t], 0, 0, 0);
+            if (++ck == nkb) {                           // a row group is complete: row n0 + cg * 16 + fq * 4 + i of token fr
+                const int n = n0 + cg * 16 + fq * 4, valid = a.N - n;
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    const int tok = t * 16 + fr;
+                    if (tok < a.T && valid > 0) {
+                        if (a.part) store_result(a.part, CLT_DT_F32, (((long)slice * (gridDim.x / a.row_blocks / a.slices) + layer) * a.T + tok) * a.N + n, acc[t], valid, valid >= 4 && a.N % 4 == 0);
+                        else {
+                            if (a.bias)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) if (i < valid) acc[t][i] += a.bias[layer * a.bbias + n + i];
+                            store_result(a.y, a.y_dtype, tok * a.y_token + layer * a.y_layer + n, acc[t], valid, valid >= 4 && a.y_vec);
+                        }
+                    }
+                    acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                ck = 0;
+                ++cg;
+            }
+        }
+    }
+}
+
+// partial sums of the slices -> results, slices in order
+__global__ __launch_bounds__(256) void rows8_fold_kernel(Rows8Args a, int layers, long n) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;                 // (layer, token, column)
+    if (i >= n) return;
+    const long lt = i / a.N;
+    const int c = (int)(i - lt * a.N), layer = (int)(lt / a.T), t = (int)(lt - (long)layer * a.T);
+    float s = 0.0f;
+    const float* p = a.part + i;
+    int k = 0;
+    for (; k + 8 <= a.slices; k += 8) {                                  // eight requests at a time, added in order
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = p[(k + j) * n];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+    }
+    for (; k < a.slices; ++k) s += p[k * n];
+    if (a.bias) s += a.bias[layer * a.bbias + c];
+    store_result(a.y, a.y_dtype, t * a.y_token + layer * a.y_layer + c, f32x4{s, 0.0f, 0.0f, 0.0f}, 1, false);
+}
+
+// How the work is cut: blocks of K per slice, slices, row groups per wave.  Rows first (no partial sums); K is cut where the
+// packed x does not fit LDS or where rows give less than two blocks a CU, down to 4 blocks of k a slice (a stream needs some
+// length); a wave takes more row groups as long as that leaves three blocks a CU (x is packed once per block).
+struct Cut { int slice_kb, slices, groups, row_blocks; };
+Cut cut_rows8(int T, int L, int N, int KB) {
+    Cut c;
+    const int fit = (LDS_CAP / T - 16) / 256;                            // blocks of k whose x fits LDS (>= 8 for 64 tokens)
+    const long rb = (N + WAVES * 16 - 1) / (WAVES * 16);
+    long slices = (KB + fit - 1) / fit;
+    const long want = 512;
+    if (L * rb * slices < want) {
+        const long by_grid = (want + L * rb - 1) / (L * rb), most = KB / 4 > 0 ? KB / 4 : 1;
+        const long s = by_grid < most ? by_grid : most;
+        if (s > slices) slices = s;
+        // cutting into two only pays when the stream is long: the second launch costs as much as ~16 steps
+        if (slices * 16 > KB && (KB + fit - 1) / fit == 1) slices = KB >= 32 ? KB / 16 : 1;
+    }
+    c.slice_kb = (int)((KB + slices - 1) / slices);
+    c.slices = (KB + c.slice_kb - 1) / c.slice_kb;
+    long g = L * rb * c.slices / 768;
+    c.groups = (int)(g < 1 ? 1 : g > 16 ? 16 : g);
+    c.row_blocks = (int)((N + (long)WAVES * 16 * c.groups - 1) / ((long)WAVES * 16 * c.groups));
+    return c;
+}
+
+template <int MT> int launch_rows(const Rows8Args& a, int fmt, long blocks, int lds, hipStream_t st) {
+    const auto f = fmt ? rows8_kernel<MT, 1> : rows8_kernel<MT, 0>;
+    if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return CLT_ERR_LAUNCH;
+    f<<<dim3((unsigned)blocks), dim3(WAVES * 64), lds, st>>>(a);
+    CLT_LAUNCH_CHECK();
+    return CLT_OK;
+}
+}  // namespace
+
+extern "C" size_t clt_linear8_rows_workspace_bytes(int tokens, int layers, int N, int K) {
+    if (tokens <= 0 || tokens > MAX_T || layers <= 0 || N <= 0 || K <= 0) return 0;
+    const Cut c = cut_rows8(tokens, layers, N, (int)(up128(K) / 128));
+    return c.slices > 1 ? (size_t)c.slices * layers * tokens * N * 4 : 0;
+}
+
+extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride, long x_layer_stride, const void* w, const void* w_scale,
+                                int w_format, long ldw, long ldws, long w_batch, long ws_batch, const float* bias, long bias_batch,
+                                void* y, int y_dtype, long y_token_stride, long y_layer_stride, int tokens, int layers, int N, int K,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+    if (tokens <= 0 || layers <= 0 || N <= 0 || K <= 0 || x_dtype < 0 || x_dtype > 2 || y_dtype < 0 || y_dtype > 2 || (w_format & ~1)) return CLT_ERR_SHAPE;
+    if (tokens > MAX_T) return 1;                                        // the many-token form: clt_pack8 + clt_gemm8
+    if (!x || !w || !w_scale || !y || ldw < up128(K) || ldws < N) return CLT_ERR_SHAPE;
+    const size_t xs = x_dtype == CLT_DT_F32 ? 4 : 2, ys = y_dtype == CLT_DT_F32 ? 4 : 2;
+    if (!aligned16(w) || ldw % 16 || w_batch % 16 || ((uintptr_t)x & (xs - 1)) || ((uintptr_t)y & (ys - 1)) || ((uintptr_t)bias & 3)) return CLT_ERR_ALIGN;
+    const int KB = (int)(up128(K) / 128);
+    const Cut c = cut_rows8(tokens, layers, N, KB);
+    const size_t need = clt_linear8_rows_workspace_bytes(tokens, layers, N, K);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) return CLT_ERR_WORKSPACE;
+    Rows8Args a;
+    a.x = x; a.x_token = x_token_stride; a.x_layer = x_layer_stride; a.x_dtype = x_dtype;
+    a.w = static_cast<const uint8_t*>(w); a.ws = static_cast<const uint8_t*>(w_scale); a.ldw = ldw; a.ldws = ldws; a.bw = w_batch; a.bws = ws_batch;
+    a.bias = bias; a.bbias = bias_batch;
+    a.y = y; a.y_token = y_token_stride; a.y_layer = y_layer_stride; a.y_dtype = y_dtype;
+    a.part = c.slices > 1 ? static_cast<float*>(workspace) : nullptr;
+    a.T = tokens; a.N = N; a.K = K; a.KB = KB; a.slice_kb = c.slice_kb; a.slices = c.slices; a.groups = c.groups; a.row_blocks = c.row_blocks;
+    a.vec = aligned16(x) && x_token_stride % (long)(16 / xs) == 0 && x_layer_stride % (long)(16 / xs) == 0;
+    a.y_vec = (uintptr_t)y % (4 * ys) == 0 && y_token_stride % 4 == 0 && y_layer_stride % 4 == 0;
+    const long blocks = (long)layers * c.slices * c.row_blocks;
+    if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
+    const int lds = tokens * (c.slice_kb * 256 + 16);
+    const hipStream_t st = as_stream(stream);
+    const int rc = tokens <= 16 ? launch_rows<1>(a, w_format, blocks, lds, st) : tokens <= 32 ? launch_rows<2>(a, w_format, blocks, lds, st)
+                                                                                              : launch_rows<4>(a, w_format, blocks, lds, st);
+    if (rc != CLT_OK || c.slices == 1) return rc;
+    const long n = (long)layers * tokens * N, fold = (n + 255) / 256;
+    if (fold > 0x7fffffffL) return CLT_ERR_RANGE;
+    rows8_fold_kernel<<<dim3((unsigned)fold), dim3(256), 0, st>>>(a, layers, n);
+    CLT_LAUNCH_CHECK();
+    return CLT_OK;
+}

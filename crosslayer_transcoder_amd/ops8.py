@@ -16,6 +16,8 @@ from ._lib import CltError, lib
 
 BLOCK = 128
 FORMATS = {"e4m3": 0, "e5m2": 1}
+#: tokens up to which linear8 streams the weights past all of them in one launch (clt_linear8_rows)
+FEW_TOKENS = 64
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -239,6 +241,17 @@ def linear8(x: torch.Tensor, w: Block8, bias: Optional[torch.Tensor] = None, out
     dt = x.dtype if out_dtype is None else out_dtype
     if dt not in _DT:
         raise TypeError(f"expected float32, bfloat16 or float16, got {dt}")
-    y = torch.empty((T, L, w.rows), dtype=dt, device=x.device)
-    gemm8(quantize8(x.transpose(0, 1)), w, bias, out=y.transpose(0, 1))
+    N = w.rows
+    y = torch.empty((T, L, N), dtype=dt, device=x.device)
+    if 0 < T <= FEW_TOKENS and K and N and L:
+        bias = _bias(bias, L, N, x.device)
+        nws = lib.clt_linear8_rows_workspace_bytes(T, L, N, K)
+        ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
+        with _on(x.device):
+            _call("clt_linear8_rows", x.data_ptr(), _DT[x.dtype], x.stride(0), x.stride(1), w.data.data_ptr(), w.scale.data_ptr(),
+                  FORMATS[w.fmt], w.data.stride(1), w.scale.stride(1), w.data.stride(0), w.scale.stride(0),
+                  bias.data_ptr() if bias is not None else None, N, y.data_ptr(), _DT[dt], L * N, N, T, L, N, K,
+                  ws.data_ptr() if nws else None, nws, _stream(x.device))
+    else:
+        gemm8(quantize8(x.transpose(0, 1)), w, bias, out=y.transpose(0, 1))
     return y.squeeze(1) if two else y
