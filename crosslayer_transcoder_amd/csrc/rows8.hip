@@ -2,12 +2,13 @@
 // map.  x is packed (e4m3, blocks along K) on the way; products are exact and sums fp32 whatever the result's type (bf16 matrix
 // instructions on the values held, as clt_gemm8's fp32 form).
 //
-// Bound: HBM, the N * K weight bytes once.  A block of 8 waves owns a layer, a slice of K and R rows of w.  It packs its slice of
-// x into LDS (the values held, as bf16 — once per block, so R is made as large as the grid allows), then every wave streams 16
-// rows x 128 k (2 KB) a step, four steps ahead in registers: 64 KB in flight per block of 8 waves, which is what 8 TB/s over
-// 256 CUs needs at ~2 us of latency.  The first steps are requested before x is packed.  Tokens ride the instruction's "N" index
-// (16 of them, repeated where there are fewer), weight rows its "M" index.  Where rows alone give too few blocks, K is cut into
-// slices whose partial sums a second launch adds in order.
+// Bound: HBM, the N * K weight bytes once.  A block of 8 waves owns a layer, a slice of K and some rows of w.  It packs its slice
+// of x into LDS (the values held, as bf16), then every wave streams 1 or 2 groups of 16 rows x 128 k (2 KB each) a step, two to
+// four steps ahead in registers; the first steps are requested before x is packed.  Tokens ride the matrix instruction's "N"
+// index (16 of them, repeated where there are fewer), weight rows its "M" index.  Where rows alone give too few blocks, K is cut
+// into slices whose partial sums a second launch adds in order.
+// Measured: 768 -> 32768, 1 token 7.1 us (an empty launch: 3.3); 12 layers of it, 302 MB of weights: 57 us = 5.3 TB/s (1 token), 80 us
+// (32 tokens); 393216 -> 768, 1 token: 73 us = 4.1 TB/s with the second launch.
 #include "block8_common.h"
 
 namespace {
@@ -22,8 +23,7 @@ struct Rows8Args {
     const float* bias; long bbias;
     void* y; long y_token, y_layer; int y_dtype;     // results, or
     float* part;                                     // partial sums [slice][layer][token][N] when K is cut
-    int T, N, K, KB, slice_kb, slices, groups;       // groups: row groups of 16 per wave
-    int row_blocks;
+    int T, N, K, KB, slice_kb, slices, chunks, row_blocks, layers;
     int x_dtype, vec, y_vec;
 };
 
@@ -66,41 +66,43 @@ __device__ __forceinline__ void store_result(void* y, int dtype, long at, f32x4 
     }
 }
 
-// MT: groups of 16 tokens; FMT: format of the weights
-template <int MT, int FMT> __global__ __launch_bounds__(WAVES * 64) void rows8_kernel(Rows8Args a) {
+// MT: groups of 16 tokens; G: groups of 16 weight rows a wave has in hand; FMT: format of the weights.  A step is G x 16 rows x 128 k;
+// D steps are in flight.
+template <int MT, int G, int FMT> __global__ __launch_bounds__(WAVES * 64, MT >= 4 ? 2 : 4) void rows8_kernel(Rows8Args a) {
+    constexpr int D = G == 1 && MT < 4 ? 4 : 2;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
     const int rbk = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks, slice = rest % a.slices, layer = rest / a.slices;
     const int kb0 = slice * a.slice_kb, nkb = min(a.slice_kb, a.KB - kb0);
     const int pitch = a.slice_kb * 256 + 16;             // bytes of a token's values in LDS
-    const int n0 = (rbk * WAVES + w) * a.groups * 16;
-    const int ngroups = min(a.groups, (a.N - n0 + 15) >> 4);     // (<= 0: nothing for this wave but packing)
-    const int steps = max(ngroups, 0) * nkb;
-    const uint8_t *W = a.w + layer * a.bw + (long)kb0 * 128 + fq * 32, *S = a.ws + layer * a.bws + (long)kb0 * a.ldws;
+    const uint8_t *W = a.w + layer * a.bw + (long)kb0 * 128 + fq * 16, *S = a.ws + layer * a.bws + (long)kb0 * a.ldws;
+    int n0 = (rbk * a.chunks * WAVES + w) * G * 16;      // first row of the wave's chunk; the next is WAVES * G * 16 further
 
-    // ---- weight stream: step s is row group s / nkb, block s % nkb
-    constexpr int U = 4;
-    uint4 q[U][2];
-    int sc[U];
-    int lg = 0, lk = 0;                                  // next step to request
-    auto request = [&](int u) {
-        const int row = min(n0 + lg * 16 + fr, a.N - 1);
-        const uint4* p = reinterpret_cast<const uint4*>(W + (long)row * a.ldw + lk * 128);
-        q[u][0] = p[0];
-        q[u][1] = p[1];
-        sc[u] = S[(long)lk * a.ldws + row];
-        if (++lk == nkb) { lk = 0; ++lg; }
-    };
+    uint4 q[D][G][2];
+    int sc[D][G];
+    const uint8_t* wrow[G];
+    int srow[G];
+    auto request = [&](int d, int kb) {
+        const int k = min(kb, nkb - 1);
 #pragma unroll
-    for (int u = 0; u < U; ++u) if (u < steps) request(u);
-
+        for (int g = 0; g < G; ++g) {
+            const uint4* p = reinterpret_cast<const uint4*>(wrow[g] + k * 128);
+            q[d][g][0] = p[0];                               // k = fq * 16 .. + 15 and 64 + fq * 16 ..: 64 contiguous bytes of a row per request
+            q[d][g][1] = p[4];
+            sc[d][g] = S[(long)k * a.ldws + srow[g]];
+        }
+    };
     // ---- pack the slice of x: 16 lanes a block of 128 of one token, 8 elements a lane
-    for (int id = tid >> 4; id < a.T * nkb; id += WAVES * 4) {
+    constexpr int P = 3;                                 // items a lane group has in flight (their latency is the block's start-up)
+    float xv0[P][8];
+    auto load_item = [&](int id, float* v) {
         const int t = id / nkb, kb = id - t * nkb, k = (kb0 + kb) * 128 + fr * 8;
-        float v[8];
         const long at = t * a.x_token + layer * a.x_layer + k;
         if (a.x_dtype == CLT_DT_F32) load_x8<CLT_DT_F32>(a.x, at, a.K - k, a.vec, v);
         else if (a.x_dtype == CLT_DT_BF16) load_x8<CLT_DT_BF16>(a.x, at, a.K - k, a.vec, v);
         else load_x8<CLT_DT_F16>(a.x, at, a.K - k, a.vec, v);
+    };
+    auto pack_item = [&](int id, const float* v) {
+        const int t = id / nkb, kb = id - t * nkb;
         uint32_t m = 0u;
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = max(m, finite_abs_bits(v[j]));
@@ -110,57 +112,96 @@ template <int MT, int FMT> __global__ __launch_bounds__(WAVES * 64) void rows8_k
         const float f = exp2_int(-e), g = exp2_int(e);
         const uint32_t lo = pack_codes<0>(v[0] * f, v[1] * f, v[2] * f, v[3] * f), hi = pack_codes<0>(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
         *reinterpret_cast<bf16x8*>(r8_smem + t * pitch + kb * 256 + fr * 16) = widen8<0>(lo, hi, g);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (LDS only: the weight requests stay in flight)
+    };
+    const int items = a.T * nkb, first = tid >> 4;
+    auto load_items = [&](int id) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) if (id + p * WAVES * 4 < items) load_item(id + p * WAVES * 4, xv0[p]);
+    };
+    load_items(first);                                   // (ahead of the weight requests: loads return in order)
 
     const unsigned char* xrow[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xrow[t] = r8_smem + min(t * 16 + fr, a.T - 1) * pitch + fq * 64;
-    f32x4 acc[MT];
+    for (int t = 0; t < MT; ++t) xrow[t] = r8_smem + min(t * 16 + fr, a.T - 1) * pitch + fq * 32;
+    for (int chunk = 0; chunk < a.chunks; ++chunk) {
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    int cg = 0, ck = 0;
-    for (int base = 0; base < steps; base += U) {
+        for (int g = 0; g < G; ++g) {
+            srow[g] = min(n0 + g * 16 + fr, a.N - 1);        // rows past the end: loaded, never stored
+            wrow[g] = W + (long)srow[g] * a.ldw;
+        }
+        f32x4 bv[G];                                         // (ahead of the requests too)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (base + u >= steps) break;
-            const uint32_t c[8] = {q[u][0].x, q[u][0].y, q[u][0].z, q[u][0].w, q[u][1].x, q[u][1].y, q[u][1].z, q[u][1].w};
-            const float s = __uint_as_float((uint32_t)sc[u] << 23);
-            bf16x8 h[4];
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = widen8<FMT>(c[2 * j], c[2 * j + 1], s);
-            if (base + u + U < steps) request(u);
+            for (int i = 0; i < 4; ++i) bv[g][i] = a.bias && !a.part ? a.bias[layer * a.bbias + min(n0 + g * 16 + fq * 4 + i, a.N - 1)] : 0.0f;
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+        for (int d = 0; d < D; ++d) request(d, d);
+        if (chunk == 0) {
+            for (int id = first; id < items; id += P * WAVES * 4) {
+                if (id != first) load_items(id);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h[j], *reinterpret_cast<const bf16x8*>(xrow[t] + ck * 256 + j * 16), acc[t], 0, 0, 0);
-            if (++ck == nkb) {                           // a row group is complete: row n0 + cg * 16 + fq * 4 + i of token fr
-                const int n = n0 + cg * 16 + fq * 4, valid = a.N - n;
+                for (int p = 0; p < P; ++p) if (id + p * WAVES * 4 < items) pack_item(id + p * WAVES * 4, xv0[p]);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (LDS only: the weight requests stay in flight)
+        }
+        f32x4 acc[G][MT];
 #pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    const int tok = t * 16 + fr;
-                    if (tok < a.T && valid > 0) {
-                        if (a.part) store_result(a.part, CLT_DT_F32, (((long)slice * (gridDim.x / a.row_blocks / a.slices) + layer) * a.T + tok) * a.N + n, acc[t], valid, valid >= 4 && a.N % 4 == 0);
-                        else {
-                            if (a.bias)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) if (i < valid) acc[t][i] += a.bias[layer * a.bbias + n + i];
-                            store_result(a.y, a.y_dtype, tok * a.y_token + layer * a.y_layer + n, acc[t], valid, valid >= 4 && a.y_vec);
-                        }
-                    }
-                    acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < MT; ++t) acc[g][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        auto product = [&](int d, int kb) {
+            float ws[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                int b = sc[d][g];
+                asm volatile("" : "+v"(b));                  // (the byte is not looked at, i.e. waited for, before its step)
+                ws[g] = __uint_as_float((uint32_t)b << 23);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                bf16x8 xv[MT];
+#pragma unroll
+                for (int t = 0; t < MT; ++t) xv[t] = *reinterpret_cast<const bf16x8*>(xrow[t] + kb * 256 + (j >> 1) * 128 + (j & 1) * 16);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const uint4 u = q[d][g][j >> 1];
+                    const bf16x8 h = widen8<FMT>(j & 1 ? u.z : u.x, j & 1 ? u.w : u.y, ws[g]);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) acc[g][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(h, xv[t], acc[g][t], 0, 0, 0);
                 }
-                ck = 0;
-                ++cg;
+            }
+        };
+        int kb = 0;
+        for (; kb + 2 * D <= nkb; kb += D) {                 // (no condition around a request: the compiler would wait for it at the join)
+#pragma unroll
+            for (int d = 0; d < D; ++d) { product(d, kb + d); request(d, kb + d + D); }
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (kb + d < nkb) product(d, kb + d);
+            if (kb + d + D < nkb) request(d, kb + d + D);
+        }
+#pragma unroll
+        for (int d = 0; d < D; ++d) if (kb + d + D < nkb) product(d, kb + d + D);
+        const int nc = n0;
+        n0 += WAVES * G * 16;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {                        // row nc + g * 16 + fq * 4 + i of token t * 16 + fr
+            const int n = nc + g * 16 + fq * 4, valid = a.N - n;
+            if (valid <= 0) continue;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int tok = t * 16 + fr;
+                if (tok >= a.T) continue;
+                if (a.part) store_result(a.part, CLT_DT_F32, (((long)slice * a.layers + layer) * a.T + tok) * a.N + n, acc[g][t], valid, valid >= 4 && a.N % 4 == 0);
+                else store_result(a.y, a.y_dtype, tok * a.y_token + layer * a.y_layer + n, acc[g][t] + bv[g], valid, valid >= 4 && a.y_vec);
             }
         }
     }
 }
 
 // partial sums of the slices -> results, slices in order
-__global__ __launch_bounds__(256) void rows8_fold_kernel(Rows8Args a, int layers, long n) {
+__global__ __launch_bounds__(256) void rows8_fold_kernel(Rows8Args a, long n) {
     const long i = (long)blockIdx.x * 256 + threadIdx.x;                 // (layer, token, column)
     if (i >= n) return;
     const long lt = i / a.N;
@@ -180,33 +221,36 @@ __global__ __launch_bounds__(256) void rows8_fold_kernel(Rows8Args a, int layers
     store_result(a.y, a.y_dtype, t * a.y_token + layer * a.y_layer + c, f32x4{s, 0.0f, 0.0f, 0.0f}, 1, false);
 }
 
-// How the work is cut: blocks of K per slice, slices, row groups per wave.  Rows first (no partial sums); K is cut where the
-// packed x does not fit LDS or where rows give less than two blocks a CU, down to 4 blocks of k a slice (a stream needs some
-// length); a wave takes more row groups as long as that leaves three blocks a CU (x is packed once per block).
-struct Cut { int slice_kb, slices, groups, row_blocks; };
+// How the work is cut: blocks of K per slice, slices, row groups in a wave's hand (G), chunks of rows per block.  Rows first (no
+// partial sums); K is cut where the packed x does not fit LDS or where rows give less than two blocks a CU, down to 16 blocks of
+// k a slice (the second launch costs about as much as a wave's 16 steps).  G grows while every CU keeps two blocks (x is read from
+// LDS once for G row groups); what is left over becomes chunks, so that x is packed once per resident block.
+struct Cut { int slice_kb, slices, g, chunks, row_blocks; };
 Cut cut_rows8(int T, int L, int N, int KB) {
     Cut c;
     const int fit = (LDS_CAP / T - 16) / 256;                            // blocks of k whose x fits LDS (>= 8 for 64 tokens)
-    const long rb = (N + WAVES * 16 - 1) / (WAVES * 16);
+    const long rb = (N + WAVES * 16 - 1) / (WAVES * 16), want = 512;
     long slices = (KB + fit - 1) / fit;
-    const long want = 512;
     if (L * rb * slices < want) {
-        const long by_grid = (want + L * rb - 1) / (L * rb), most = KB / 4 > 0 ? KB / 4 : 1;
+        const long by_grid = (want + L * rb - 1) / (L * rb), most = KB / 16 > 0 ? KB / 16 : 1;
         const long s = by_grid < most ? by_grid : most;
         if (s > slices) slices = s;
-        // cutting into two only pays when the stream is long: the second launch costs as much as ~16 steps
-        if (slices * 16 > KB && (KB + fit - 1) / fit == 1) slices = KB >= 32 ? KB / 16 : 1;
     }
     c.slice_kb = (int)((KB + slices - 1) / slices);
     c.slices = (KB + c.slice_kb - 1) / c.slice_kb;
-    long g = L * rb * c.slices / 768;
-    c.groups = (int)(g < 1 ? 1 : g > 16 ? 16 : g);
-    c.row_blocks = (int)((N + (long)WAVES * 16 * c.groups - 1) / ((long)WAVES * 16 * c.groups));
+    const long blocks = L * rb * c.slices;                               // at G = 1
+    const int most_g = T <= 16 ? 2 : 1;                                  // (two row groups and 32 tokens: one block per CU instead of two, 87 against 80 us)
+    c.g = 1;
+    while (c.g < most_g && blocks >= 2 * c.g * want) c.g *= 2;
+    const long rows = (long)WAVES * 16 * c.g, per_layer = (N + rows - 1) / rows;
+    c.chunks = (int)(L * per_layer * c.slices / 2048) + 1;
+    if (c.chunks > per_layer) c.chunks = (int)per_layer;
+    c.row_blocks = (int)((per_layer + c.chunks - 1) / c.chunks);
     return c;
 }
 
-template <int MT> int launch_rows(const Rows8Args& a, int fmt, long blocks, int lds, hipStream_t st) {
-    const auto f = fmt ? rows8_kernel<MT, 1> : rows8_kernel<MT, 0>;
+template <int MT, int G> int launch_rows(const Rows8Args& a, int fmt, long blocks, int lds, hipStream_t st) {
+    const auto f = fmt ? rows8_kernel<MT, G, 1> : rows8_kernel<MT, G, 0>;
     if (lds > 64 * 1024 && hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) return CLT_ERR_LAUNCH;
     f<<<dim3((unsigned)blocks), dim3(WAVES * 64), lds, st>>>(a);
     CLT_LAUNCH_CHECK();
@@ -239,19 +283,21 @@ extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride,
     a.bias = bias; a.bbias = bias_batch;
     a.y = y; a.y_token = y_token_stride; a.y_layer = y_layer_stride; a.y_dtype = y_dtype;
     a.part = c.slices > 1 ? static_cast<float*>(workspace) : nullptr;
-    a.T = tokens; a.N = N; a.K = K; a.KB = KB; a.slice_kb = c.slice_kb; a.slices = c.slices; a.groups = c.groups; a.row_blocks = c.row_blocks;
+    a.T = tokens; a.N = N; a.K = K; a.KB = KB; a.slice_kb = c.slice_kb; a.slices = c.slices; a.chunks = c.chunks; a.row_blocks = c.row_blocks; a.layers = layers;
     a.vec = aligned16(x) && x_token_stride % (long)(16 / xs) == 0 && x_layer_stride % (long)(16 / xs) == 0;
     a.y_vec = (uintptr_t)y % (4 * ys) == 0 && y_token_stride % 4 == 0 && y_layer_stride % 4 == 0;
     const long blocks = (long)layers * c.slices * c.row_blocks;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
     const int lds = tokens * (c.slice_kb * 256 + 16);
     const hipStream_t st = as_stream(stream);
-    const int rc = tokens <= 16 ? launch_rows<1>(a, w_format, blocks, lds, st) : tokens <= 32 ? launch_rows<2>(a, w_format, blocks, lds, st)
-                                                                                              : launch_rows<4>(a, w_format, blocks, lds, st);
+    int rc;
+    if (tokens <= 16) rc = c.g == 1 ? launch_rows<1, 1>(a, w_format, blocks, lds, st) : launch_rows<1, 2>(a, w_format, blocks, lds, st);
+    else if (tokens <= 32) rc = launch_rows<2, 1>(a, w_format, blocks, lds, st);
+    else rc = launch_rows<4, 1>(a, w_format, blocks, lds, st);
     if (rc != CLT_OK || c.slices == 1) return rc;
     const long n = (long)layers * tokens * N, fold = (n + 255) / 256;
     if (fold > 0x7fffffffL) return CLT_ERR_RANGE;
-    rows8_fold_kernel<<<dim3((unsigned)fold), dim3(256), 0, st>>>(a, layers, n);
+    rows8_fold_kernel<<<dim3((unsigned)fold), dim3(256), 0, st>>>(a, n);
     CLT_LAUNCH_CHECK();
     return CLT_OK;
 }

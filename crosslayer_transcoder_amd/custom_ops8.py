@@ -31,20 +31,40 @@ def _form_shapes(L, rows, cols):
 
 
 # ---- one linear map per layer: the encoder (W [L, N, K] in memory) and the per-layer decoder (W [L, K, N]) -----------------
-@torch.library.custom_op("clt_hip::linear8", mutates_args=(), device_types=_DEV)
-def linear8(x: Tensor, W: Tensor, b: Optional[Tensor], kn: bool, keep_x: bool, keep_w: bool) -> List[Tensor]:
-    """x [T, L, K], W [L, N, K] (kn: [L, K, N]) -> [y [T, L, N], kept x (codes, scale bytes), kept W (codes, scale bytes)];
-    the kept tensors are empty where keep_x / keep_w is false."""
+def _forward(x, W, b, kn, keep_x, keep_w):
+    """-> y [T, L, N], kept x (codes, scale bytes), kept W (codes, scale bytes); None where not kept."""
     T, L, K = x.shape
     N = W.shape[2] if kn else W.shape[1]
-    x3 = ops8._dense(x).transpose(0, 1)
-    q, s, xt, xs, _ = ops8.pack8_raw(x3, _E4M3, True, keep_x)
+    q, s, xt, xs, _ = ops8.pack8_raw(ops8._dense(x).transpose(0, 1), _E4M3, True, keep_x)
     # the contraction over K reads the [N, K] form, the input gradient the [K, N] form
     d, ds, t, ts, _ = ops8.pack8_raw(ops8._dense(W), _E4M3, keep_w or not kn, keep_w or kn, tiles=True)
     (f, fs), (g, gs) = ((t, ts), (d, ds)) if kn else ((d, ds), (t, ts))
     y = torch.empty((T, L, N), dtype=x.dtype, device=x.device)
     gemm8(Block8(q, s, T, K), Block8(f, fs, N, K), b, out=y.transpose(0, 1))
-    return [y, xt if keep_x else _u8(x, 0), xs if keep_x else _u8(x, 0), g if keep_w else _u8(x, 0), gs if keep_w else _u8(x, 0)]
+    return y, xt, xs, (g if keep_w else None), (gs if keep_w else None)
+
+
+def _gradients(dy, xt, xs, w, ws, K, kn, need_dx, w_dtype, need_db):
+    """-> dx [T, L, K], dW (shape of W), db fp32 [L, N]; None where not asked for (w_dtype None: no dW)."""
+    T, L, N = dy.shape
+    need_dw = w_dtype is not None
+    # (the bias gradient rides along with a pack; alone it still takes one)
+    q, s, qt, st, db = ops8.pack8_raw(ops8._dense(dy).transpose(0, 1), _E4M3, need_dx or not need_dw, need_dw, sums=need_db)
+    dx = dW = None
+    if need_dx:
+        dx = torch.empty((T, L, K), dtype=dy.dtype, device=dy.device)
+        gemm8(Block8(q, s, T, N), Block8(w, ws, K, N), out=dx.transpose(0, 1))
+    if need_dw:
+        xk, gk = Block8(xt, xs, K, T), Block8(qt, st, N, T)
+        dW = gemm8(xk, gk, out_dtype=w_dtype) if kn else gemm8(gk, xk, out_dtype=w_dtype)
+    return dx, dW, db
+
+
+@torch.library.custom_op("clt_hip::linear8", mutates_args=(), device_types=_DEV)
+def linear8(x: Tensor, W: Tensor, b: Optional[Tensor], kn: bool, keep_x: bool, keep_w: bool) -> List[Tensor]:
+    """x [T, L, K], W [L, N, K] (kn: [L, K, N]) -> [y [T, L, N], kept x (codes, scale bytes), kept W (codes, scale bytes)];
+    the kept tensors are empty where keep_x / keep_w is false."""
+    return [_u8(x, 0) if t is None else t for t in _forward(x, W, b, kn, keep_x, keep_w)]
 
 
 @linear8.register_fake
@@ -60,19 +80,7 @@ def _(x, W, b, kn, keep_x, keep_w):
 def linear8_bwd(dy: Tensor, xt: Tensor, xs: Tensor, w: Tensor, ws: Tensor, K: int, kn: bool, need_dx: bool, w_dtype: Optional[torch.dtype],
                 need_db: bool) -> List[Tensor]:
     """-> [dx [T, L, K], dW (shape of W), db fp32 [L, N]], empty where not asked for (w_dtype None: no dW)."""
-    T, L, N = dy.shape
-    need_dw = w_dtype is not None
-    g3 = ops8._dense(dy).transpose(0, 1)
-    # (the bias gradient rides along with a pack; alone it still takes one)
-    q, s, qt, st, db = ops8.pack8_raw(g3, _E4M3, need_dx or not need_dw, need_dw, sums=need_db)
-    dx, dW = dy.new_empty(0), dy.new_empty(0)
-    if need_dx:
-        dx = torch.empty((T, L, K), dtype=dy.dtype, device=dy.device)
-        gemm8(Block8(q, s, T, N), Block8(w, ws, K, N), out=dx.transpose(0, 1))
-    if need_dw:
-        xk, gk = Block8(xt, xs, K, T), Block8(qt, st, N, T)
-        dW = gemm8(xk, gk, out_dtype=w_dtype) if kn else gemm8(gk, xk, out_dtype=w_dtype)
-    return [dx, dW, db if need_db else dy.new_empty(0)]
+    return [dy.new_empty(0) if t is None else t for t in _gradients(dy, xt, xs, w, ws, K, kn, need_dx, w_dtype, need_db)]
 
 
 @linear8_bwd.register_fake
@@ -101,11 +109,32 @@ def _backward(ctx, grads):
 linear8.register_autograd(_backward, setup_context=_setup)
 
 
+class _Linear8(torch.autograd.Function):
+    """The same two functions without the dispatcher's Python layers, for eager calls (a forward and backward of a few tokens:
+    400 us of host time through the registered ops)."""
+
+    @staticmethod
+    def forward(ctx, x, W, b, kn):
+        y, *kept = _forward(x, W, b, kn, ctx.needs_input_grad[1], ctx.needs_input_grad[0])
+        ctx.save_for_backward(*kept)
+        ctx.kn, ctx.K, ctx.w_dtype, ctx.b = kn, x.shape[2], W.dtype, None if b is None else (b.dtype, b.shape)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx, dW, db = _gradients(dy, *ctx.saved_tensors, ctx.K, ctx.kn, need_x, ctx.w_dtype if need_w else None, need_b)
+        return dx, dW, db.to(ctx.b[0]).reshape(ctx.b[1]) if need_b else None, None
+
+
 def _linear(x, W, b, kn):
     if x.dim() != 3 or W.dim() != 3 or W.shape[0] != x.shape[1] or W.shape[1 if kn else 2] != x.shape[2]:
         raise ValueError(f"x {tuple(x.shape)} ([tokens, layers, features]) does not match W {tuple(W.shape)}")
-    grad = torch.is_grad_enabled()
-    return torch.ops.clt_hip.linear8(x, W, b, kn, grad and W.requires_grad, grad and x.requires_grad)[0]
+    if torch.compiler.is_compiling():
+        grad = torch.is_grad_enabled()
+        return torch.ops.clt_hip.linear8(x, W, b, kn, grad and W.requires_grad, grad and x.requires_grad)[0]
+    return _Linear8.apply(x, W, b, kn)
 
 
 def encoder8(xs: Tensor, W: Tensor, b: Optional[Tensor]) -> Tensor:

@@ -25,19 +25,22 @@ def _up(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK * BLOCK
 
 
-def _call(name, *args):
-    rc = getattr(lib, name)(*args)
+def _call(fn, *args):
+    rc = fn(*args)
     if rc:
-        raise CltError(name, rc)
+        raise CltError(fn.__name__, rc)
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(device):
     """The tensors' device made current for a launch (a no-op when it is already)."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _fmt(fmt: str) -> int:
@@ -129,7 +132,7 @@ def pack8_raw(x: torch.Tensor, fmt: int, along: bool, across: bool, tiles: bool 
         ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
         cs = torch.empty((L, C), dtype=torch.float32, device=x.device)
     with _on(x.device):
-        _call("clt_pack8", x.data_ptr(), _DT[x.dtype], x.stride(1), x.stride(0), L, R, C, fmt, int(tiles),
+        _call(lib.clt_pack8, x.data_ptr(), _DT[x.dtype], x.stride(1), x.stride(0), L, R, C, fmt, int(tiles),
               q.data_ptr() if along else None, s.data_ptr() if along else None, qt.data_ptr() if across else None,
               st.data_ptr() if across else None, cs.data_ptr() if sums else None, ws.data_ptr() if sums else None, nws, _stream(x.device))
     return q, s, qt, st, cs
@@ -176,7 +179,7 @@ def dequantize8(q: Block8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     out = torch.empty((q.batch, q.rows, q.cols), dtype=dtype, device=q.device)
     if out.numel():
         with _on(q.device):
-            _call("clt_unpack8", q.data.data_ptr(), q.scale.data_ptr(), FORMATS[q.fmt], q.batch, q.rows, q.cols, q.data.stride(1),
+            _call(lib.clt_unpack8, q.data.data_ptr(), q.scale.data_ptr(), FORMATS[q.fmt], q.batch, q.rows, q.cols, q.data.stride(1),
                   q.scale.stride(1), q.data.stride(0), q.scale.stride(0), out.data_ptr(), _DT[dtype], _stream(q.device))
     return out
 
@@ -220,7 +223,7 @@ def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: 
     bias = _bias(bias, L, N, a.device)
     if out.numel():
         with _on(a.device):
-            _call("clt_gemm8", a.data.data_ptr(), a.scale.data_ptr(), FORMATS[a.fmt], a.data.stride(1), a.scale.stride(1),
+            _call(lib.clt_gemm8, a.data.data_ptr(), a.scale.data_ptr(), FORMATS[a.fmt], a.data.stride(1), a.scale.stride(1),
                   a.data.stride(0), a.scale.stride(0), b.data.data_ptr(), b.scale.data_ptr(), FORMATS[b.fmt], b.data.stride(1),
                   b.scale.stride(1), b.data.stride(0), b.scale.stride(0), out.data_ptr(), _DT[out.dtype], out.stride(1) if M > 1 else N,
                   out.stride(0), bias.data_ptr() if bias is not None else None, N, M, N, K, L, int(accumulate), _stream(a.device))
@@ -248,7 +251,7 @@ def linear8(x: torch.Tensor, w: Block8, bias: Optional[torch.Tensor] = None, out
         nws = lib.clt_linear8_rows_workspace_bytes(T, L, N, K)
         ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
         with _on(x.device):
-            _call("clt_linear8_rows", x.data_ptr(), _DT[x.dtype], x.stride(0), x.stride(1), w.data.data_ptr(), w.scale.data_ptr(),
+            _call(lib.clt_linear8_rows, x.data_ptr(), _DT[x.dtype], x.stride(0), x.stride(1), w.data.data_ptr(), w.scale.data_ptr(),
                   FORMATS[w.fmt], w.data.stride(1), w.scale.stride(1), w.data.stride(0), w.scale.stride(0),
                   bias.data_ptr() if bias is not None else None, N, y.data_ptr(), _DT[dt], L * N, N, T, L, N, K,
                   ws.data_ptr() if nws else None, nws, _stream(x.device))

@@ -565,3 +565,18 @@ def test_refusals_of_the_training_ops():
         C.encoder8(torch.zeros(4, 2, 8), torch.zeros(3, 8, 3), None)
     with pytest.raises(ValueError):
         C.encoder8(torch.zeros(4, 8), torch.zeros(2, 8, 3), None)
+
+
+@gpu
+def test_registered_op_equals_the_eager_function():
+    """The dispatcher op (what torch.compile captures) and the eager autograd function give the same bits, forward and backward."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    x, W, b = (rnd(*s, seed=i, spread=False).requires_grad_() for i, s in enumerate(((40, 2, 130), (2, 130, 70), (2, 70))))
+    dy = rnd(40, 2, 70, seed=9, spread=False)
+    y = C.plt_decoder8(x, W, b)
+    z = torch.ops.clt_hip.linear8(x, W, b, True, True, True)[0]
+    assert torch.equal(y, z)
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(y, (x, W, b), dy), torch.autograd.grad(z, (x, W, b), dy)))
+    c = torch.compile(lambda *t: C.plt_decoder8(*t), backend="aot_eager")(x, W, b)
+    assert torch.equal(c, y)
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(c, (x, W, b), dy), torch.autograd.grad(C.plt_decoder8(x, W, b), (x, W, b), dy)))
