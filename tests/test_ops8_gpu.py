@@ -411,7 +411,7 @@ def test_only_what_is_needed_is_kept():
     from crosslayer_transcoder_amd import custom_ops8 as C
     x, W, b = rnd(256, 2, 512, seed=1), rnd(2, 512, 128, seed=2), None
     out = torch.ops.clt_hip.linear8(x, W, b, True, True, False)
-    assert sum(t.numel() for t in out[1:]) == x.numel() + x.numel() // 128 and out[3].numel() == 0
+    assert out[1].numel() == x.numel() + x.numel() // 128
     for nx, nw in ((True, False), (False, True)):
         xi, Wi = x.clone().requires_grad_(nx), W.clone().requires_grad_(nw)
         C.plt_decoder8(xi, Wi, b).sum().backward()                                # (an expanded incoming gradient)
@@ -437,8 +437,8 @@ def test_opcheck():
     x, b = rnd(9, 2, 40, seed=1, spread=False).requires_grad_(), rnd(2, 30, seed=2, spread=False).requires_grad_()
     W = rnd(2, 40, 30, seed=3, spread=False).requires_grad_()
     cases = {"linear8": (x, W, b, True, True, True)}
-    kept = torch.ops.clt_hip.linear8(x.detach(), W.detach(), b.detach(), True, True, True)[1:]
-    cases["linear8_bwd"] = (rnd(9, 2, 30, seed=4, spread=False), *kept, 40, True, True, torch.float32, True)
+    kept = torch.ops.clt_hip.linear8(x.detach(), W.detach(), b.detach(), True, True, True)[1]
+    cases["linear8_bwd"] = (rnd(9, 2, 30, seed=4, spread=False), kept, 40, True, True, True, torch.float32, True)
     assert set(cases) == set(C.REGISTERED8)
     for name, args in cases.items():
         torch.library.opcheck(getattr(torch.ops.clt_hip, name).default, args)
