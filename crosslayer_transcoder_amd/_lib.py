@@ -110,7 +110,8 @@ SIGNATURES = {
     "clt_pack8_sums_workspace_bytes": (SZ, [I, I, I]),
     "clt_pack8": (I, [P, I, L, L, I, I, I, I, I, P, P, P, P, P, P, SZ, P]),
     "clt_unpack8": (I, [P, P, I, I, I, I, L, L, L, L, P, I, P]),
-    "clt_gemm8": (I, [P, P, I, L, L, L, L, P, P, I, L, L, L, L, P, I, L, L, P, L, I, I, I, I, I, P]),
+    "clt_gemm8_workspace_bytes": (SZ, [I, I, I, I]),
+    "clt_gemm8": (I, [P, P, I, L, L, L, L, P, P, I, L, L, L, L, P, I, L, L, P, L, I, I, I, I, I, P, SZ, P]),
     "clt_linear8_rows_workspace_bytes": (SZ, [I, I, I, I]),
     "clt_linear8_rows": (I, [P, I, L, L, P, P, I, L, L, L, L, P, L, P, I, L, L, I, I, I, I, P, SZ, P]),
 }

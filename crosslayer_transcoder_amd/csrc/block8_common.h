@@ -78,11 +78,31 @@ struct Gemm8Args {
     long lda, ldas, ldb, ldbs, ldc;          // pitches: code rows, scale-byte rows (one per block of 128), C rows
     long ba, bas, bb, bbs, bc, bbias;        // batch strides
     int M, N, KB, tilesA, tilesB;
-    int accumulate;
+    int accumulate, batch;
+    int slices, slice_kb; float* part;       // K in slices: partial sums [slice][batch][M][N], else nullptr
 };
 
-// 256 x 256 tiles; returns 1 where the shape is the small tiles' (gemm8_large.hip)
-int clt_internal_gemm8_large(const Gemm8Args& g, int fa, int fb, int dtype, int batch, hipStream_t st);
+// 256 x 256 tiles (gemm8_large.hip): the shapes that take them, and the launch
+bool clt_internal_gemm8_large_applies(int M, int N, int KB, int batch);
+int clt_internal_gemm8_large(const Gemm8Args& g, int fa, int fb, int dtype, hipStream_t st);
+
+// Four consecutive columns of a row of C: one store where the row's alignment allows it (vec), else element by element
+template <int DT> __device__ __forceinline__ void b8_store4(void* c, long at, b8_f32x4 v, int valid, bool vec, int accumulate) {
+    typename Elem<DT>::type* p = static_cast<typename Elem<DT>::type*>(c) + at;
+    if constexpr (DT == CLT_DT_F32) {
+        if (vec && valid >= 4) {
+            b8_f32x4* q = reinterpret_cast<b8_f32x4*>(p);
+            *q = accumulate ? *q + v : v;
+        } else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i < valid) p[i] = accumulate ? p[i] + v[i] : v[i];
+    } else {
+        if (vec && valid >= 4) *reinterpret_cast<uint2*>(p) = make_uint2(pack_out16<DT>(v[0], v[1]), pack_out16<DT>(v[2], v[3]));
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i < valid) p[i] = f32_to_elem<DT>(v[i]);
+    }
+}
 
 // eight codes (two dwords) x 2^e -> eight bf16
 template <int FMT> __device__ __forceinline__ b8_bf16x8 widen8(uint32_t lo, uint32_t hi, float scale) {

@@ -9,114 +9,111 @@
 //     the alignment loss is far below the result's own rounding (2^-9 bf16, 2^-12 fp16).
 //   32-bit results: the codes become bf16 in registers (2^e x code is exact in bf16) and go through v_mfma_f32_16x16x32_bf16:
 //     exact products, fp32 sums, at the 16-bit rate.
-// B rows ride the instruction's "M" index and A rows its "N" index, so a lane's four accumulators are four consecutive columns
-// of one row of C.
+// B rows ride the instruction's "M" index and A rows its "N" index, so a lane's accumulators are consecutive columns of a row of C.
+//
+// This file: the entry point and the form for everything that does not fill the chip with 256 x 256 tiles (gemm8_large.hip): 128 x 128
+// tiles, K cut into slices where tiles are few (partial sums in fp32, added in order by a second launch).
 #include "block8_common.h"
 
 namespace {
 typedef b8_f32x4 f32x4;
+typedef b8_i32x8 i32x8;
+typedef b8_bf16x8 bf16x8;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
 
-// Four consecutive columns of a row of C: 16- or 8-byte store where the row's alignment allows it (vec), else element by element
-template <int DT> __device__ __forceinline__ void store4(void* c, long at, f32x4 v, int valid, bool vec, int accumulate) {
-    typename Elem<DT>::type* p = static_cast<typename Elem<DT>::type*>(c) + at;
-    if constexpr (DT == CLT_DT_F32) {
-        if (vec && valid >= 4) {
-            f32x4* q = reinterpret_cast<f32x4*>(p);
-            *q = accumulate ? *q + v : v;
-        } else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if (i < valid) p[i] = accumulate ? p[i] + v[i] : v[i];
-    } else {
-        if (vec && valid >= 4) *reinterpret_cast<uint2*>(p) = make_uint2(pack_out16<DT>(v[0], v[1]), pack_out16<DT>(v[2], v[3]));
-        else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if (i < valid) p[i] = f32_to_elem<DT>(v[i]);
-    }
-}
+// One block of 4 waves of 64 x 64.  Blocks of k (16 KB of A, 16 KB of B, their scale bytes) arrive by DMA in a ring of four LDS
+// buffers, three ahead; a block's fragments are read while the previous block's products run, one barrier a block.
+// LDS rows of 128 bytes, 16-byte chunks XOR-swizzled with bits 1..3 of the row.  Row p of a 64-row half is matrix row
+// (p % 16) * 4 + p / 16 (A) or c(p % 16) * 4 + p / 16 (B, c(4 q + i) = 4 i + q): a lane's four fragments are four consecutive rows,
+// so their scales are one dword, and its accumulators of the four B fragments are four consecutive columns.
+// Per block of k: 64 instruction slots of 8 cycles against 96 KB through LDS (768 cycles).  Measured: see DEPTH below.
+constexpr int OPB = 128 * 128, STG = 2 * OPB + 512, DEPTH = 4;
+constexpr int PIECES = 9;                            // DMA instructions of a wave per block of k
+extern __shared__ __attribute__((aligned(1024))) unsigned char t8_smem[];
 
-// 128 x 128 tile, 4 waves of 64 x 64, one k-block (128 bytes a row) staged through registers into LDS while the next is loaded.
-// LDS rows are 128 bytes whose 16-byte chunks are XOR-swizzled with bits 1..3 of the row (conflict-free fragment reads).
-template <int DT, int FA, int FB> __global__ __launch_bounds__(256) void gemm8_kernel(Gemm8Args g) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 128 * 128];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, fr = lane & 15, fq = lane >> 4;
+template <int DT, int FA, int FB> __global__ __launch_bounds__(256, 1) void gemm8_kernel(Gemm8Args g) {
+    constexpr bool WIDE = DT == CLT_DT_F32;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
     const int wb = w >> 1, wa = w & 1;
-    const long per = (long)g.tilesA * g.tilesB, batch = blockIdx.x / per;
-    const int t = (int)(blockIdx.x - batch * per), ta = t % g.tilesA, tb = t / g.tilesA;
-    const int a0 = ta * 128, b0 = tb * 128;
-    const uint8_t *A = g.a + batch * g.ba, *B = g.b + batch * g.bb, *As = g.as + batch * g.bas, *Bs = g.bs + batch * g.bbs;
+    const int nwg = g.tilesA * g.tilesB;
+    int id = blockIdx.x;
+    const int tile = id % nwg;
+    id /= nwg;
+    const int slice = id % g.slices, batch = id / g.slices;
+    const int a0 = tile % g.tilesA * 128, b0 = tile / g.tilesA * 128;
+    const int k0 = slice * g.slice_kb, nk = min(g.slice_kb, g.KB - k0);
 
-    const uint8_t *pa[4], *pb[4];
-    int at[4];
+    // DMA: piece i of wave w fills LDS rows (4 i + w) * 8 .. + 7 of an operand.  Ranges end behind the tile's last row: rows past the
+    // matrix arrive as zeros (the range check counts the scalar offset, here the block of k, too).
+    auto rsrc = [](const void* p, long records) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)records, 0x00020000); };
+    __amdgpu_buffer_rsrc_t rA = rsrc(g.a + batch * g.ba + (long)a0 * g.lda, (long)min(g.M - a0, 128) * g.lda);
+    __amdgpu_buffer_rsrc_t rB = rsrc(g.b + batch * g.bb + (long)b0 * g.ldb, (long)min(g.N - b0, 128) * g.ldb);
+    const int srow = (int)(w & 1 ? g.ldbs : g.ldas);     // even waves bring A's scale bytes, odd waves B's
+    __amdgpu_buffer_rsrc_t rS = rsrc(w & 1 ? g.bs + batch * g.bbs + b0 : g.as + batch * g.bas + a0,
+                                     (long)(g.KB - 1) * srow + min(((w & 1 ? g.N - b0 : g.M - a0) + 3) & ~3, 128));
+    const __amdgpu_buffer_rsrc_t none = rsrc(g.a, 0);
+    const int q8 = (w & 1) * 8 + (lane >> 3), ch = (lane & 7) ^ ((q8 >> 1) & 7);
+    const int vA = (q8 * 4 + (w >> 1)) * (int)g.lda + ch * 16;
+    const int vB = ((((q8 & 3) << 2) | (q8 >> 2)) * 4 + (w >> 1)) * (int)g.ldb + ch * 16;
+    auto stage = [&](int k) {                            // block k of the slice (behind the end: nothing, zeros arrive)
+        unsigned char* base = t8_smem + (k & (DEPTH - 1)) * STG;
+        const bool live = k < nk;
+        const __amdgpu_buffer_rsrc_t pa = live ? rA : none, pb = live ? rB : none, ps = live ? rS : none;
+        const int kb = k0 + k;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int id = i * 256 + tid, row = id >> 3, ch = id & 7;
-        pa[i] = A + (long)min(a0 + row, g.M - 1) * g.lda + ch * 16;          // rows past the edge: loaded, never stored
-        pb[i] = B + (long)min(b0 + row, g.N - 1) * g.ldb + ch * 16;
-        at[i] = row * 128 + ((ch ^ ((row >> 1) & 7)) << 4);
-    }
-    int ra[4], rb[4];
+        for (int i = 0; i < 4; ++i) {
+            const int rows = (i & 1) * 2 + (i >> 1) * 64;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(pa, (lds_void*)(base + (i * 4 + w) * 1024), 16, vA + rows * (int)g.lda, kb * 128, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(pb, (lds_void*)(base + OPB + (i * 4 + w) * 1024), 16, vB + rows * (int)g.ldb, kb * 128, 0, 0);
+        }
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(ps, (lds_void*)(base + 2 * OPB + (w & 1) * 256), 4, lane * 4, kb * srow, 0, 0);
+    };
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        ra[n] = min(a0 + wa * 64 + n * 16 + fr, g.M - 1);
-        rb[n] = min(b0 + wb * 64 + n * 16 + fr, g.N - 1);
-    }
+    for (int k = 0; k < DEPTH; ++k) stage(k);
+
     f32x4 acc[4][4];
 #pragma unroll
     for (int m = 0; m < 4; ++m)
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    uint4 va[4], vb[4];
-    int sa[4], sb[4];
-    auto load = [&](int kb) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            va[i] = *reinterpret_cast<const uint4*>(pa[i] + (long)kb * 128);
-            vb[i] = *reinterpret_cast<const uint4*>(pb[i] + (long)kb * 128);
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) { sa[n] = As[kb * g.ldas + ra[n]]; sb[n] = Bs[kb * g.ldbs + rb[n]]; }
+    const int x = fr >> 1, lo = (fq ^ x) << 4;
+    const int rowA = (wa * 64 + fr) * 128, rowB = OPB + (wb * 64 + fr) * 128;
+    const int scA = 2 * OPB + wa * 64 + fr * 4, scB = 2 * OPB + 256 + wb * 64 + (((fr & 3) << 2) | (fr >> 2)) * 4;
+    i32x8 fa[2][4], fb[2][4];
+    int sa[2], sb[2];
+    auto ld = [&](const unsigned char* p) {              // chunks fq and fq + 4: any split of the block's k that both operands share
+        const i32x4 u = *reinterpret_cast<const i32x4*>(p + lo), v = *reinterpret_cast<const i32x4*>(p + (lo ^ 64));
+        return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    if (g.KB > 0) load(0);
-    for (int kb = 0; kb < g.KB; ++kb) {
-        __syncthreads();                                   // every wave has read the previous block
+    auto fragments = [&](int k, int s) {
+        const unsigned char* base = t8_smem + (k & (DEPTH - 1)) * STG;
+        sa[s] = *reinterpret_cast<const int*>(base + scA);
+        sb[s] = *reinterpret_cast<const int*>(base + scB);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            *reinterpret_cast<uint4*>(lds + at[i]) = va[i];
-            *reinterpret_cast<uint4*>(lds + 16384 + at[i]) = vb[i];
-        }
-        int ca[4], cb[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) { ca[n] = sa[n]; cb[n] = sb[n]; }
-        if (kb + 1 < g.KB) load(kb + 1);
-        __syncthreads();
-        // a lane's 32 codes of a row: 16-byte chunks fq and fq + 4 (the same k for both operands; the order inside a block is free)
-        b8_i32x8 fa[4], fb[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int x = fr >> 1, rowa = (wa * 64 + n * 16 + fr) * 128, rowb = 16384 + (wb * 64 + n * 16 + fr) * 128;
-            const int4 a_lo = *reinterpret_cast<const int4*>(lds + rowa + ((fq ^ x) << 4)), a_hi = *reinterpret_cast<const int4*>(lds + rowa + (((fq + 4) ^ x) << 4));
-            const int4 b_lo = *reinterpret_cast<const int4*>(lds + rowb + ((fq ^ x) << 4)), b_hi = *reinterpret_cast<const int4*>(lds + rowb + (((fq + 4) ^ x) << 4));
-            fa[n] = b8_i32x8{a_lo.x, a_lo.y, a_lo.z, a_lo.w, a_hi.x, a_hi.y, a_hi.z, a_hi.w};
-            fb[n] = b8_i32x8{b_lo.x, b_lo.y, b_lo.z, b_lo.w, b_hi.x, b_hi.y, b_hi.z, b_hi.w};
-        }
-        if constexpr (DT != CLT_DT_F32) {
-#pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[m], fa[n], acc[m][n], FB, FA, 0, cb[m], 0, ca[n]);
+        for (int n = 0; n < 4; ++n) { fa[s][n] = ld(base + rowA + n * 2048); fb[s][n] = ld(base + rowB + n * 2048); }
+    };
+    auto products = [&](int s) {
+        if constexpr (!WIDE) {
+#define G8_MFMA(M_, N_) acc[M_][N_] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[s][M_], fa[s][N_], acc[M_][N_], FB, FA, M_, sb[s], N_, sa[s]);
+#define G8_ROW(M_) G8_MFMA(M_, 0) G8_MFMA(M_, 1) G8_MFMA(M_, 2) G8_MFMA(M_, 3)
+            G8_ROW(0) G8_ROW(1) G8_ROW(2) G8_ROW(3)
+#undef G8_ROW
+#undef G8_MFMA
         } else {
             float xa[4], xb[4];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) { xa[n] = exp2_int(ca[n] - 127); xb[n] = exp2_int(cb[n] - 127); }
+            for (int n = 0; n < 4; ++n) {
+                xa[n] = __uint_as_float((((uint32_t)sa[s] >> (8 * n)) & 0xffu) << 23);
+                xb[n] = __uint_as_float((((uint32_t)sb[s] >> (8 * n)) & 0xffu) << 23);
+            }
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                b8_bf16x8 ha[4], hb[4];
+            for (int j = 0; j < 4; ++j) {
+                bf16x8 ha[4], hb[4];
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
-                    ha[n] = widen8<FA>((uint32_t)fa[n][2 * s], (uint32_t)fa[n][2 * s + 1], xa[n]);
-                    hb[n] = widen8<FB>((uint32_t)fb[n][2 * s], (uint32_t)fb[n][2 * s + 1], xb[n]);
+                    ha[n] = widen8<FA>((uint32_t)fa[s][n][2 * j], (uint32_t)fa[s][n][2 * j + 1], xa[n]);
+                    hb[n] = widen8<FB>((uint32_t)fb[s][n][2 * j], (uint32_t)fb[s][n][2 * j + 1], xb[n]);
                 }
 #pragma unroll
                 for (int m = 0; m < 4; ++m)
@@ -124,54 +121,147 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256) void gemm8_k
                     for (int n = 0; n < 4; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb[m], ha[n], acc[m][n], 0, 0, 0);
             }
         }
+    };
+    // this wave's pieces of the next block have landed (the two blocks behind it may be on their way) and its reads are complete
+#define G8_NEXT() asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(2 * PIECES) : "memory")
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(3 * PIECES) : "memory");
+    fragments(0, 0);
+    int k = 0;
+    for (; k + 1 < nk; k += 2) {
+        G8_NEXT();
+        fragments(k + 1, 1);
+        stage(k + DEPTH);
+        products(0);
+        G8_NEXT();
+        fragments(k + 2, 0);
+        stage(k + 1 + DEPTH);
+        products(1);
     }
-    constexpr int VEC = 4;
-    const size_t es = DT == CLT_DT_F32 ? 4 : 2;
-    const bool vec = ((uintptr_t)g.c % (VEC * es)) == 0 && g.ldc % VEC == 0 && g.bc % VEC == 0;
-    const float* bias = g.bias ? g.bias + batch * g.bbias : nullptr;
+    if (k < nk) products(0);
+#undef G8_NEXT
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no DMA into this block's LDS outlives it
+
+    // for (n, i) a lane has row 4 fr + n and four columns 4 (4 i + fq) ..
+    const bool part = g.part != nullptr;
+    const float* bias = g.bias && !part ? g.bias + batch * g.bbias : nullptr;
+    const int ldc_part = g.N;
+    const bool vec = part ? g.N % 4 == 0 : ((uintptr_t)g.c % (WIDE ? 16 : 8)) == 0 && g.ldc % 4 == 0 && g.bc % 4 == 0;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        const int col = b0 + wb * 64 + m * 16 + fq * 4, valid = g.N - col;
+    for (int i = 0; i < 4; ++i) {
+        const int col = b0 + wb * 64 + (i * 4 + fq) * 4, valid = g.N - col;
         f32x4 bv = {0.0f, 0.0f, 0.0f, 0.0f};
         if (bias)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) if (i < valid) bv[i] = bias[col + i];
+            for (int j = 0; j < 4; ++j) bv[j] = bias[min(col + j, g.N - 1)];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            const int row = a0 + wa * 64 + n * 16 + fr;
-            if (row < g.M && valid > 0) store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, acc[m][n] + bv, valid, vec, g.accumulate);
+            const int row = a0 + wa * 64 + fr * 4 + n;
+            if (row >= g.M || valid <= 0) continue;
+            const f32x4 v = f32x4{acc[0][n][i], acc[1][n][i], acc[2][n][i], acc[3][n][i]} + bv;
+            if (part) b8_store4<CLT_DT_F32>(g.part, (((long)slice * g.batch + batch) * g.M + row) * ldc_part + col, v, valid, vec, 0);
+            else b8_store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, v, valid, vec, g.accumulate);
         }
     }
 }
 
+// partial sums of the slices -> C, slices in order; four columns a thread
+template <int DT> __global__ __launch_bounds__(256) void gemm8_fold_kernel(Gemm8Args g, int quads, long total) {
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    if (id >= total) return;
+    const long r = id / quads;                           // row of the whole batch
+    const int col = (int)(id - r * quads) * 4, valid = g.N - col, batch = (int)(r / g.M), row = (int)(r - (long)batch * g.M);
+    const long step = (long)g.batch * g.M * g.N;
+    const float* p = g.part + r * g.N + col;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (valid >= 4 && g.N % 4 == 0) {
+        int k = 0;
+        for (; k + 4 <= g.slices; k += 4) {              // four requests at a time, added in order
+            f32x4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4*>(p + (k + j) * step);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += v[j];
+        }
+        for (; k < g.slices; ++k) s += *reinterpret_cast<const f32x4*>(p + k * step);
+    } else
+        for (int k = 0; k < g.slices; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (j < valid) s[j] += p[k * step + j];
+    if (g.bias)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] += g.bias[batch * g.bbias + min(col + j, g.N - 1)];
+    const bool vec = ((uintptr_t)g.c % (DT == CLT_DT_F32 ? 16 : 8)) == 0 && g.ldc % 4 == 0 && g.bc % 4 == 0;
+    b8_store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, s, valid, vec, g.accumulate);
+}
+
+// Slices of K: enough blocks for two thirds of the chip, no slice shorter than 8 blocks of k (the second launch and its traffic
+// cost about as much), partial sums of at most 256 MB.
+int slices_of(int M, int N, int KB, int batch) {
+    const long tiles = ((long)(M - 1) / 128 + 1) * ((N - 1) / 128 + 1) * batch;
+    if (tiles >= 160 || KB < 16) return 1;
+    long s = 256 / tiles;
+    if (s > KB / 8) s = KB / 8;
+    const long bytes = (long)batch * M * N * 4;
+    while (s > 1 && s * bytes > (256L << 20)) --s;
+    if (s < 2) return 1;
+    const int per = (int)((KB + s - 1) / s);
+    return (KB + per - 1) / per;
+}
+
+template <int DT, int FA, int FB> int launch_fmt(const Gemm8Args& g, long blocks, hipStream_t st) {
+    const auto f = gemm8_kernel<DT, FA, FB>;
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, DEPTH * STG) != hipSuccess) return CLT_ERR_LAUNCH;
+    f<<<dim3((unsigned)blocks), dim3(256), DEPTH * STG, st>>>(g);
+    CLT_LAUNCH_CHECK();
+    return CLT_OK;
+}
 template <int DT> int launch(const Gemm8Args& g, int fa, int fb, long blocks, hipStream_t st) {
-    const dim3 gr((unsigned)blocks), t(256);
-    if (fa == 0 && fb == 0) gemm8_kernel<DT, 0, 0><<<gr, t, 0, st>>>(g);
-    else if (fa == 1 && fb == 0) gemm8_kernel<DT, 1, 0><<<gr, t, 0, st>>>(g);
-    else if (fa == 0) gemm8_kernel<DT, 0, 1><<<gr, t, 0, st>>>(g);
-    else gemm8_kernel<DT, 1, 1><<<gr, t, 0, st>>>(g);
+    const int rc = fa == 0 ? (fb == 0 ? launch_fmt<DT, 0, 0>(g, blocks, st) : launch_fmt<DT, 0, 1>(g, blocks, st))
+                           : (fb == 0 ? launch_fmt<DT, 1, 0>(g, blocks, st) : launch_fmt<DT, 1, 1>(g, blocks, st));
+    if (rc != CLT_OK || !g.part) return rc;
+    const int quads = (g.N - 1) / 4 + 1;
+    const long total = (long)g.batch * g.M * quads, fold = (total + 255) / 256;
+    if (fold > 0x7fffffffL) return CLT_ERR_RANGE;
+    gemm8_fold_kernel<DT><<<dim3((unsigned)fold), dim3(256), 0, st>>>(g, quads, total);
     CLT_LAUNCH_CHECK();
     return CLT_OK;
 }
 }  // namespace
 
+extern "C" size_t clt_gemm8_workspace_bytes(int M, int N, int K, int batch) {
+    if (M <= 0 || N <= 0 || K <= 0 || batch <= 0) return 0;
+    const int KB = (int)(up128(K) / 128);
+    if (clt_internal_gemm8_large_applies(M, N, KB, batch)) return 0;
+    const int s = slices_of(M, N, KB, batch);
+    return s > 1 ? (size_t)s * batch * M * N * 4 : 0;
+}
+
 extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long ldas, long a_batch, long as_batch,
                          const void* b, const void* b_scale, int b_format, long ldb, long ldbs, long b_batch, long bs_batch,
                          void* c, int c_dtype, long ldc, long c_batch, const float* bias, long bias_batch, int M, int N, int K,
-                         int batch, int accumulate, void* stream) {
+                         int batch, int accumulate, void* workspace, size_t workspace_bytes, void* stream) {
     if (M <= 0 || N <= 0 || K < 0 || batch <= 0 || c_dtype < 0 || c_dtype > 2 || (a_format & ~1) || (b_format & ~1) || !c) return CLT_ERR_SHAPE;
     if (accumulate && c_dtype != CLT_DT_F32) return CLT_ERR_SHAPE;                 // (a 16-bit sum would round at every call)
     const int KB = (int)(up128(K) / 128);
-    if (KB && (!a || !a_scale || !b || !b_scale || lda < up128(K) || ldb < up128(K) || ldas < M || ldbs < N || ldc < N)) return CLT_ERR_SHAPE;
+    if (ldc < N || (KB && (!a || !a_scale || !b || !b_scale || lda < up128(K) || ldb < up128(K) || ldas < M || ldbs < N))) return CLT_ERR_SHAPE;
     if (KB && (!aligned16(a) || !aligned16(b) || lda % 16 || ldb % 16 || a_batch % 16 || b_batch % 16)) return CLT_ERR_ALIGN;
+    if (KB && (((uintptr_t)a_scale & 3) || ((uintptr_t)b_scale & 3) || ldas % 4 || ldbs % 4 || as_batch % 4 || bs_batch % 4)) return CLT_ERR_ALIGN;
     if (((uintptr_t)c & (c_dtype == CLT_DT_F32 ? 3 : 1)) || ((uintptr_t)bias & 3)) return CLT_ERR_ALIGN;
+    // 32-bit offsets inside a tile's rows and over an operand's scale bytes
+    if (KB && (256 * lda > 0x7fffffffL || 256 * ldb > 0x7fffffffL || KB * ldas > 0x7ffffeffL || KB * ldbs > 0x7ffffeffL)) return CLT_ERR_RANGE;
     Gemm8Args g = {static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(a_scale), static_cast<const uint8_t*>(b),
                    static_cast<const uint8_t*>(b_scale), c, bias, lda, ldas, ldb, ldbs, ldc, a_batch, as_batch, b_batch, bs_batch,
-                   c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate};
+                   c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 1, KB, nullptr};
     const hipStream_t st = as_stream(stream);
-    const int rc = clt_internal_gemm8_large(g, a_format, b_format, c_dtype, batch, st);
-    if (rc <= 0) return rc;                                  // (1: the shape is the small tiles')
-    const long blocks = (long)g.tilesA * g.tilesB * batch;
+    if (clt_internal_gemm8_large_applies(M, N, KB, batch) && 256 * ldc * 4 <= 0x7fffffffL) return clt_internal_gemm8_large(g, a_format, b_format, c_dtype, st);
+    // (a result whose rows lie further apart than the large form's offsets reach runs here, unsliced: no workspace was asked for)
+    if (!clt_internal_gemm8_large_applies(M, N, KB, batch)) g.slices = slices_of(M, N, KB, batch);
+    if (g.slices > 1) {
+        if (!workspace || !aligned16(workspace) || workspace_bytes < clt_gemm8_workspace_bytes(M, N, K, batch)) return CLT_ERR_WORKSPACE;
+        g.part = static_cast<float*>(workspace);
+        g.slice_kb = (KB + g.slices - 1) / g.slices;
+    }
+    const long blocks = (long)g.tilesA * g.tilesB * batch * g.slices;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
     return c_dtype == CLT_DT_F32 ? launch<CLT_DT_F32>(g, a_format, b_format, blocks, st)
            : c_dtype == CLT_DT_BF16 ? launch<CLT_DT_BF16>(g, a_format, b_format, blocks, st)

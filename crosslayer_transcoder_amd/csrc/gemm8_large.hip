@@ -309,17 +309,17 @@ template <int DT> int launch_fmt(const Gemm8Args& g, int fa, int fb, int total, 
 }
 }  // namespace
 
-int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, int batch, hipStream_t st) {
+// a chip's worth of tiles, mostly full ones
+bool clt_internal_gemm8_large_applies(int M, int N, int KB, int batch) {
+    const long total = ((long)(M - 1) / 256 + 1) * ((N - 1) / 256 + 1) * batch;
+    return KB >= 1 && M >= 128 && N >= 128 && total >= 128 && total <= 0x3fffffffL;
+}
+
+int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, hipStream_t st) {
     Gemm8Args g = g0;
     g.tilesA = (g.M - 1) / 256 + 1; g.tilesB = (g.N - 1) / 256 + 1;
-    const long total = (long)g.tilesA * g.tilesB * batch;
-    // a chip's worth of tiles, mostly full ones
-    if (g.KB < 1 || g.M < 128 || g.N < 128 || total < 128 || total > 0x3fffffffL) return 1;
-    // 32-bit offsets inside a tile's rows and over a scale row's blocks, whole dwords of scale bytes
-    if (256 * g.lda > 0x7fffffffL || 256 * g.ldb > 0x7fffffffL || (long)g.KB * g.ldas > 0x7ffffeffL || (long)g.KB * g.ldbs > 0x7ffffeffL) return 1;
-    if (256 * g.ldc * 4 > 0x7fffffffL) return 1;
-    if (g.ldas % 4 || g.ldbs % 4 || g.bas % 4 || g.bbs % 4 || ((uintptr_t)g.as & 3) || ((uintptr_t)g.bs & 3)) return 1;
-    return dtype == CLT_DT_F32 ? launch_fmt<CLT_DT_F32>(g, fa, fb, (int)total, st)
-           : dtype == CLT_DT_BF16 ? launch_fmt<CLT_DT_BF16>(g, fa, fb, (int)total, st)
-                                  : launch_fmt<CLT_DT_F16>(g, fa, fb, (int)total, st);
+    const int total = g.tilesA * g.tilesB * g.batch;
+    return dtype == CLT_DT_F32 ? launch_fmt<CLT_DT_F32>(g, fa, fb, total, st)
+           : dtype == CLT_DT_BF16 ? launch_fmt<CLT_DT_BF16>(g, fa, fb, total, st)
+                                  : launch_fmt<CLT_DT_F16>(g, fa, fb, total, st);
 }

@@ -78,8 +78,11 @@ def _gemm(a, b, K, out, ldc, cb, bias, nbias, st):
     (aq, as_, L, M), (bq, bs, _, N) = a, b
     k = _up(K)
     sa, sb = _up(M), _up(N)
+    nws = lib.clt_gemm8_workspace_bytes(M, N, K, L)
+    ws = torch.empty(nws, dtype=torch.uint8, device=out.device) if nws else None
     _call(lib.clt_gemm8, aq, as_, _E4M3, k, sa, M * k, k // 128 * sa, bq, bs, _E4M3, k, sb, N * k, k // 128 * sb, out.data_ptr(),
-          _DT[out.dtype], ldc, cb, bias.data_ptr() if bias is not None else None, nbias, M, N, K, L, 0, st)
+          _DT[out.dtype], ldc, cb, bias.data_ptr() if bias is not None else None, nbias, M, N, K, L, 0,
+          ws.data_ptr() if nws else None, nws, st)
 
 
 def _gradients(dy, kept, K, kn, has_x, need_dx, w_dtype, need_db):

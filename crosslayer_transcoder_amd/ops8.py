@@ -62,7 +62,7 @@ def _dense(x: torch.Tensor, dims=(2, 3)) -> torch.Tensor:
 class Block8:
     """A batch of matrices [L, rows, cols] in 8 bits.  data: uint8 [L, rows, >= cols rounded up to 128], rows 16-byte aligned,
     codes of `fmt` ("e4m3" / "e5m2"), ZERO behind column `cols` up to the next multiple of 128; scale: uint8 [L, >= blocks of 128
-    columns, >= rows], byte e + 127 for the scale 2^e of a row's block.  The pack functions below make it; one may be built
+    columns, >= rows], rows 4-byte aligned, byte e + 127 for the scale 2^e of a row's block.  The pack functions below make it; one may be built
     from kept tensors (a checkpoint of packed weights) as well."""
     __slots__ = ("data", "scale", "rows", "cols", "fmt")
 
@@ -76,8 +76,9 @@ class Block8:
             raise ValueError("codes [L, rows, bytes] and scale bytes [L, blocks, rows] have three dimensions")
         if rows < 0 or cols < 0 or data.shape[1] != rows or data.shape[2] < _up(cols) or scale.shape[1] < _up(cols) // BLOCK or scale.shape[2] < rows:
             raise ValueError(f"codes {tuple(data.shape)} / scale bytes {tuple(scale.shape)} do not hold a [{rows}, {cols}] matrix")
-        if data.numel() and (data.stride(2) != 1 or scale.stride(2) != 1 or data.stride(1) % 16 or data.stride(0) % 16 or data.data_ptr() % 16):
-            raise ValueError("packed rows are dense and start at multiples of 16 bytes")
+        if data.numel() and (data.stride(2) != 1 or scale.stride(2) != 1 or data.stride(1) % 16 or data.stride(0) % 16 or data.data_ptr() % 16
+                             or scale.stride(1) % 4 or scale.stride(0) % 4 or scale.data_ptr() % 4):
+            raise ValueError("packed rows are dense and start at multiples of 16 bytes (codes) and 4 bytes (scales)")
         self.data, self.scale, self.rows, self.cols, self.fmt = data, scale, rows, cols, fmt
 
     @property
@@ -222,11 +223,14 @@ def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: 
         raise ValueError(f"out must be an [{L}, {M}, {N}] tensor of non-overlapping dense rows on the operands' device")
     bias = _bias(bias, L, N, a.device)
     if out.numel():
+        nws = lib.clt_gemm8_workspace_bytes(M, N, K, L)
+        ws = torch.empty(nws, dtype=torch.uint8, device=a.device) if nws else None
         with _on(a.device):
             _call(lib.clt_gemm8, a.data.data_ptr(), a.scale.data_ptr(), FORMATS[a.fmt], a.data.stride(1), a.scale.stride(1),
                   a.data.stride(0), a.scale.stride(0), b.data.data_ptr(), b.scale.data_ptr(), FORMATS[b.fmt], b.data.stride(1),
                   b.scale.stride(1), b.data.stride(0), b.scale.stride(0), out.data_ptr(), _DT[out.dtype], out.stride(1) if M > 1 else N,
-                  out.stride(0), bias.data_ptr() if bias is not None else None, N, M, N, K, L, int(accumulate), _stream(a.device))
+                  out.stride(0), bias.data_ptr() if bias is not None else None, N, M, N, K, L, int(accumulate),
+                  ws.data_ptr() if nws else None, nws, _stream(a.device))
     return out
 
 

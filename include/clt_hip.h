@@ -553,11 +553,13 @@ int clt_unpack8(const void* q, const void* s, int format, int batch, int rows, i
                 long q_batch_stride, long s_batch_stride, void* out, int dtype, void* stream);
 /* C[M][N] (+)= A[M][K] * B[N][K]^T + bias[N], batched; pitches and batch strides of A, B in bytes, of C and bias in elements.
  * c_dtype bf16 / fp16: 8-bit matrix instructions (products aligned to ~14 bits in groups of 16, fp32 sums, one rounding);
- * c_dtype fp32: exact products (bf16 instructions), fp32 sums; accumulate != 0 (fp32 only): C += . K = 0 gives the bias. */
+ * c_dtype fp32: exact products (bf16 instructions), fp32 sums; accumulate != 0 (fp32 only): C += . K = 0 gives the bias.
+ * Scale rows: 4-byte aligned, readable up to a multiple of 4 bytes.  workspace (16-byte aligned): partial sums where K is cut. */
+size_t clt_gemm8_workspace_bytes(int M, int N, int K, int batch);
 int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long ldas, long a_batch, long as_batch,
               const void* b, const void* b_scale, int b_format, long ldb, long ldbs, long b_batch, long bs_batch,
               void* c, int c_dtype, long ldc, long c_batch, const float* bias, long bias_batch, int M, int N, int K, int batch,
-              int accumulate, void* stream);
+              int accumulate, void* workspace, size_t workspace_bytes, void* stream);
 /* y[t][l][:] = x[t][l][:] * w[l]^T + bias[l] for few tokens (at most 64; returns 1 for more: clt_pack8 + clt_gemm8), x packed on the
  * way (e4m3, blocks along K), exact products, fp32 sums.  x, y: unit stride in K / N, token and layer strides in elements. */
 size_t clt_linear8_rows_workspace_bytes(int tokens, int layers, int N, int K);

@@ -160,7 +160,8 @@ def check_product(y, a, b, bias=None, base=None):
 
 
 PRODUCTS = [(1, 1, 1, 1), (1, 1, 110, 32), (2, 16, 110, 32), (1, 5, 768, 1000), (3, 33, 130, 257), (1, 128, 128, 128), (1, 200, 1000, 300),
-            (2, 257, 513, 129), (1, 64, 4096, 96), (12, 3, 256, 64), (1, 300, 384, 512)]
+            (2, 257, 513, 129), (1, 64, 4096, 96), (12, 3, 256, 64), (1, 300, 384, 512), (1, 100, 9000, 130), (2, 33, 20000, 15),
+            (1, 130, 2048, 260), (1, 250, 2300, 77), (40, 100, 2500, 100)]
 
 
 @gpu
@@ -517,16 +518,17 @@ def test_refusals_of_tensors():
 def test_refusals_of_block8():
     from crosslayer_transcoder_amd.ops8 import Block8
     u = lambda *s: torch.zeros(*s, dtype=torch.uint8)                            # noqa: E731
-    Block8(u(2, 5, 128), u(2, 1, 5), 5, 100)
-    for args in ((u(2, 5, 128), u(2, 1, 4), 5, 100), (u(2, 5, 112), u(2, 1, 5), 5, 100), (u(2, 5, 128), u(2, 1, 5), 5, 129),
-                 (u(2, 5, 128), u(1, 1, 5), 5, 100), (u(2, 4, 128), u(2, 1, 5), 5, 100), (u(5, 128), u(1, 5), 5, 100),
-                 (u(2, 128, 5).mT, u(2, 1, 5), 5, 100), (u(2, 5, 136)[:, :, :130], u(2, 1, 5), 5, 100), (u(2, 5, 256)[:, :, 1:129], u(2, 1, 5), 5, 100)):
+    Block8(u(2, 5, 128), u(2, 1, 8), 5, 100)
+    for args in ((u(2, 5, 128), u(2, 1, 4), 5, 100), (u(2, 5, 112), u(2, 1, 8), 5, 100), (u(2, 5, 128), u(2, 1, 8), 5, 129),
+                 (u(2, 5, 128), u(1, 1, 8), 5, 100), (u(2, 4, 128), u(2, 1, 8), 5, 100), (u(5, 128), u(1, 8), 5, 100),
+                 (u(2, 5, 128), u(2, 1, 5), 5, 100), (u(2, 5, 128), u(2, 1, 16)[:, :, 1:9], 5, 100),
+                 (u(2, 128, 5).mT, u(2, 1, 8), 5, 100), (u(2, 5, 136)[:, :, :130], u(2, 1, 8), 5, 100), (u(2, 5, 256)[:, :, 1:129], u(2, 1, 8), 5, 100)):
         with pytest.raises(ValueError):
             Block8(*args)
     with pytest.raises(ValueError):
-        Block8(u(2, 5, 128), u(2, 1, 5), 5, 100, "e3m4")
+        Block8(u(2, 5, 128), u(2, 1, 8), 5, 100, "e3m4")
     with pytest.raises(TypeError):
-        Block8(u(2, 5, 128).float(), u(2, 1, 5), 5, 100)
+        Block8(u(2, 5, 128).float(), u(2, 1, 8), 5, 100)
     q = Block8(u(2, 5, 384), u(2, 3, 128), 5, 300)
     assert q.first_rows(3).rows == 3 and q.first_columns(256).cols == 256 and q.of_batch(1).batch == 1
     for bad in (lambda: q.first_rows(6), lambda: q.first_columns(200), lambda: q.first_columns(384)):
@@ -549,10 +551,11 @@ def test_refusals_of_the_library():
     assert pack(cs=p) == -3 and pack(cs=p, ws=p, n=255) == -3
 
     def gemm(a=p, lda=128, ldas=128, b=p, ldb=128, ldbs=128, c=p, dt=0, ldc=64, M=4, N=4, K=100, batch=1, acc=0, fa=0, bias=None):
-        return lib.clt_gemm8(a, p, fa, lda, ldas, 0, 0, b, p, 0, ldb, ldbs, 0, 0, c, dt, ldc, 0, bias, 0, M, N, K, batch, acc, None)
+        return lib.clt_gemm8(a, p, fa, lda, ldas, 0, 0, b, p, 0, ldb, ldbs, 0, 0, c, dt, ldc, 0, bias, 0, M, N, K, batch, acc, None, 0, None)
 
     assert [gemm(M=0), gemm(N=0), gemm(K=-1), gemm(batch=0), gemm(dt=3), gemm(dt=1, acc=1), gemm(lda=112), gemm(ldbs=3), gemm(ldc=3), gemm(fa=2), gemm(c=None), gemm(a=None)] == [-1] * 12
-    assert [gemm(a=p + 8), gemm(lda=136), gemm(c=p + 2), gemm(bias=p + 1)] == [-4] * 4
+    assert [gemm(a=p + 8), gemm(lda=136), gemm(c=p + 2), gemm(bias=p + 1), gemm(ldas=130)] == [-4] * 5
+    assert gemm(K=5000, lda=5120, ldb=5120) == -3 and gemm(lda=1 << 24) == -6
     assert lib.clt_unpack8(p, p, 0, 1, 4, 100, 112, 128, 0, 0, p, 0, None) == -1
     assert lib.clt_unpack8(p, p, 0, 1, 4, 100, 136, 128, 0, 0, p, 0, None) == -4
 
