@@ -40,29 +40,34 @@ template <int N, class F> __device__ __forceinline__ void unroll(F f) {
 typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 
+struct Tile { int batch, a0, b0; };
+// block -> tile: every XCD (block index mod 8) works on a contiguous range of tiles, walked in panels of 4 A tiles with the A tile
+// fastest, so that the blocks an XCD runs together share operand tiles in its L2
+__device__ __forceinline__ Tile decode_tile(const Gemm8Args& g, int vb) {
+    const int nwg = g.tilesA * g.tilesB;
+    Tile t;
+    t.batch = vb / nwg;
+    int lid = vb - t.batch * nwg;
+    const int xcd = lid & 7, q = nwg >> 3, r = nwg & 7;
+    lid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lid >> 3);
+    constexpr int GA = 4;
+    const int full = g.tilesA / GA, rem = g.tilesA - full * GA, per = GA * g.tilesB;
+    int ta, tb;
+    if (lid < full * per) { const int pn = lid / per, x = lid - pn * per; tb = x / GA; ta = pn * GA + (x - tb * GA); }
+    else { const int x = lid - full * per; tb = x / rem; ta = full * GA + (x - tb * rem); }
+    t.a0 = ta * 256; t.b0 = tb * 256;
+    return t;
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, long records) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)records, 0x00020000);
+}
+
 template <int DT, int FA, int FB>
 __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int total) {
-    constexpr bool WIDE = DT == CLT_DT_F32;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wb = w >> 1, wa = w & 1, fr = lane & 15, fq = lane >> 4;
-    const int nwg = g.tilesA * g.tilesB, nk = g.KB;
-    struct Tile { int batch, a0, b0; };
-    // block -> tile: every XCD (block index mod 8) works on a contiguous range of tiles, walked in panels of 4 A tiles with the A tile
-    // fastest, so that the blocks an XCD runs together share operand tiles in its L2
-    auto decode = [&](int vb) {
-        Tile t;
-        t.batch = vb / nwg;
-        int lid = vb - t.batch * nwg;
-        const int xcd = lid & 7, q = nwg >> 3, r = nwg & 7;
-        lid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lid >> 3);
-        constexpr int GA = 4;
-        const int full = g.tilesA / GA, rem = g.tilesA - full * GA, per = GA * g.tilesB;
-        int ta, tb;
-        if (lid < full * per) { const int pn = lid / per, x = lid - pn * per; tb = x / GA; ta = pn * GA + (x - tb * GA); }
-        else { const int x = lid - full * per; tb = x / rem; ta = full * GA + (x - tb * rem); }
-        t.a0 = ta * 256; t.b0 = tb * 256;
-        return t;
-    };
+    const int nk = g.KB;
+    auto decode = [&](int vb) { return decode_tile(g, vb); };
 
     // ---- DMA: piece i of wave w fills LDS rows (4 i + w) * 8 .. + 7; a lane supplies 16 bytes (chunk XOR-swizzled with bits 1..3 of the
     // row).  Descriptors start at the tile's first row and end behind its last one: rows past the matrix arrive as zeros.
@@ -71,7 +76,6 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     const int vA = (q8 * 8 + (w >> 1)) * (int)g.lda + ch * 16;
     const int vB = ((((q8 & 3) << 2) | (q8 >> 2)) * 8 + (w >> 1)) * (int)g.ldb + ch * 16;
     __amdgpu_buffer_rsrc_t rA, rB, rS, rBias;
-    auto rsrc = [](const void* p, long records) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)records, 0x00020000); };
     auto aim = [&](const Tile& t) {
         rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda, (long)min(g.M - t.a0, 256) * g.lda);
         rB = rsrc(g.b + t.batch * g.bb + (long)t.b0 * g.ldb, (long)min(g.N - t.b0, 256) * g.ldb);
@@ -102,7 +106,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     for (int m = 0; m < 8; ++m)
 #pragma unroll
         for (int n = 0; n < 8; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int NST = WIDE ? 64 : 32;                   // stores of an interior tile per lane
+    constexpr int NST = 32;                               // stores of an interior tile per lane
 
     // ---- the stream of k-blocks: staging runs two blocks ahead of the products, across tiles
     int vb = blockIdx.x, svb = vb, skt = 0, sslot = 0, slot = 0, buf = 0;
@@ -129,118 +133,57 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     // Buffer handover: this wave's reads of the block are complete and its pieces of the next block have landed; then all waves'.
     // Vector memory retires in order: in a tile's first block the next block's pieces are older than the previous tile's stores,
-    // which may stay outstanding (63 is the counter's limit).  One asm statement: the scheduling region around it stays whole.
+    // which may stay outstanding.  One asm statement: the scheduling region around it stays whole.
     auto handover = [](int kt) {
-        asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(0)\n1:\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_barrier" ::"s"(kt), "i"(NST < 63 ? NST : 63) : "scc", "memory");
+        asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(0)\n1:\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_barrier" ::"s"(kt), "i"(NST) : "scc", "memory");
     };
     const int lo = (fq ^ x) << 4;
     int aA = rowA, aB = rowB, aSA = scA, aSB = scB;       // the block's addresses; the other buffer's by XOR
     auto flip = [&]() { aA ^= STG; aB ^= STG; aSA ^= 512; aSB ^= 512; };
 
-    // fast path state: fragments of the current block (and, from its second half on, of the next); 32-bit path state below
+    // fragments of the current block (and, from its second half on, of the next)
     i32x8 fa[8], fb[8];
     i32x2 sa, sb;
     auto ld = [&](int at, int off) {                      // chunks fq and fq + 4: any split of the block's k that both operands share
         const i32x4 u = *reinterpret_cast<const i32x4*>(g8_smem + (at + lo) + off), v = *reinterpret_cast<const i32x4*>(g8_smem + (at + (lo ^ 64)) + off);
         return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    // 32-bit results: a block is 4 steps of 32 k; a lane's 8 codes of a row and step are 8 bytes
-    const int half = (fq & 1) << 3, cq = fq >> 1;
-    auto ldw = [&](int at, int off, int s) { return *reinterpret_cast<const i32x2*>(g8_smem + (at + ((((2 * s) + cq) ^ x) << 4) + half) + off); };
-    i32x2 rb[8];
-    bf16x8 ha[8], hb;
-    float xa[8], xb[8];
-    auto scales = [&](float* d, int at) {
-        const i32x2 u = *reinterpret_cast<const i32x2*>(g8_smem + at);
+    sa = *reinterpret_cast<const i32x2*>(g8_smem + aSA);
+    sb = *reinterpret_cast<const i32x2*>(g8_smem + aSB);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = __uint_as_float((((uint32_t)u[j >> 2] >> (8 * (j & 3))) & 0xffu) << 23);
-    };
-    if constexpr (!WIDE) {
-        sa = *reinterpret_cast<const i32x2*>(g8_smem + aSA);
-        sb = *reinterpret_cast<const i32x2*>(g8_smem + aSB);
+    for (int n = 0; n < 8; ++n) fa[n] = ld(aA, n * 2048);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) fa[n] = ld(aA, n * 2048);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) fb[m] = ld(aB, m * 2048);
-    } else {
-        scales(xa, aSA);
-        scales(xb, aSB);
-#pragma unroll
-        for (int n = 0; n < 8; ++n) { const i32x2 r = ldw(aA, n * 2048, 0); ha[n] = widen8<FA>((uint32_t)r[0], (uint32_t)r[1], xa[n]); }
-#pragma unroll
-        for (int m = 0; m < 8; ++m) rb[m] = ldw(aB, m * 2048, 0);
-        hb = widen8<FB>((uint32_t)rb[0][0], (uint32_t)rb[0][1], xb[0]);
-    }
+    for (int m = 0; m < 4; ++m) fb[m] = ld(aB, m * 2048);
 
     for (;;) {
         for (int kt = 0; kt < nk; ++kt) {
             advance(nt);
-            if constexpr (!WIDE) {
-                // 64 instructions a block.  First half: B fragments 0..3, A fragments fastest; B fragments 4..7 are read meanwhile.
-                // Handover.  Second half: A fragment by A fragment against B fragments 4..7; the block after next is staged, the
-                // next block's B fragments 0..3 are read, and every A fragment is replaced by the next block's after its last use.
-                auto mfma = [&](auto m_, auto n_) {
-                    constexpr int m = decltype(m_)::value, n = decltype(n_)::value;
-                    acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[m], fa[n], acc[m][n], FB, FA, m & 3, sb[m >> 2], n & 3, sa[n >> 2]);
-                    __builtin_amdgcn_sched_barrier(0);
-                };
-                unroll<4>([&](auto m) {
-                    fb[m + 4] = ld(aB, (m + 4) * 2048);
-                    __builtin_amdgcn_sched_barrier(0);
-                    unroll<8>([&](auto n) { mfma(m, n); });
+            // 64 instructions a block.  First half: B fragments 0..3, A fragments fastest; B fragments 4..7 are read meanwhile.
+            // Handover.  Second half: A fragment by A fragment against B fragments 4..7; the block after next is staged, the
+            // next block's B fragments 0..3 are read, and every A fragment is replaced by the next block's after its last use.
+            auto mfma = [&](auto m_, auto n_) {
+                constexpr int m = decltype(m_)::value, n = decltype(n_)::value;
+                acc[m][n] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[m], fa[n], acc[m][n], FB, FA, m & 3, sb[m >> 2], n & 3, sa[n >> 2]);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            unroll<4>([&](auto m) {
+                fb[m + 4] = ld(aB, (m + 4) * 2048);
+                __builtin_amdgcn_sched_barrier(0);
+                unroll<8>([&](auto n) { mfma(m, n); });
+            });
+            handover(kt);
+            flip();
+            const i32x2 sa_n = *reinterpret_cast<const i32x2*>(g8_smem + aSA), sb_n = *reinterpret_cast<const i32x2*>(g8_smem + aSB);
+            scale_piece(buf, skt);
+            unroll<8>([&](auto n) {
+                unroll<4>([&](auto j) {
+                    if constexpr (j < 2 && n < 4) piece(buf, skt, 2 * n + j);
+                    if constexpr (j == 2 && n >= 4) fb[n - 4] = ld(aB, (n - 4) * 2048);
+                    mfma(std::integral_constant<int, 4 + decltype(j)::value>{}, n);
                 });
-                handover(kt);
-                flip();
-                const i32x2 sa_n = *reinterpret_cast<const i32x2*>(g8_smem + aSA), sb_n = *reinterpret_cast<const i32x2*>(g8_smem + aSB);
-                scale_piece(buf, skt);
-                unroll<8>([&](auto n) {
-                    unroll<4>([&](auto j) {
-                        if constexpr (j < 2 && n < 4) piece(buf, skt, 2 * n + j);
-                        if constexpr (j == 2 && n >= 4) fb[n - 4] = ld(aB, (n - 4) * 2048);
-                        mfma(std::integral_constant<int, 4 + decltype(j)::value>{}, n);
-                    });
-                    fa[n] = ld(aA, n * 2048);
-                });
-                sa = sa_n; sb = sb_n;
-            } else {
-                // 4 steps of 8 groups (B fragment m) of 8 instructions of 16 cycles.  In a step the next step's codes are read (groups
-                // 0..3), its A fragments converted (groups 4..7) and every B fragment one group ahead of its use.
-                float xa_n[8], xb_n[8];
-                unroll<4>([&](auto s) {
-                    constexpr int S = decltype(s)::value;
-                    i32x2 ra_n[8], rb_n[8];
-                    bf16x8 ha_n[8];
-                    if constexpr (S == 3) {
-                        handover(kt);
-                        flip();
-                        scales(xa_n, aSA);
-                        scales(xb_n, aSB);
-                        scale_piece(buf, skt);
-                    }
-                    unroll<8>([&](auto m_) {
-                        constexpr int m = decltype(m_)::value;
-                        if constexpr (m < 4) {
-#pragma unroll
-                            for (int j = 2 * m; j < 2 * m + 2; ++j) { ra_n[j] = ldw(aA, j * 2048, (S + 1) & 3); rb_n[j] = ldw(aB, j * 2048, (S + 1) & 3); }
-                        } else {
-#pragma unroll
-                            for (int j = 2 * m - 8; j < 2 * m - 6; ++j) ha_n[j] = widen8<FA>((uint32_t)ra_n[j][0], (uint32_t)ra_n[j][1], S == 3 ? xa_n[j] : xa[j]);
-                        }
-                        if constexpr (S == 3) piece(buf, skt, m);
-                        bf16x8 hb_n;
-                        if constexpr (m < 7) hb_n = widen8<FB>((uint32_t)rb[m + 1][0], (uint32_t)rb[m + 1][1], xb[m + 1]);
-                        else hb_n = widen8<FB>((uint32_t)rb_n[0][0], (uint32_t)rb_n[0][1], S == 3 ? xb_n[0] : xb[0]);
-#pragma unroll
-                        for (int n = 0; n < 8; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb, ha[n], acc[m][n], 0, 0, 0);
-                        hb = hb_n;
-                        __builtin_amdgcn_sched_barrier(0);
-                    });
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) { ha[j] = ha_n[j]; rb[j] = rb_n[j]; }
-                });
-#pragma unroll
-                for (int j = 0; j < 8; ++j) { xa[j] = xa_n[j]; xb[j] = xb_n[j]; }
-            }
+                fa[n] = ld(aA, n * 2048);
+            });
+            sa = sa_n; sb = sb_n;
             buf ^= 1;
         }
         const Tile cur = t;
@@ -253,7 +196,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
         // ---- results: for (n, i) a lane has row 8 fr + n and eight columns 8 (4 i + fq) ..
         typedef typename Elem<DT>::type T;
         const int r0 = wa * 128 + fr * 8, c0 = wb * 128 + fq * 8;
-        const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N && !g.accumulate;
+        const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N;
         T* ctile = static_cast<T*>(g.c) + cur.batch * g.bc + (long)cur.a0 * g.ldc + cur.b0;
         const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + c0;
         const bool has_bias = g.bias != nullptr;
@@ -267,20 +210,12 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
                 f32x4 hi = f32x4{acc[4][n][i], acc[5][n][i], acc[6][n][i], acc[7][n][i]};
                 if (has_bias) { lo += *reinterpret_cast<const f32x4*>(bl + i * 32); hi += *reinterpret_cast<const f32x4*>(bl + i * 32 + 4); }
                 T* p = reinterpret_cast<T*>(reinterpret_cast<char*>(ctile + (long)n * g.ldc + i * 32) + at);
-                if constexpr (WIDE) {
-                    if (interior) { *reinterpret_cast<f32x4_u*>(p) = lo; *reinterpret_cast<f32x4_u*>(p + 4) = hi; }
-                    else if (n < rows)
+                const u32x4_u u = {pack_out16<DT>(lo[0], lo[1]), pack_out16<DT>(lo[2], lo[3]), pack_out16<DT>(hi[0], hi[1]), pack_out16<DT>(hi[2], hi[3])};
+                if (interior) *reinterpret_cast<u32x4_u*>(p) = u;
+                else if (n < rows)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (i * 32 + j < cols) { const float v = j < 4 ? lo[j & 3] : hi[j & 3]; p[j] = g.accumulate ? p[j] + v : v; }
-                } else {
-                    const u32x4_u u = {pack_out16<DT>(lo[0], lo[1]), pack_out16<DT>(lo[2], lo[3]), pack_out16<DT>(hi[0], hi[1]), pack_out16<DT>(hi[2], hi[3])};
-                    if (interior) *reinterpret_cast<u32x4_u*>(p) = u;
-                    else if (n < rows)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (i * 32 + j < cols) p[j] = (T)(u[j >> 1] >> (16 * (j & 1)));
-                }
+                    for (int j = 0; j < 8; ++j)
+                        if (i * 32 + j < cols) p[j] = (T)(u[j >> 1] >> (16 * (j & 1)));
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -294,18 +229,165 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no DMA into this block's LDS outlives it
 }
 
-template <int DT, int FA, int FB> int launch(const Gemm8Args& g, int total, hipStream_t st) {
-    const auto f = gemm8_large_kernel<DT, FA, FB>;
+// ---- 32-bit results: the codes become bf16 in registers and the products run at the 16-bit rate, so a block of k costs twice the
+// cycles for the same LDS bytes: 8 waves of 128 x 64 (B x A; 192 KB of reads in 4096 cycles), two per SIMD, whose conversions run
+// under each other's matrix instructions.  Tiles, DMA, row order and the stream of blocks as above; A fragments are 4 rows of a
+// 64-row group (row 4 * lane + n).
+template <int FA, int FB>
+__global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, int total) {
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wb = w >> 2, wa = w & 3, fr = lane & 15, fq = lane >> 4;
+    const int nk = g.KB;
+    // piece i of wave w fills LDS rows (8 i + w) * 8 .. + 7
+    const int q8 = (w & 1) * 8 + (lane >> 3), ch = (lane & 7) ^ ((q8 >> 1) & 7);
+    const int vA = (q8 * 4 + (w >> 1)) * (int)g.lda + ch * 16;
+    const int vB = ((((q8 & 3) << 2) | (q8 >> 2)) * 8 + (w >> 1)) * (int)g.ldb + ch * 16;
+    const int srow = (int)(w & 1 ? g.ldbs : g.ldas);
+    __amdgpu_buffer_rsrc_t rA, rB, rS;
+    int vb = blockIdx.x, svb = vb, skt = 0, sslot = 0, slot = 0, buf = 0;
+    auto enter = [&](const Tile& t) {
+        if (svb < total) {
+            rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda, (long)min(g.M - t.a0, 256) * g.lda);
+            rB = rsrc(g.b + t.batch * g.bb + (long)t.b0 * g.ldb, (long)min(g.N - t.b0, 256) * g.ldb);
+            const uint8_t* sp = w & 1 ? g.bs + t.batch * g.bbs + t.b0 : g.as + t.batch * g.bas + t.a0;
+            rS = rsrc(sp, (long)(nk - 1) * srow + min(((w & 1 ? g.N - t.b0 : g.M - t.a0) + 3) & ~3, 256));
+            if (g.bias && w == 2) {
+                __amdgpu_buffer_rsrc_t r = rsrc(g.bias + t.batch * g.bbias + t.b0, min(g.N - t.b0, 256) * 4L);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(g8_smem + BIAS_BASE + sslot * 1024), 16, lane * 16, 0, 0, 0);
+            }
+        } else { rA = rsrc(g.a, 0); rB = rsrc(g.b, 0); rS = rsrc(g.as, 0); }
+    };
+    auto advance = [&](const Tile& next) {
+        if (++skt == nk) { skt = 0; svb += (int)gridDim.x; sslot = (sslot + 1) & 3; enter(next); }
+    };
+    auto piece = [&](int b, int kt, int i) {
+        unsigned char* base = g8_smem + b * STG + (i * 8 + w) * 1024;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rA, (lds_void*)base, 16, vA + i * 64 * (int)g.lda, kt * 128, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rB, (lds_void*)(base + OPB), 16, vB + ((i >> 1) * 128 + (i & 1) * 4) * (int)g.ldb, kt * 128, 0, 0);
+    };
+    auto scale_piece = [&](int b, int kt) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rS, (lds_void*)(g8_smem + SCALE_BASE + b * 512 + (w & 1) * 256), 4, lane * 4, kt * srow, 0, 0);
+    };
+    f32x4 acc[8][4];
+#pragma unroll
+    for (int m = 0; m < 8; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int NST = 32;                               // stores of an interior tile per lane
+    Tile t = decode_tile(g, vb);
+    enter(t);
+    for (int k = 0; k < 2; ++k) {
+        if (k) advance(decode_tile(g, svb + (int)gridDim.x));
+        scale_piece(k, skt);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) piece(k, skt, i);
+    }
+    Tile nt = decode_tile(g, svb + (int)gridDim.x);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    auto handover = [](int kt) {
+        asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(0)\n1:\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_barrier" ::"s"(kt), "i"(NST) : "scc", "memory");
+    };
+    const int x = fr >> 1, half = (fq & 1) << 3, cq = fq >> 1, cB = ((fr & 3) << 2) | (fr >> 2);
+    int aA = (wa * 64 + fr) * 128 + half + ((cq ^ x) << 4), aB = aA - wa * 64 * 128 + OPB + wb * 128 * 128;
+    int aSA = SCALE_BASE + wa * 64 + fr * 4, aSB = SCALE_BASE + 256 + wb * 128 + cB * 8;
+    // a lane's 8 codes of a row and step of 32 k; scales as floats
+    auto ldw = [&](int at, int off) { return *reinterpret_cast<const i32x2*>(g8_smem + at + off); };
+    i32x2 ra[4], rb[8], sv;
+    uint32_t su;
+    float xa[4], xb[8];
+    auto load_scales = [&]() { su = *reinterpret_cast<const uint32_t*>(g8_smem + aSA); sv = *reinterpret_cast<const i32x2*>(g8_smem + aSB); };
+    load_scales();
+#pragma unroll
+    for (int n = 0; n < 4; ++n) ra[n] = ldw(aA, n * 2048);
+#pragma unroll
+    for (int m = 0; m < 8; ++m) rb[m] = ldw(aB, m * 2048);
+    for (;;) {
+        // A loop over steps of 32 k: one instruction per accumulator and iteration keeps every accumulator where it is (unrolled by block,
+        // the register allocator moves them around).  The step's codes are in registers: A's are converted, then B's fragment by
+        // fragment, and the next step's are read behind them.  A block's last step reads the next block: the handover is ahead of it.
+        for (int it = 0; it < 4 * nk; ++it) {
+            const int step = it & 3;
+            if (step == 0) {
+                advance(nt);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) xa[j] = __uint_as_float(((su >> (8 * j)) & 0xffu) << 23);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xb[j] = __uint_as_float((((uint32_t)sv[j >> 2] >> (8 * (j & 3))) & 0xffu) << 23);
+            }
+            if (step == 3) {
+                handover(it >> 2);
+                aA ^= STG; aB ^= STG; aSA ^= 512; aSB ^= 512;
+                load_scales();
+                scale_piece(buf, skt);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) piece(buf, skt, i);
+                buf ^= 1;
+            }
+            const int next = ((it + 1) & 3) << 5, nA = aA ^ next, nB = aB ^ next;
+            bf16x8 ha[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                ha[n] = widen8<FA>((uint32_t)ra[n][0], (uint32_t)ra[n][1], xa[n]);
+                ra[n] = ldw(nA, n * 2048);
+            }
+            unroll<8>([&](auto m_) {
+                constexpr int m = decltype(m_)::value;
+                const bf16x8 hb = widen8<FB>((uint32_t)rb[m][0], (uint32_t)rb[m][1], xb[m]);
+                rb[m] = ldw(nB, m * 2048);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb, ha[n], acc[m][n], 0, 0, 0);
+            });
+        }
+        const Tile cur = t;
+        const int cslot = slot;
+        vb += (int)gridDim.x;
+        slot = (slot + 1) & 3;
+        const bool more = vb < total;
+        if (more) t = decode_tile(g, vb);
+        nt = decode_tile(g, svb + (int)gridDim.x);
+        // ---- results: for (n, i) a lane has row 4 fr + n of its 64 and eight columns 8 (4 i + fq) .. of its 128
+        const int r0 = wa * 64 + fr * 4, c0 = wb * 128 + fq * 8;
+        const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N && !g.accumulate;
+        float* ctile = static_cast<float*>(g.c) + cur.batch * g.bc + (long)cur.a0 * g.ldc + cur.b0;
+        const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + c0;
+        const bool has_bias = g.bias != nullptr;
+        const int rows = g.M - cur.a0 - r0, cols = g.N - cur.b0 - c0;
+        const unsigned at = (unsigned)(r0 * (int)g.ldc + c0) * 4u;
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f32x4 lo = f32x4{acc[0][n][i], acc[1][n][i], acc[2][n][i], acc[3][n][i]};
+                f32x4 hi = f32x4{acc[4][n][i], acc[5][n][i], acc[6][n][i], acc[7][n][i]};
+                if (has_bias) { lo += *reinterpret_cast<const f32x4*>(bl + i * 32); hi += *reinterpret_cast<const f32x4*>(bl + i * 32 + 4); }
+                float* p = reinterpret_cast<float*>(reinterpret_cast<char*>(ctile + (long)n * g.ldc + i * 32) + at);
+                if (interior) { *reinterpret_cast<f32x4_u*>(p) = lo; *reinterpret_cast<f32x4_u*>(p + 4) = hi; }
+                else if (n < rows)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (i * 32 + j < cols) { const float v = j < 4 ? lo[j & 3] : hi[j & 3]; p[j] = g.accumulate ? p[j] + v : v; }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        if (!more) break;
+#pragma unroll
+        for (int m = 0; m < 8; ++m)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!interior) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+template <class F> int launch(F f, int threads, const Gemm8Args& g, int total, hipStream_t st) {
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES) != hipSuccess) return CLT_ERR_LAUNCH;
-    f<<<dim3((unsigned)(total < 256 ? total : 256)), dim3(256), LDS_BYTES, st>>>(g, total);
+    f<<<dim3((unsigned)(total < 256 ? total : 256)), dim3(threads), LDS_BYTES, st>>>(g, total);
     CLT_LAUNCH_CHECK();
     return CLT_OK;
 }
-template <int DT> int launch_fmt(const Gemm8Args& g, int fa, int fb, int total, hipStream_t st) {
-    if (fa == 0 && fb == 0) return launch<DT, 0, 0>(g, total, st);
-    if (fa == 1 && fb == 0) return launch<DT, 1, 0>(g, total, st);
-    if (fa == 0) return launch<DT, 0, 1>(g, total, st);
-    return launch<DT, 1, 1>(g, total, st);
+template <int FA, int FB> int launch_dtype(const Gemm8Args& g, int dtype, int total, hipStream_t st) {
+    if (dtype == CLT_DT_F32) return launch(gemm8_large_f32_kernel<FA, FB>, 512, g, total, st);
+    if (dtype == CLT_DT_BF16) return launch(gemm8_large_kernel<CLT_DT_BF16, FA, FB>, 256, g, total, st);
+    return launch(gemm8_large_kernel<CLT_DT_F16, FA, FB>, 256, g, total, st);
 }
 }  // namespace
 
@@ -319,7 +401,6 @@ int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, hip
     Gemm8Args g = g0;
     g.tilesA = (g.M - 1) / 256 + 1; g.tilesB = (g.N - 1) / 256 + 1;
     const int total = g.tilesA * g.tilesB * g.batch;
-    return dtype == CLT_DT_F32 ? launch_fmt<CLT_DT_F32>(g, fa, fb, total, st)
-           : dtype == CLT_DT_BF16 ? launch_fmt<CLT_DT_BF16>(g, fa, fb, total, st)
-                                  : launch_fmt<CLT_DT_F16>(g, fa, fb, total, st);
+    return fa == 0 ? (fb == 0 ? launch_dtype<0, 0>(g, dtype, total, st) : launch_dtype<0, 1>(g, dtype, total, st))
+                   : (fb == 0 ? launch_dtype<1, 0>(g, dtype, total, st) : launch_dtype<1, 1>(g, dtype, total, st));
 }
