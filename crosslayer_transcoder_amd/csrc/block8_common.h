@@ -25,17 +25,18 @@ __device__ __forceinline__ uint32_t finite_abs_bits(float x) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
     return b < 0x7f800000u ? b : 0u;
 }
-// four values, already scaled into the format's range -> four codes (nearest, ties to even)
-template <int FMT> __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
-    int r = 0;
+// four values / 2^e -> four codes (nearest, ties to even; the conversion takes the scale)
+template <int FMT> __device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d, float scale) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    s16x2 r = {0, 0};
     if constexpr (FMT) {
-        r = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, r, false);
-        r = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, r, true);
+        r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(r, a, b, scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_bf8_f32(r, c, d, scale, true);
     } else {
-        r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, r, false);
-        r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
     }
-    return (uint32_t)r;
+    return __builtin_bit_cast(uint32_t, r);
 }
 // four codes -> four values (unscaled, exact)
 typedef float b8_f32x2 __attribute__((ext_vector_type(2)));
@@ -53,6 +54,29 @@ template <int DT> __device__ __forceinline__ float elem_to_f32(typename Elem<DT>
     if constexpr (DT == CLT_DT_F32) return v;
     else if constexpr (DT == CLT_DT_BF16) return bf16_to_f32(v);
     else return f16_to_f32(v);
+}
+// 16-byte accesses to rows that are aligned to their element only (unaligned vector accesses are legal here)
+typedef uint32_t b8_u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
+typedef float b8_f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+// 8 consecutive elements of a row as fp32; `n` valid, the rest 0
+template <int DT> __device__ __forceinline__ void b8_load8(const typename Elem<DT>::type* p, int n, float v[8]) {
+    if (n >= 8) {
+        if constexpr (DT == CLT_DT_F32) {
+            const b8_f32x4_u a = reinterpret_cast<const b8_f32x4_u*>(p)[0], b = reinterpret_cast<const b8_f32x4_u*>(p + 4)[0];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { v[k] = a[k]; v[k + 4] = b[k]; }
+        } else {
+            const b8_u32x4_u u = *reinterpret_cast<const b8_u32x4_u*>(p);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[2 * k] = elem_to_f32<DT>((uint16_t)(u[k] & 0xffffu));
+                v[2 * k + 1] = elem_to_f32<DT>((uint16_t)(u[k] >> 16));
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = k < n ? elem_to_f32<DT>(p[k]) : 0.0f;
+    }
 }
 // two fp32 -> one dword of 16-bit results, nearest even (fp16: overflow gives inf; the loss scaler's flag is not touched here)
 template <int DT> __device__ __forceinline__ uint32_t pack_out16(float lo, float hi) {

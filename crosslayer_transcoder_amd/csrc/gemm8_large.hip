@@ -36,9 +36,8 @@ template <int N, class F> __device__ __forceinline__ void unroll(F f) {
     if constexpr (N > 0) { unroll<N - 1>(f); f(std::integral_constant<int, N - 1>{}); }
 }
 
-// 16-byte stores of rows that are aligned to their element only
-typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
-typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef b8_u32x4_u u32x4_u;
+typedef b8_f32x4_u f32x4_u;
 
 struct Tile { int batch, a0, b0; };
 // block -> tile: every XCD (block index mod 8) works on a contiguous range of tiles, walked in panels of 4 A tiles with the A tile

@@ -12,34 +12,12 @@
 
 namespace {
 
-// 8 consecutive elements of a row into fp32; `n` valid (the rest 0); vec: 16-byte loads allowed
-template <int DT> __device__ __forceinline__ void load8(const typename Elem<DT>::type* p, int n, bool vec, float v[8]) {
-    if (n >= 8 && vec) {
-        if constexpr (DT == CLT_DT_F32) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                v[2 * k] = elem_to_f32<DT>((uint16_t)(w[k] & 0xffffu));
-                v[2 * k + 1] = elem_to_f32<DT>((uint16_t)(w[k] >> 16));
-            }
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = k < n ? elem_to_f32<DT>(p[k]) : 0.0f;
-    }
-}
-
 struct Pack8Args {
     const void* x; long row_stride, batch_stride;
     uint8_t *q, *s;            // row form (or nullptr): codes [L][R][Cp], scale bytes [L][Cp / 128][Rp]
     uint8_t *qt, *st;          // transposed form (or nullptr): codes [L][C][Rp], scale bytes [L][Rp / 128][Cp]
     float* sums;               // column sums of each 128-row block [L][Rp / 128][C] (or nullptr)
     int R, C, tiles_r, tiles_c;
-    bool vec;
 };
 
 template <int DT, int FMT, bool TILES> __global__ __launch_bounds__(256) void pack8_kernel(Pack8Args a) {
@@ -62,20 +40,28 @@ template <int DT, int FMT, bool TILES> __global__ __launch_bounds__(256) void pa
     for (int i = 0; i < 8; ++i) {
         const int r = r0 + rg * 8 + i;
         const T* p = static_cast<const T*>(a.x) + b * a.batch_stride + (long)r * a.row_stride + c0 + cg * 8;
-        load8<DT>(p, r < a.R ? nc : 0, a.vec, v[i]);
+        b8_load8<DT>(p, r < a.R ? nc : 0, v[i]);
     }
-    // maxima of the finite magnitudes, per row (over the 16 lanes of a row) and per column (over rows: 4 lanes, 4 waves)
+    // maxima of the finite magnitudes, per row (over the 16 lanes of a row) and per column (over rows: 4 lanes, 4 waves).  As unsigned
+    // integers the magnitudes of inf and NaN are larger than every finite one: only where one shows up are they sorted out.
     uint32_t rm[8], cm[8];
+    auto maxima = [&](auto bits) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) rm[k] = cm[k] = 0u;
+        for (int k = 0; k < 8; ++k) rm[k] = cm[k] = 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t m = finite_abs_bits(v[i][j]);
-            rm[i] = max(rm[i], m);
-            cm[j] = max(cm[j], m);
-        }
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t m = bits(v[i][j]);
+                rm[i] = max(rm[i], m);
+                cm[j] = max(cm[j], m);
+            }
+    };
+    maxima([](float x) { return __float_as_uint(x) & 0x7fffffffu; });
+    uint32_t most = 0u;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) most = max(most, rm[k]);
+    if (most >= 0x7f800000u) maxima([](float x) { return finite_abs_bits(x); });
     if (TILES) {
         uint32_t m = 0u;
 #pragma unroll
@@ -133,11 +119,11 @@ template <int DT, int FMT, bool TILES> __global__ __launch_bounds__(256) void pa
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int e = block_exponent<FMT>(rm[i]), r = r0 + rg * 8 + i;
-            const float f = exp2_int(-e);
+            const float f = exp2_int(e);
             sb[i >> 2] |= (uint32_t)(e + 127) << (8 * (i & 3));
             uint2 o;
-            o.x = pack_codes<FMT>(v[i][0] * f, v[i][1] * f, v[i][2] * f, v[i][3] * f);
-            o.y = pack_codes<FMT>(v[i][4] * f, v[i][5] * f, v[i][6] * f, v[i][7] * f);
+            o.x = pack_codes<FMT>(v[i][0], v[i][1], v[i][2], v[i][3], f);
+            o.y = pack_codes<FMT>(v[i][4], v[i][5], v[i][6], v[i][7], f);
             if (r < a.R) *reinterpret_cast<uint2*>(a.q + (b * a.R + r) * Cp + c0 + cg * 8) = o;
         }
         if (cg == 0) *reinterpret_cast<uint2*>(a.s + (b * a.tiles_c + tc) * Rp + r0 + rg * 8) = make_uint2(sb[0], sb[1]);
@@ -147,11 +133,11 @@ template <int DT, int FMT, bool TILES> __global__ __launch_bounds__(256) void pa
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int e = block_exponent<FMT>(cm[j]), c = cg * 8 + j;
-            const float f = exp2_int(-e);
+            const float f = exp2_int(e);
             sb[j >> 2] |= (uint32_t)(e + 127) << (8 * (j & 3));
             uint2 o;
-            o.x = pack_codes<FMT>(v[0][j] * f, v[1][j] * f, v[2][j] * f, v[3][j] * f);
-            o.y = pack_codes<FMT>(v[4][j] * f, v[5][j] * f, v[6][j] * f, v[7][j] * f);
+            o.x = pack_codes<FMT>(v[0][j], v[1][j], v[2][j], v[3][j], f);
+            o.y = pack_codes<FMT>(v[4][j], v[5][j], v[6][j], v[7][j], f);
             // 8-byte chunk rg of column c, chunks XOR-swizzled with the column group (the 16 groups of a store hit 16 chunks)
             *reinterpret_cast<uint2*>(tile + c * B8 + ((rg ^ cg) << 3)) = o;
         }
@@ -181,7 +167,7 @@ __global__ __launch_bounds__(256) void fold_sums_kernel(const float* part, float
 // codes -> values 2^e x code, rounded once to the output type; 16 codes a thread (bound: HBM, 1 + es bytes an element)
 template <int DT> __global__ __launch_bounds__(256) void unpack8_kernel(const uint8_t* q, const uint8_t* s, int fmt, int R, int C,
                                                                         long pitch, long Rp, long q_batch, long s_batch, void* out,
-                                                                        int chunks, long total, bool vec) {
+                                                                        int chunks, long total) {
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
     if (id >= total) return;
     const long row = id / chunks;                        // row of the whole batch
@@ -192,16 +178,16 @@ template <int DT> __global__ __launch_bounds__(256) void unpack8_kernel(const ui
     const float f = exp2_int((int)s[b * s_batch + (long)(c >> 7) * Rp + r] - 127);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     typename Elem<DT>::type* o = static_cast<typename Elem<DT>::type*>(out) + row * C + c;
-    if (vec) {                                           // C % 16 == 0 and an aligned base: whole 16-element pieces
+    if (c + 16 <= C) {
 #pragma unroll
         for (int k = 0; k < 4; k += 2) {
             const b8_f32x4 x = unpack_codes(fmt, w[k]) * f, y = unpack_codes(fmt, w[k + 1]) * f;
             if constexpr (DT == CLT_DT_F32) {
-                reinterpret_cast<float4*>(o)[k] = make_float4(x[0], x[1], x[2], x[3]);
-                reinterpret_cast<float4*>(o)[k + 1] = make_float4(y[0], y[1], y[2], y[3]);
+                reinterpret_cast<b8_f32x4_u*>(o)[k] = x;
+                reinterpret_cast<b8_f32x4_u*>(o)[k + 1] = y;
             } else
-                reinterpret_cast<uint4*>(o)[k >> 1] = make_uint4(pack_out16<DT>(x[0], x[1]), pack_out16<DT>(x[2], x[3]),
-                                                                 pack_out16<DT>(y[0], y[1]), pack_out16<DT>(y[2], y[3]));
+                reinterpret_cast<b8_u32x4_u*>(o)[k >> 1] = b8_u32x4_u{pack_out16<DT>(x[0], x[1]), pack_out16<DT>(x[2], x[3]),
+                                                                      pack_out16<DT>(y[0], y[1]), pack_out16<DT>(y[2], y[3])};
         }
     } else {
 #pragma unroll
@@ -242,7 +228,6 @@ extern "C" int clt_pack8(const void* x, int dtype, long row_stride, long batch_s
     const size_t need = clt_pack8_sums_workspace_bytes(batch, rows, cols);
     if (column_sums && (!workspace || workspace_bytes < need)) return CLT_ERR_WORKSPACE;
     a.sums = column_sums ? static_cast<float*>(workspace) : nullptr;
-    a.vec = aligned16(x) && row_stride % (long)(16 / es) == 0 && batch_stride % (long)(16 / es) == 0;
     const long blocks = (long)batch * a.tiles_r * a.tiles_c;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
     const hipStream_t hs = as_stream(stream);
@@ -262,14 +247,13 @@ extern "C" int clt_unpack8(const void* q, const void* s, int format, int batch, 
     if (pitch < up128(cols) || scale_pitch < rows) return CLT_ERR_SHAPE;
     const size_t es = dtype == CLT_DT_F32 ? 4 : 2;
     if (!aligned16(q) || pitch % 16 || q_batch_stride % 16 || ((uintptr_t)out & (es - 1))) return CLT_ERR_ALIGN;
-    const bool vec = aligned16(out) && cols % 16 == 0;
     const int chunks = (cols - 1) / 16 + 1;
     const long total = (long)batch * rows * chunks, blocks = (total + 255) / 256;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
     const dim3 g((unsigned)blocks), t(256);
     const hipStream_t hs = as_stream(stream);
     const uint8_t *qp = static_cast<const uint8_t*>(q), *sp = static_cast<const uint8_t*>(s);
-#define UNPACK(DT) unpack8_kernel<DT><<<g, t, 0, hs>>>(qp, sp, format, rows, cols, pitch, scale_pitch, q_batch_stride, s_batch_stride, out, chunks, total, vec)
+#define UNPACK(DT) unpack8_kernel<DT><<<g, t, 0, hs>>>(qp, sp, format, rows, cols, pitch, scale_pitch, q_batch_stride, s_batch_stride, out, chunks, total)
     if (dtype == CLT_DT_F32) UNPACK(CLT_DT_F32); else if (dtype == CLT_DT_BF16) UNPACK(CLT_DT_BF16); else UNPACK(CLT_DT_F16);
 #undef UNPACK
     CLT_LAUNCH_CHECK();

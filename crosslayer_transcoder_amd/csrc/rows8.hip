@@ -24,27 +24,10 @@ struct Rows8Args {
     void* y; long y_token, y_layer; int y_dtype;     // results, or
     float* part;                                     // partial sums [slice][layer][token][N] when K is cut
     int T, N, K, KB, slice_kb, slices, chunks, row_blocks, layers;
-    int x_dtype, vec, y_vec;
+    int x_dtype, y_vec;
 };
 
 extern __shared__ __attribute__((aligned(16))) unsigned char r8_smem[];
-
-template <int DT> __device__ __forceinline__ void load_x8(const void* x, long at, int n, bool vec, float v[8]) {
-    const typename Elem<DT>::type* p = static_cast<const typename Elem<DT>::type*>(x) + at;
-    if (vec && n >= 8) {
-        if constexpr (DT == CLT_DT_F32) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const uint32_t q[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) { v[2 * k] = elem_to_f32<DT>((uint16_t)(q[k] & 0xffffu)); v[2 * k + 1] = elem_to_f32<DT>((uint16_t)(q[k] >> 16)); }
-        }
-    } else
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = k < n ? elem_to_f32<DT>(p[k]) : 0.0f;
-}
 
 // `valid` of four consecutive results; whole: one store (valid >= 4 and the row's alignment allows it)
 __device__ __forceinline__ void store_result(void* y, int dtype, long at, f32x4 v, int valid, bool whole) {
@@ -97,9 +80,9 @@ template <int MT, int G, int FMT> __global__ __launch_bounds__(WAVES * 64, MT >=
     auto load_item = [&](int id, float* v) {
         const int t = id / nkb, kb = id - t * nkb, k = (kb0 + kb) * 128 + fr * 8;
         const long at = t * a.x_token + layer * a.x_layer + k;
-        if (a.x_dtype == CLT_DT_F32) load_x8<CLT_DT_F32>(a.x, at, a.K - k, a.vec, v);
-        else if (a.x_dtype == CLT_DT_BF16) load_x8<CLT_DT_BF16>(a.x, at, a.K - k, a.vec, v);
-        else load_x8<CLT_DT_F16>(a.x, at, a.K - k, a.vec, v);
+        if (a.x_dtype == CLT_DT_F32) b8_load8<CLT_DT_F32>(static_cast<const float*>(a.x) + at, a.K - k, v);
+        else if (a.x_dtype == CLT_DT_BF16) b8_load8<CLT_DT_BF16>(static_cast<const uint16_t*>(a.x) + at, a.K - k, v);
+        else b8_load8<CLT_DT_F16>(static_cast<const uint16_t*>(a.x) + at, a.K - k, v);
     };
     auto pack_item = [&](int id, const float* v) {
         const int t = id / nkb, kb = id - t * nkb;
@@ -109,8 +92,8 @@ template <int MT, int G, int FMT> __global__ __launch_bounds__(WAVES * 64, MT >=
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
         const int e = block_exponent<0>(m);
-        const float f = exp2_int(-e), g = exp2_int(e);
-        const uint32_t lo = pack_codes<0>(v[0] * f, v[1] * f, v[2] * f, v[3] * f), hi = pack_codes<0>(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+        const float g = exp2_int(e);
+        const uint32_t lo = pack_codes<0>(v[0], v[1], v[2], v[3], g), hi = pack_codes<0>(v[4], v[5], v[6], v[7], g);
         *reinterpret_cast<bf16x8*>(r8_smem + t * pitch + kb * 256 + fr * 16) = widen8<0>(lo, hi, g);
     };
     const int items = a.T * nkb, first = tid >> 4;
@@ -284,7 +267,6 @@ extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride,
     a.y = y; a.y_token = y_token_stride; a.y_layer = y_layer_stride; a.y_dtype = y_dtype;
     a.part = c.slices > 1 ? static_cast<float*>(workspace) : nullptr;
     a.T = tokens; a.N = N; a.K = K; a.KB = KB; a.slice_kb = c.slice_kb; a.slices = c.slices; a.chunks = c.chunks; a.row_blocks = c.row_blocks; a.layers = layers;
-    a.vec = aligned16(x) && x_token_stride % (long)(16 / xs) == 0 && x_layer_stride % (long)(16 / xs) == 0;
     a.y_vec = (uintptr_t)y % (4 * ys) == 0 && y_token_stride % 4 == 0 && y_layer_stride % 4 == 0;
     const long blocks = (long)layers * c.slices * c.row_blocks;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
