@@ -103,8 +103,17 @@ struct Gemm8Args {
     long ba, bas, bb, bbs, bc, bbias;        // batch strides
     int M, N, KB, tilesA, tilesB;
     int accumulate, batch;
+    uint32_t inv_tiles, inv_panel, inv_rem;  // reciprocals of the large form's tile order (fast_div)
     int slices, slice_kb; float* part;       // K in slices: partial sums [slice][batch][M][N], else nullptr
 };
+
+// n / d for n < 2^31 with inv = (2^32 - 1) / d from the host: the estimate is at most one too small.  (A division in a kernel costs a
+// few hundred cycles of dependent vector instructions, and a lone wave per SIMD has nothing to put under them.)
+__device__ __forceinline__ int fast_div(int n, int d, uint32_t inv) {
+    int q = (int)__umulhi((uint32_t)n, inv);
+    if (n - q * d >= d) ++q;
+    return q;
+}
 
 // 256 x 256 tiles (gemm8_large.hip): the shapes that take them, and the launch
 bool clt_internal_gemm8_large_applies(int M, int N, int KB, int batch);

@@ -251,7 +251,7 @@ extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long 
     if (KB && (256 * lda > 0x7fffffffL || 256 * ldb > 0x7fffffffL || KB * ldas > 0x7ffffeffL || KB * ldbs > 0x7ffffeffL)) return CLT_ERR_RANGE;
     Gemm8Args g = {static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(a_scale), static_cast<const uint8_t*>(b),
                    static_cast<const uint8_t*>(b_scale), c, bias, lda, ldas, ldb, ldbs, ldc, a_batch, as_batch, b_batch, bs_batch,
-                   c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 1, KB, nullptr};
+                   c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 0u, 0u, 0u, 1, KB, nullptr};
     const hipStream_t st = as_stream(stream);
     if (clt_internal_gemm8_large_applies(M, N, KB, batch) && 256 * ldc * 4 <= 0x7fffffffL) return clt_internal_gemm8_large(g, a_format, b_format, c_dtype, st);
     // (a result whose rows lie further apart than the large form's offsets reach runs here, unsliced: no workspace was asked for)

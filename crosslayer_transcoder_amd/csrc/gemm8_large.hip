@@ -13,7 +13,9 @@
 // c(4 q + i) = 4 i + q (B), so fragment j of a wave is rows 8 * lane + j: (a) the scale bytes of a lane's eight fragments are eight
 // consecutive bytes — one 8-byte read per operand and block, the instruction picks its byte by op_sel; (b) a lane's
 // accumulators of the eight B fragments are eight consecutive columns of C — 16 bytes of 16-bit results, 32 of fp32 — and four
-// lanes make 64 / 128 consecutive bytes: stores need no transposition.
+// lanes make 64 / 128 consecutive bytes.  16-bit results pass through a 4 KB slab of LDS a wave, so that 256 bytes of a row leave
+// together, and past the caches, which hold the operands' panels (4096 x 768 x 32768 x 12: 1728 -> 1462 us; without the slab the
+// uncached stores are slower than cached ones, 1765 us).
 #include <type_traits>
 #include "block8_common.h"
 
@@ -27,7 +29,9 @@ constexpr int OPB = 256 * 128;                        // one operand's block in 
 constexpr int STG = 2 * OPB;
 constexpr int SCALE_BASE = 2 * STG;                   // per buffer: 256 scale bytes of A, 256 of B
 constexpr int BIAS_BASE = SCALE_BASE + 2 * 512;       // four slots of 256 floats (a tile's, while up to two more are on their way)
-constexpr int LDS_BYTES = BIAS_BASE + 4 * 1024;
+constexpr int SLAB_BASE = BIAS_BASE + 4 * 1024;       // a slab a wave: 16 rows of 128 16-bit results (padded against conflicts)
+constexpr int SLAB_ROW = 256 + 16, SLAB = 16 * SLAB_ROW;
+constexpr int LDS_BYTES = SLAB_BASE + 4 * SLAB;
 static_assert(LDS_BYTES <= 160 * 1024, "LDS");
 extern __shared__ __attribute__((aligned(1024))) unsigned char g8_smem[];
 typedef __attribute__((address_space(3))) void lds_void;
@@ -38,22 +42,23 @@ template <int N, class F> __device__ __forceinline__ void unroll(F f) {
 
 typedef b8_u32x4_u u32x4_u;
 typedef b8_f32x4_u f32x4_u;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+constexpr int GA = 4;                                 // A tiles of a panel
 struct Tile { int batch, a0, b0; };
 // block -> tile: every XCD (block index mod 8) works on a contiguous range of tiles, walked in panels of 4 A tiles with the A tile
 // fastest, so that the blocks an XCD runs together share operand tiles in its L2
 __device__ __forceinline__ Tile decode_tile(const Gemm8Args& g, int vb) {
     const int nwg = g.tilesA * g.tilesB;
     Tile t;
-    t.batch = vb / nwg;
+    t.batch = fast_div(vb, nwg, g.inv_tiles);
     int lid = vb - t.batch * nwg;
     const int xcd = lid & 7, q = nwg >> 3, r = nwg & 7;
     lid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lid >> 3);
-    constexpr int GA = 4;
     const int full = g.tilesA / GA, rem = g.tilesA - full * GA, per = GA * g.tilesB;
     int ta, tb;
-    if (lid < full * per) { const int pn = lid / per, x = lid - pn * per; tb = x / GA; ta = pn * GA + (x - tb * GA); }
-    else { const int x = lid - full * per; tb = x / rem; ta = full * GA + (x - tb * rem); }
+    if (lid < full * per) { const int pn = fast_div(lid, per, g.inv_panel), x = lid - pn * per; tb = x / GA; ta = pn * GA + (x - tb * GA); }
+    else { const int x = lid - full * per; tb = fast_div(x, rem, g.inv_rem); ta = full * GA + (x - tb * rem); }
     t.a0 = ta * 256; t.b0 = tb * 256;
     return t;
 }
@@ -192,31 +197,42 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
         const bool more = vb < total;
         if (more) t = decode(vb);
         nt = decode(svb + (int)gridDim.x);
-        // ---- results: for (n, i) a lane has row 8 fr + n and eight columns 8 (4 i + fq) ..
+        // ---- results: for (n, i) a lane has row 8 fr + n and eight columns 8 (4 i + fq) .. of its wave's 128 x 128: 16 bytes.  Row by row
+        // (n) they pass through the wave's own slab of LDS, so that 16 lanes store 256 consecutive bytes.
         typedef typename Elem<DT>::type T;
-        const int r0 = wa * 128 + fr * 8, c0 = wb * 128 + fq * 8;
-        const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N;
-        T* ctile = static_cast<T*>(g.c) + cur.batch * g.bc + (long)cur.a0 * g.ldc + cur.b0;
-        const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + c0;
-        const bool has_bias = g.bias != nullptr;
-        const int rows = g.M - cur.a0 - r0, cols = g.N - cur.b0 - c0;
-        const unsigned at = (unsigned)(r0 * (int)g.ldc + c0) * (unsigned)sizeof(T);      // a lane's offset in the tile: 32 bits (host check)
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
+        const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N, has_bias = g.bias != nullptr;
+        const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + wb * 128 + fq * 8;
+        T* ctile = static_cast<T*>(g.c) + cur.batch * g.bc + (long)(cur.a0 + wa * 128) * g.ldc + cur.b0 + wb * 128;
+        unsigned char* slab = g8_smem + SLAB_BASE + w * SLAB;
+        const int wr = fr * SLAB_ROW + fq * 16, rd = fq * SLAB_ROW + fr * 16;
+        const unsigned at = (unsigned)(fq * 8 * (int)g.ldc + fr * 8) * (unsigned)sizeof(T);      // a lane's offset: 32 bits (host check)
+        const int rows = g.M - (cur.a0 + wa * 128 + fq * 8), cols = g.N - (cur.b0 + wb * 128 + fr * 8);
+        auto put = [&](int n) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 f32x4 lo = f32x4{acc[0][n][i], acc[1][n][i], acc[2][n][i], acc[3][n][i]};
                 f32x4 hi = f32x4{acc[4][n][i], acc[5][n][i], acc[6][n][i], acc[7][n][i]};
                 if (has_bias) { lo += *reinterpret_cast<const f32x4*>(bl + i * 32); hi += *reinterpret_cast<const f32x4*>(bl + i * 32 + 4); }
-                T* p = reinterpret_cast<T*>(reinterpret_cast<char*>(ctile + (long)n * g.ldc + i * 32) + at);
-                const u32x4_u u = {pack_out16<DT>(lo[0], lo[1]), pack_out16<DT>(lo[2], lo[3]), pack_out16<DT>(hi[0], hi[1]), pack_out16<DT>(hi[2], hi[3])};
-                if (interior) *reinterpret_cast<u32x4_u*>(p) = u;
-                else if (n < rows)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (i * 32 + j < cols) p[j] = (T)(u[j >> 1] >> (16 * (j & 1)));
-                __builtin_amdgcn_sched_barrier(0);
+                *reinterpret_cast<u32x4*>(slab + wr + i * 64) = u32x4{pack_out16<DT>(lo[0], lo[1]), pack_out16<DT>(lo[2], lo[3]), pack_out16<DT>(hi[0], hi[1]), pack_out16<DT>(hi[2], hi[3])};
             }
+        };
+        put(0);
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            u32x4 v[4];                                   // (a wave's LDS operations execute in order: the next row group may follow at once)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const u32x4*>(slab + rd + k * 4 * SLAB_ROW);
+            if (n < 7) put(n + 1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {                 // rows (4 k + fq) * 8 + n
+                const u32x4 u = v[k];
+                T* p = reinterpret_cast<T*>(reinterpret_cast<char*>(ctile + (long)(k * 32 + n) * g.ldc) + at);
+                if (interior) __builtin_nontemporal_store((u32x4_u)u, reinterpret_cast<u32x4_u*>(p));
+                else if (k * 32 + n < rows)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) if (j < cols) p[j] = (T)(u[j >> 1] >> (16 * (j & 1)));
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         if (!more) break;
 #pragma unroll
@@ -399,7 +415,10 @@ bool clt_internal_gemm8_large_applies(int M, int N, int KB, int batch) {
 int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, hipStream_t st) {
     Gemm8Args g = g0;
     g.tilesA = (g.M - 1) / 256 + 1; g.tilesB = (g.N - 1) / 256 + 1;
-    const int total = g.tilesA * g.tilesB * g.batch;
+    const int total = g.tilesA * g.tilesB * g.batch, rem = g.tilesA % GA;
+    g.inv_tiles = 0xffffffffu / (uint32_t)(g.tilesA * g.tilesB);
+    g.inv_panel = 0xffffffffu / (uint32_t)(GA * g.tilesB);
+    g.inv_rem = rem ? 0xffffffffu / (uint32_t)rem : 0u;
     return fa == 0 ? (fb == 0 ? launch_dtype<0, 0>(g, dtype, total, st) : launch_dtype<0, 1>(g, dtype, total, st))
                    : (fb == 0 ? launch_dtype<1, 0>(g, dtype, total, st) : launch_dtype<1, 1>(g, dtype, total, st));
 }

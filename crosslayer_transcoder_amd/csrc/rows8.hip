@@ -1,4 +1,4 @@
-// y [T][L][N] = x [T][L][K] * w [L][N][K]^T + bias for few tokens (T <= 64) and kept 8-bit weights: the serving form of a linear
+// y [T][L][N] = x [T][L][K] * w [L][N][K]^T + bias for few tokens (T <= 32) and kept 8-bit weights: the serving form of a linear
 // map.  x is packed (e4m3, blocks along K) on the way; products are exact and sums fp32 whatever the result's type (bf16 matrix
 // instructions on the values held, as clt_gemm8's fp32 form).
 //
@@ -14,8 +14,10 @@
 namespace {
 typedef b8_f32x4 f32x4;
 typedef b8_bf16x8 bf16x8;
-constexpr int WAVES = 8, MAX_T = 64;
+constexpr int WAVES = 8, MAX_T = 32;
 constexpr int LDS_CAP = 136 * 1024;                  // packed slice of x at most
+// (64 tokens: packing and the tiled product are as fast or faster, 129 against 138 us for 768 -> 32768 x 12 layers, 47 against 101 for
+// 4096 -> 32768; 32 tokens: 121 against 81 and 24 against 26 for 32768 -> 768)
 
 struct Rows8Args {
     const void* x; long x_token, x_layer;            // strides in elements
@@ -51,8 +53,8 @@ __device__ __forceinline__ void store_result(void* y, int dtype, long at, f32x4 
 
 // MT: groups of 16 tokens; G: groups of 16 weight rows a wave has in hand; FMT: format of the weights.  A step is G x 16 rows x 128 k;
 // D steps are in flight.
-template <int MT, int G, int FMT> __global__ __launch_bounds__(WAVES * 64, MT >= 4 ? 2 : 4) void rows8_kernel(Rows8Args a) {
-    constexpr int D = G == 1 && MT < 4 ? 4 : 2;
+template <int MT, int G, int FMT> __global__ __launch_bounds__(WAVES * 64, 4) void rows8_kernel(Rows8Args a) {
+    constexpr int D = G == 1 ? 4 : 2;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
     const int rbk = blockIdx.x % a.row_blocks, rest = blockIdx.x / a.row_blocks, slice = rest % a.slices, layer = rest / a.slices;
     const int kb0 = slice * a.slice_kb, nkb = min(a.slice_kb, a.KB - kb0);
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(256) void rows8_fold_kernel(Rows8Args a, long n) {
 struct Cut { int slice_kb, slices, g, chunks, row_blocks; };
 Cut cut_rows8(int T, int L, int N, int KB) {
     Cut c;
-    const int fit = (LDS_CAP / T - 16) / 256;                            // blocks of k whose x fits LDS (>= 8 for 64 tokens)
+    const int fit = (LDS_CAP / T - 16) / 256;                            // blocks of k whose x fits LDS (>= 16 for 32 tokens)
     const long rb = (N + WAVES * 16 - 1) / (WAVES * 16), want = 512;
     long slices = (KB + fit - 1) / fit;
     if (L * rb * slices < want) {
@@ -274,8 +276,7 @@ extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride,
     const hipStream_t st = as_stream(stream);
     int rc;
     if (tokens <= 16) rc = c.g == 1 ? launch_rows<1, 1>(a, w_format, blocks, lds, st) : launch_rows<1, 2>(a, w_format, blocks, lds, st);
-    else if (tokens <= 32) rc = launch_rows<2, 1>(a, w_format, blocks, lds, st);
-    else rc = launch_rows<4, 1>(a, w_format, blocks, lds, st);
+    else rc = launch_rows<2, 1>(a, w_format, blocks, lds, st);
     if (rc != CLT_OK || c.slices == 1) return rc;
     const long n = (long)layers * tokens * N, fold = (n + 255) / 256;
     if (fold > 0x7fffffffL) return CLT_ERR_RANGE;

@@ -17,7 +17,7 @@ from ._lib import CltError, lib
 BLOCK = 128
 FORMATS = {"e4m3": 0, "e5m2": 1}
 #: tokens up to which linear8 streams the weights past all of them in one launch (clt_linear8_rows)
-FEW_TOKENS = 64
+FEW_TOKENS = 32
 _DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
