@@ -105,6 +105,7 @@ struct Gemm8Args {
     int accumulate, batch;
     uint32_t inv_tiles, inv_panel, inv_rem;  // reciprocals of the large form's tile order (fast_div)
     int slices, slice_kb; float* part;       // K in slices: partial sums [slice][batch][M][N], else nullptr
+    long slice_stride;                       // of the results (large form)
 };
 
 // n / d for n < 2^31 with inv = (2^32 - 1) / d from the host: the estimate is at most one too small.  (A division in a kernel costs a
@@ -115,8 +116,8 @@ __device__ __forceinline__ int fast_div(int n, int d, uint32_t inv) {
     return q;
 }
 
-// 256 x 256 tiles (gemm8_large.hip): the shapes that take them, and the launch
-bool clt_internal_gemm8_large_applies(int M, int N, int KB, int batch);
+// 256 x 256 tiles (gemm8_large.hip): the shapes that take them (0: none; else slices of K), and the launch
+int clt_internal_gemm8_large_slices(int M, int N, int KB, int batch);
 int clt_internal_gemm8_large(const Gemm8Args& g, int fa, int fb, int dtype, hipStream_t st);
 
 // Four consecutive columns of a row of C: one store where the row's alignment allows it (vec), else element by element

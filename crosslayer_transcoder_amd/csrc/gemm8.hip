@@ -215,10 +215,7 @@ template <int DT, int FA, int FB> int launch_fmt(const Gemm8Args& g, long blocks
     CLT_LAUNCH_CHECK();
     return CLT_OK;
 }
-template <int DT> int launch(const Gemm8Args& g, int fa, int fb, long blocks, hipStream_t st) {
-    const int rc = fa == 0 ? (fb == 0 ? launch_fmt<DT, 0, 0>(g, blocks, st) : launch_fmt<DT, 0, 1>(g, blocks, st))
-                           : (fb == 0 ? launch_fmt<DT, 1, 0>(g, blocks, st) : launch_fmt<DT, 1, 1>(g, blocks, st));
-    if (rc != CLT_OK || !g.part) return rc;
+template <int DT> int fold(const Gemm8Args& g, hipStream_t st) {
     const int quads = (g.N - 1) / 4 + 1;
     const long total = (long)g.batch * g.M * quads, fold = (total + 255) / 256;
     if (fold > 0x7fffffffL) return CLT_ERR_RANGE;
@@ -226,13 +223,17 @@ template <int DT> int launch(const Gemm8Args& g, int fa, int fb, long blocks, hi
     CLT_LAUNCH_CHECK();
     return CLT_OK;
 }
+template <int DT> int launch(const Gemm8Args& g, int fa, int fb, long blocks, hipStream_t st) {
+    const int rc = fa == 0 ? (fb == 0 ? launch_fmt<DT, 0, 0>(g, blocks, st) : launch_fmt<DT, 0, 1>(g, blocks, st))
+                           : (fb == 0 ? launch_fmt<DT, 1, 0>(g, blocks, st) : launch_fmt<DT, 1, 1>(g, blocks, st));
+    return rc != CLT_OK || !g.part ? rc : fold<DT>(g, st);
+}
 }  // namespace
 
 extern "C" size_t clt_gemm8_workspace_bytes(int M, int N, int K, int batch) {
     if (M <= 0 || N <= 0 || K <= 0 || batch <= 0) return 0;
-    const int KB = (int)(up128(K) / 128);
-    if (clt_internal_gemm8_large_applies(M, N, KB, batch)) return 0;
-    const int s = slices_of(M, N, KB, batch);
+    const int KB = (int)(up128(K) / 128), large = clt_internal_gemm8_large_slices(M, N, KB, batch);
+    const int s = large ? large : slices_of(M, N, KB, batch);
     return s > 1 ? (size_t)s * batch * M * N * 4 : 0;
 }
 
@@ -251,15 +252,22 @@ extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long 
     if (KB && (256 * lda > 0x7fffffffL || 256 * ldb > 0x7fffffffL || KB * ldas > 0x7ffffeffL || KB * ldbs > 0x7ffffeffL)) return CLT_ERR_RANGE;
     Gemm8Args g = {static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(a_scale), static_cast<const uint8_t*>(b),
                    static_cast<const uint8_t*>(b_scale), c, bias, lda, ldas, ldb, ldbs, ldc, a_batch, as_batch, b_batch, bs_batch,
-                   c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 0u, 0u, 0u, 1, KB, nullptr};
+                   c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 0u, 0u, 0u, 1, KB, nullptr, 0};
     const hipStream_t st = as_stream(stream);
-    if (clt_internal_gemm8_large_applies(M, N, KB, batch) && 256 * ldc * 4 <= 0x7fffffffL) return clt_internal_gemm8_large(g, a_format, b_format, c_dtype, st);
-    // (a result whose rows lie further apart than the large form's offsets reach runs here, unsliced: no workspace was asked for)
-    if (!clt_internal_gemm8_large_applies(M, N, KB, batch)) g.slices = slices_of(M, N, KB, batch);
+    int large = clt_internal_gemm8_large_slices(M, N, KB, batch);
+    // (results whose rows lie further apart than the large form's offsets reach: small tiles, unsliced)
+    const bool far = large == 1 && 256 * ldc * 4 > 0x7fffffffL;
+    g.slices = far ? 1 : large ? large : slices_of(M, N, KB, batch);
+    if (far || (large > 1 && 1024L * N > 0x7fffffffL)) large = 0;
     if (g.slices > 1) {
         if (!workspace || !aligned16(workspace) || workspace_bytes < clt_gemm8_workspace_bytes(M, N, K, batch)) return CLT_ERR_WORKSPACE;
         g.part = static_cast<float*>(workspace);
         g.slice_kb = (KB + g.slices - 1) / g.slices;
+    }
+    if (large) {
+        const int rc = clt_internal_gemm8_large(g, a_format, b_format, c_dtype, st);
+        if (rc != CLT_OK || !g.part) return rc;
+        return c_dtype == CLT_DT_F32 ? fold<CLT_DT_F32>(g, st) : c_dtype == CLT_DT_BF16 ? fold<CLT_DT_BF16>(g, st) : fold<CLT_DT_F16>(g, st);
     }
     const long blocks = (long)g.tilesA * g.tilesB * batch * g.slices;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;

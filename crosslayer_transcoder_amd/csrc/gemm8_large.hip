@@ -45,7 +45,7 @@ typedef b8_f32x4_u f32x4_u;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int GA = 4;                                 // A tiles of a panel
-struct Tile { int batch, a0, b0; };
+struct Tile { int batch, slice, a0, b0; };
 // block -> tile: every XCD (block index mod 8) works on a contiguous range of tiles, walked in panels of 4 A tiles with the A tile
 // fastest, so that the blocks an XCD runs together share operand tiles in its L2
 __device__ __forceinline__ Tile decode_tile(const Gemm8Args& g, int vb) {
@@ -53,6 +53,8 @@ __device__ __forceinline__ Tile decode_tile(const Gemm8Args& g, int vb) {
     Tile t;
     t.batch = fast_div(vb, nwg, g.inv_tiles);
     int lid = vb - t.batch * nwg;
+    t.slice = 0;
+    if (g.slices > 1) { t.slice = t.batch / g.slices; t.slice = t.batch - t.slice * g.slices; t.batch = (t.batch - t.slice) / g.slices; }
     const int xcd = lid & 7, q = nwg >> 3, r = nwg & 7;
     lid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lid >> 3);
     const int full = g.tilesA / GA, rem = g.tilesA - full * GA, per = GA * g.tilesB;
@@ -70,7 +72,7 @@ template <int DT, int FA, int FB>
 __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int total) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wb = w >> 1, wa = w & 1, fr = lane & 15, fq = lane >> 4;
-    const int nk = g.KB;
+    const int nk = g.slice_kb;                            // blocks of k of a tile (K, or a slice of it)
     auto decode = [&](int vb) { return decode_tile(g, vb); };
 
     // ---- DMA: piece i of wave w fills LDS rows (4 i + w) * 8 .. + 7; a lane supplies 16 bytes (chunk XOR-swizzled with bits 1..3 of the
@@ -81,10 +83,12 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     const int vB = ((((q8 & 3) << 2) | (q8 >> 2)) * 8 + (w >> 1)) * (int)g.ldb + ch * 16;
     __amdgpu_buffer_rsrc_t rA, rB, rS, rBias;
     auto aim = [&](const Tile& t) {
-        rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda, (long)min(g.M - t.a0, 256) * g.lda);
-        rB = rsrc(g.b + t.batch * g.bb + (long)t.b0 * g.ldb, (long)min(g.N - t.b0, 256) * g.ldb);
+        // (a slice of K starts slice_kb blocks into the rows: the range ends where the last row does)
+        const long k0 = (long)t.slice * g.slice_kb;
+        rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda + k0 * 128, (long)min(g.M - t.a0, 256) * g.lda - k0 * 128);
+        rB = rsrc(g.b + t.batch * g.bb + (long)t.b0 * g.ldb + k0 * 128, (long)min(g.N - t.b0, 256) * g.ldb - k0 * 128);
         // scale bytes (the dwords that hold a row's byte): even waves A's, odd waves B's — twice the same bytes instead of a branch
-        const uint8_t* sp = w & 1 ? g.bs + t.batch * g.bbs + t.b0 : g.as + t.batch * g.bas + t.a0;
+        const uint8_t* sp = w & 1 ? g.bs + t.batch * g.bbs + k0 * g.ldbs + t.b0 : g.as + t.batch * g.bas + k0 * g.ldas + t.a0;
         // (the range check counts the scalar offset, here the block's scale row, too: the range ends with this tile's rows in the last one)
         rS = rsrc(sp, (long)(nk - 1) * (w & 1 ? g.ldbs : g.ldas) + min(((w & 1 ? g.N - t.b0 : g.M - t.a0) + 3) & ~3, 256));
         if (g.bias) rBias = rsrc(g.bias + t.batch * g.bbias + t.b0, min(g.N - t.b0, 256) * 4L);
@@ -110,7 +114,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     for (int m = 0; m < 8; ++m)
 #pragma unroll
         for (int n = 0; n < 8; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int NST = 32;                               // stores of an interior tile per lane
+    constexpr int NST = DT == CLT_DT_F32 ? 63 : 32;       // stores of an interior tile per lane (63: the counter's limit, 64 are issued)
 
     // ---- the stream of k-blocks: staging runs two blocks ahead of the products, across tiles
     int vb = blockIdx.x, svb = vb, skt = 0, sslot = 0, slot = 0, buf = 0;
@@ -202,7 +206,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
         typedef typename Elem<DT>::type T;
         const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N, has_bias = g.bias != nullptr;
         const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + wb * 128 + fq * 8;
-        T* ctile = static_cast<T*>(g.c) + cur.batch * g.bc + (long)(cur.a0 + wa * 128) * g.ldc + cur.b0 + wb * 128;
+        T* ctile = static_cast<T*>(g.c) + cur.batch * g.bc + cur.slice * g.slice_stride + (long)(cur.a0 + wa * 128) * g.ldc + cur.b0 + wb * 128;
         unsigned char* slab = g8_smem + SLAB_BASE + w * SLAB;
         const int wr = fr * SLAB_ROW + fq * 16, rd = fq * SLAB_ROW + fr * 16;
         const unsigned at = (unsigned)(fq * 8 * (int)g.ldc + fr * 8) * (unsigned)sizeof(T);      // a lane's offset: 32 bits (host check)
@@ -216,6 +220,24 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
                 *reinterpret_cast<u32x4*>(slab + wr + i * 64) = u32x4{pack_out16<DT>(lo[0], lo[1]), pack_out16<DT>(lo[2], lo[3]), pack_out16<DT>(hi[0], hi[1]), pack_out16<DT>(hi[2], hi[3])};
             }
         };
+        if constexpr (DT == CLT_DT_F32) {                 // partial sums of a slice
+            const int prow = g.M - (cur.a0 + wa * 128 + fr * 8), pcol = g.N - (cur.b0 + wb * 128 + fq * 8);
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    T* p = ctile + (long)(fr * 8 + n) * g.ldc + fq * 8 + i * 32;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const f32x4 v = f32x4{acc[4 * j][n][i], acc[4 * j + 1][n][i], acc[4 * j + 2][n][i], acc[4 * j + 3][n][i]};
+                        if (interior) *reinterpret_cast<f32x4_u*>(p + 4 * j) = v;
+                        else if (n < prow)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) if (i * 32 + 4 * j + e < pcol) p[4 * j + e] = v[e];
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        } else {
         put(0);
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -233,6 +255,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
                     for (int j = 0; j < 8; ++j) if (j < cols) p[j] = (T)(u[j >> 1] >> (16 * (j & 1)));
             }
             __builtin_amdgcn_sched_barrier(0);
+        }
         }
         if (!more) break;
 #pragma unroll
@@ -252,7 +275,7 @@ template <int FA, int FB>
 __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, int total) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wb = w >> 2, wa = w & 3, fr = lane & 15, fq = lane >> 4;
-    const int nk = g.KB;
+    const int nk = g.slice_kb;                            // blocks of k of a tile (K, or a slice of it)
     // piece i of wave w fills LDS rows (8 i + w) * 8 .. + 7
     const int q8 = (w & 1) * 8 + (lane >> 3), ch = (lane & 7) ^ ((q8 >> 1) & 7);
     const int vA = (q8 * 4 + (w >> 1)) * (int)g.lda + ch * 16;
@@ -262,9 +285,10 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
     int vb = blockIdx.x, svb = vb, skt = 0, sslot = 0, slot = 0, buf = 0;
     auto enter = [&](const Tile& t) {
         if (svb < total) {
-            rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda, (long)min(g.M - t.a0, 256) * g.lda);
-            rB = rsrc(g.b + t.batch * g.bb + (long)t.b0 * g.ldb, (long)min(g.N - t.b0, 256) * g.ldb);
-            const uint8_t* sp = w & 1 ? g.bs + t.batch * g.bbs + t.b0 : g.as + t.batch * g.bas + t.a0;
+            const long k0 = (long)t.slice * g.slice_kb;
+            rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda + k0 * 128, (long)min(g.M - t.a0, 256) * g.lda - k0 * 128);
+            rB = rsrc(g.b + t.batch * g.bb + (long)t.b0 * g.ldb + k0 * 128, (long)min(g.N - t.b0, 256) * g.ldb - k0 * 128);
+            const uint8_t* sp = w & 1 ? g.bs + t.batch * g.bbs + k0 * g.ldbs + t.b0 : g.as + t.batch * g.bas + k0 * g.ldas + t.a0;
             rS = rsrc(sp, (long)(nk - 1) * srow + min(((w & 1 ? g.N - t.b0 : g.M - t.a0) + 3) & ~3, 256));
             if (g.bias && w == 2) {
                 __amdgpu_buffer_rsrc_t r = rsrc(g.bias + t.batch * g.bbias + t.b0, min(g.N - t.b0, 256) * 4L);
@@ -363,7 +387,7 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
         // ---- results: for (n, i) a lane has row 4 fr + n of its 64 and eight columns 8 (4 i + fq) .. of its 128
         const int r0 = wa * 64 + fr * 4, c0 = wb * 128 + fq * 8;
         const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N && !g.accumulate;
-        float* ctile = static_cast<float*>(g.c) + cur.batch * g.bc + (long)cur.a0 * g.ldc + cur.b0;
+        float* ctile = static_cast<float*>(g.c) + cur.batch * g.bc + cur.slice * g.slice_stride + (long)cur.a0 * g.ldc + cur.b0;
         const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + c0;
         const bool has_bias = g.bias != nullptr;
         const int rows = g.M - cur.a0 - r0, cols = g.N - cur.b0 - c0;
@@ -399,26 +423,40 @@ template <class F> int launch(F f, int threads, const Gemm8Args& g, int total, h
     CLT_LAUNCH_CHECK();
     return CLT_OK;
 }
-template <int FA, int FB> int launch_dtype(const Gemm8Args& g, int dtype, int total, hipStream_t st) {
-    if (dtype == CLT_DT_F32) return launch(gemm8_large_f32_kernel<FA, FB>, 512, g, total, st);
+// fast: 8-bit instructions (16-bit results, or the partial sums of their slices)
+template <int FA, int FB> int launch_dtype(const Gemm8Args& g, int dtype, bool fast, int total, hipStream_t st) {
+    if (dtype == CLT_DT_F32 && !fast) return launch(gemm8_large_f32_kernel<FA, FB>, 512, g, total, st);
+    if (dtype == CLT_DT_F32) return launch(gemm8_large_kernel<CLT_DT_F32, FA, FB>, 256, g, total, st);
     if (dtype == CLT_DT_BF16) return launch(gemm8_large_kernel<CLT_DT_BF16, FA, FB>, 256, g, total, st);
     return launch(gemm8_large_kernel<CLT_DT_F16, FA, FB>, 256, g, total, st);
 }
 }  // namespace
 
-// a chip's worth of tiles, mostly full ones
-bool clt_internal_gemm8_large_applies(int M, int N, int KB, int batch) {
+// Slices of K the large form runs a shape in (1: whole; 0: the shape is the small tiles').  Whole where the tiles fill half the chip;
+// fewer tiles (at least 64) and 128 and some are multiplied to about a chip's worth by cutting K, where every slice keeps 32 blocks
+// (50 us: the partial sums and their folding cost a tenth of it) and the cut is even.
+int clt_internal_gemm8_large_slices(int M, int N, int KB, int batch) {
     const long total = ((long)(M - 1) / 256 + 1) * ((N - 1) / 256 + 1) * batch;
-    return KB >= 1 && M >= 128 && N >= 128 && total >= 128 && total <= 0x3fffffffL;
+    if (KB < 1 || M < 128 || N < 128 || total < 64 || total > 0x3fffffffL) return 0;
+    for (int s = (int)(256 / total); s > 1; --s)
+        if (KB % s == 0 && KB / s >= 32) return s;
+    return total >= 128 ? 1 : 0;
 }
 
+// dtype: of the product asked for (it picks the instructions); g.part: partial sums go there, unfolded
 int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, hipStream_t st) {
     Gemm8Args g = g0;
+    const bool fast = dtype != CLT_DT_F32;
     g.tilesA = (g.M - 1) / 256 + 1; g.tilesB = (g.N - 1) / 256 + 1;
-    const int total = g.tilesA * g.tilesB * g.batch, rem = g.tilesA % GA;
+    if (g.part) {
+        g.c = g.part; g.ldc = g.N; g.bc = (long)g.M * g.N; g.slice_stride = g.batch * g.bc;
+        g.bias = nullptr; g.accumulate = 0;
+        dtype = CLT_DT_F32;
+    }
+    const int total = g.tilesA * g.tilesB * g.batch * g.slices, rem = g.tilesA % GA;
     g.inv_tiles = 0xffffffffu / (uint32_t)(g.tilesA * g.tilesB);
     g.inv_panel = 0xffffffffu / (uint32_t)(GA * g.tilesB);
     g.inv_rem = rem ? 0xffffffffu / (uint32_t)rem : 0u;
-    return fa == 0 ? (fb == 0 ? launch_dtype<0, 0>(g, dtype, total, st) : launch_dtype<0, 1>(g, dtype, total, st))
-                   : (fb == 0 ? launch_dtype<1, 0>(g, dtype, total, st) : launch_dtype<1, 1>(g, dtype, total, st));
+    return fa == 0 ? (fb == 0 ? launch_dtype<0, 0>(g, dtype, fast, total, st) : launch_dtype<0, 1>(g, dtype, fast, total, st))
+                   : (fb == 0 ? launch_dtype<1, 0>(g, dtype, fast, total, st) : launch_dtype<1, 1>(g, dtype, fast, total, st));
 }

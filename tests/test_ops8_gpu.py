@@ -178,7 +178,8 @@ def test_product(shape, out):
 
 
 #: enough 256 x 256 tiles to fill the chip: whole and partial ones, 1, 2, 3 and many blocks of k, odd rows of results
-LARGE = [(1, 3000, 100, 2901), (12, 700, 256, 1100), (12, 701, 300, 1101), (3, 2048, 1024, 2048), (33, 300, 640, 515), (1, 128, 384, 40000)]
+LARGE = [(1, 3000, 100, 2901), (12, 700, 256, 1100), (12, 701, 300, 1101), (3, 2048, 1024, 2048), (33, 300, 640, 515), (1, 128, 384, 40000),
+         (1, 2100, 8192, 1801), (2, 1100, 12200, 1700)]            # (and K in two and three slices)
 
 
 @gpu
