@@ -3,7 +3,7 @@
 Host side mirrors the reference's module / YAML contract; all arithmetic runs in
 hand-written HIP kernels (csrc/) reached through the C ABI in include/clt_hip.h.
 """
-from .precision import get_precision, precision, set_precision  # noqa: F401
+from .precision import contractions8, get_precision, precision, set_contractions8, set_precision  # noqa: F401
 
 REF_PREFIX = "crosslayer_transcoder."
 OUR_PREFIX = "crosslayer_transcoder_amd."

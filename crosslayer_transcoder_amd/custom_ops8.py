@@ -213,5 +213,136 @@ def plt_decoder8(feat: Tensor, W: Tensor, b: Optional[Tensor]) -> Tensor:
     return _linear(feat, W, b, True)
 
 
+# ---- cross-layer decoder: recons[:, l] = feat[:, :l+1].flatten(1) @ W_l.flatten(0, 1) + b[l] (reference model/clt.py:334-343) ----------
+# Blocks run along the flattened (source layer, feature) axis.  The features are packed once and every target layer contracts over its
+# first (l + 1) F columns; where F is no multiple of 128 a block would straddle that border, and every prefix is packed by itself.
+def _clt_forward(feat, b, Ws, keep_x, keep_w):
+    """-> recons [B, L, d], kept: [x transposed (codes, scale bytes)] + [W_l for the input gradient (codes, scale bytes)] ..."""
+    feat = ops8._dense(feat, (3,)).contiguous()
+    B, L, F = feat.shape
+    d = Ws[0].shape[2]
+    if not (L and F and d):
+        raise ValueError(f"empty map: features {tuple(feat.shape)}, W_0 {tuple(Ws[0].shape)}")
+    flat = feat.view(B, L * F)
+    out = torch.empty((B, L, d), dtype=feat.dtype, device=feat.device)
+    whole = F % ops8.BLOCK == 0
+    q, s, xt, xs, _ = ops8.pack8_raw(flat.unsqueeze(0), _E4M3, whole, keep_x) if whole or keep_x else (None,) * 5
+    kept = [xt, xs] if keep_x else []
+    x = ops8.Block8(q, s, B, L * F) if whole else None
+    for l, W in enumerate(Ws):
+        K = (l + 1) * F
+        dq, ds, tq, ts, _ = ops8.pack8_raw(ops8._dense(W, (3,)).reshape(1, K, d), _E4M3, keep_w, True, tiles=True)
+        if keep_w:
+            kept += [dq, ds]
+        ops8.gemm8(x.first_columns(K) if whole else ops8.quantize8(flat[:, :K]), ops8.Block8(tq, ts, d, K), None if b is None else b[l:l + 1],
+                   out=out[:, l].unsqueeze(0))
+    return out, kept
+
+
+def _clt_gradients(g, kept, F, has_x, need_dx, w_dtypes, need_db):
+    """-> dfeat fp32 [B, L, F], [dW_l [l + 1, F, d]], db fp32 [L, d]; None where not asked for (w_dtypes empty: no dW)."""
+    g = ops8._dense(g, (3,))
+    B, L, d = g.shape
+    q, s, qt, qs, db = ops8.pack8_raw(g.transpose(0, 1), _E4M3, need_dx or not w_dtypes, bool(w_dtypes), sums=need_db)
+    dx, dWs = None, None
+    if need_dx:
+        dx = torch.empty((B, L * F), dtype=torch.float32, device=g.device)
+        ws = kept[2:] if has_x else kept
+        for l in range(L - 1, -1, -1):                     # (the last layer reaches every column and writes; the others add)
+            K = (l + 1) * F
+            ops8.gemm8(ops8.Block8(q[l:l + 1], s[l:l + 1], B, d), ops8.Block8(ws[2 * l], ws[2 * l + 1], K, d), out=dx[:, :K].unsqueeze(0), accumulate=l != L - 1)
+        dx = dx.view(B, L, F)
+    if w_dtypes:
+        x = ops8.Block8(kept[0], kept[1], L * F, B)
+        dWs = [ops8.gemm8(x.first_rows((l + 1) * F), ops8.Block8(qt[l:l + 1], qs[l:l + 1], d, B), out_dtype=dt).view(l + 1, F, d)
+               for l, dt in enumerate(w_dtypes)]
+    return dx, dWs, db
+
+
+@torch.library.custom_op("clt_hip::clt_decoder8", mutates_args=(), device_types=_DEV)
+def _clt_decoder8_op(feat: Tensor, b: Optional[Tensor], Ws: List[Tensor], keep_x: bool, keep_w: bool) -> List[Tensor]:
+    """-> [recons [B, L, d], the tensors kept for the backward pass]."""
+    out, kept = _clt_forward(feat, b, Ws, keep_x, keep_w)
+    return [out] + kept
+
+
+@_clt_decoder8_op.register_fake
+def _(feat, b, Ws, keep_x, keep_w):
+    B, L, F = feat.shape
+    d = Ws[0].shape[2]
+    form = lambda rows, cols: [feat.new_empty((1, rows, _up(cols)), dtype=torch.uint8), feat.new_empty((1, _up(cols) // 128, _up(rows)), dtype=torch.uint8)]  # noqa: E731
+    kept = form(L * F, B) if keep_x else []
+    for l in range(L if keep_w else 0):
+        kept += form((l + 1) * F, d)
+    return [feat.new_empty(B, L, d)] + kept
+
+
+@torch.library.custom_op("clt_hip::clt_decoder8_bwd", mutates_args=(), device_types=_DEV)
+def _clt_decoder8_bwd(g: Tensor, kept: List[Tensor], F: int, has_x: bool, need_dx: bool, w_dtype: Optional[torch.dtype], need_db: bool) -> List[Tensor]:
+    """-> [dfeat fp32, db fp32 (empty where not asked for), dW_0, ..., dW_{L-1} (w_dtype None: none)]."""
+    dx, dWs, db = _clt_gradients(g, kept, F, has_x, need_dx, [w_dtype] * g.shape[1] if w_dtype is not None else [], need_db)
+    return [g.new_empty(0) if t is None else t for t in (dx, db)] + (dWs or [])
+
+
+@_clt_decoder8_bwd.register_fake
+def _(g, kept, F, has_x, need_dx, w_dtype, need_db):
+    B, L, d = g.shape
+    f32 = torch.float32
+    out = [g.new_empty((B, L, F), dtype=f32) if need_dx else g.new_empty(0), g.new_empty((L, d), dtype=f32) if need_db else g.new_empty(0)]
+    return out + [g.new_empty((l + 1, F, d), dtype=w_dtype) for l in range(L if w_dtype is not None else 0)]
+
+
+def _clt_setup(ctx, inputs, output):
+    feat, b, Ws, ctx.keep_x, ctx.keep_w = inputs
+    ctx.F, ctx.x_dtype, ctx.w_dtype, ctx.b = feat.shape[2], feat.dtype, Ws[0].dtype, None if b is None else (b.dtype, b.shape)
+    ctx.save_for_backward(*output[1:])
+
+
+def _clt_backward(ctx, grads):
+    need_x, need_b, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1], any(ctx.needs_input_grad[2])
+    if (need_w and not ctx.keep_x) or (need_x and not ctx.keep_w):
+        raise RuntimeError("clt_decoder8 was called without keeping what this gradient needs (keep_x for dW, keep_w for the features')")
+    dx, db, *dWs = torch.ops.clt_hip.clt_decoder8_bwd(grads[0], list(ctx.saved_tensors), ctx.F, ctx.keep_x, need_x, ctx.w_dtype if need_w else None, need_b)
+    return dx.to(ctx.x_dtype) if need_x else None, db.to(ctx.b[0]).reshape(ctx.b[1]) if need_b else None, list(dWs) if need_w else None, None, None
+
+
+_clt_decoder8_op.register_autograd(_clt_backward, setup_context=_clt_setup)
+
+
+class _CltDecoder8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, feat, b, *Ws):
+        need_w = any(ctx.needs_input_grad[2:])
+        out, kept = _clt_forward(feat, b, Ws, need_w, ctx.needs_input_grad[0])
+        ctx.save_for_backward(*kept)
+        ctx.F, ctx.x_dtype, ctx.has_x, ctx.w_dtypes = feat.shape[2], feat.dtype, need_w, [w.dtype for w in Ws]
+        ctx.b = None if b is None else (b.dtype, b.shape)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        need = ctx.needs_input_grad
+        dx, dWs, db = _clt_gradients(g, ctx.saved_tensors, ctx.F, ctx.has_x, need[0], ctx.w_dtypes if any(need[2:]) else [], need[1])
+        dWs = [None] * len(ctx.w_dtypes) if dWs is None else [dW if n else None for dW, n in zip(dWs, need[2:])]
+        return (dx.to(ctx.x_dtype) if need[0] else None, db.to(ctx.b[0]).reshape(ctx.b[1]) if need[1] else None, *dWs)
+
+
+def clt_decoder8(feat: Tensor, b: Optional[Tensor], Ws: List[Tensor]) -> Tensor:
+    """recons [B, L, d] from feat [B, L, F] and Ws[l] [l + 1, F, d], b [L, d] (`clt_hip::clt_decoder`'s arguments)."""
+    if feat.dim() != 3 or len(Ws) != feat.shape[1] or any(W.dim() != 3 or tuple(W.shape) != (l + 1, feat.shape[2], Ws[0].shape[2]) for l, W in enumerate(Ws)):
+        raise ValueError(f"features {tuple(feat.shape)} do not match the decoder weights {[tuple(W.shape) for W in Ws]}")
+    if any(W.device != feat.device or W.dtype != Ws[0].dtype for W in Ws):
+        raise ValueError("the decoder weights are of one type, on the features' device")
+    if b is not None and tuple(b.shape) != (len(Ws), Ws[0].shape[2]):
+        raise ValueError(f"bias {tuple(b.shape)} does not match {len(Ws)} layers of {Ws[0].shape[2]}")
+    if torch.compiler.is_compiling():
+        grad = torch.is_grad_enabled()
+        return torch.ops.clt_hip.clt_decoder8(feat, b, list(Ws), grad and any(W.requires_grad for W in Ws), grad and feat.requires_grad)[0]
+    if not torch.is_grad_enabled():
+        return _clt_forward(feat, b, Ws, False, False)[0]
+    return _CltDecoder8.apply(feat, b, *Ws)
+
+
 #: names of the registered ops, for tests and introspection
-REGISTERED8 = ("linear8", "linear8_bwd")
+REGISTERED8 = ("linear8", "linear8_bwd", "clt_decoder8", "clt_decoder8_bwd")

@@ -11,7 +11,8 @@ import yaml
 from safetensors.torch import save_file
 
 from .. import custom_ops  # noqa: F401  (registers torch.ops.clt_hip.*)
-from ..precision import get_precision
+from .. import custom_ops8, ops8
+from ..precision import contractions8_enabled, get_precision
 from .serializable_module import SerializableModule
 from .standardize import Standardizer
 
@@ -54,10 +55,18 @@ class Encoder(SerializableModule):
             self.b.zero_()
 
     @torch.no_grad()
-    def forward_layer(self, acts_norm, layer: int):
-        """Inference: [batch, seq, d_acts] of ONE layer -> [batch, seq, d_features] (clt.py:134-145)."""
+    def pack8(self) -> "ops8.Block8":
+        """The weights in 8-bit block-scaled form, for forward_layer(packed=...): made once, kept by the caller."""
+        return ops8.quantize8_weights(self.Wt)
+
+    @torch.no_grad()
+    def forward_layer(self, acts_norm, layer: int, packed: Optional["ops8.Block8"] = None):
+        """Inference: [batch, seq, d_acts] of ONE layer -> [batch, seq, d_features] (clt.py:134-145).  packed: pack8()'s weights, one
+        pass over which gives the features (a byte a weight instead of a cast copy); the result has the activations' type."""
         from .. import ops
         shp = acts_norm.shape
+        if packed is not None:
+            return ops8.linear8(acts_norm.reshape(-1, shp[-1]), packed.of_batch(layer), self.b[layer]).reshape(*shp[:-1], self.d_features)
         x = _operand(acts_norm.reshape(-1, 1, shp[-1]))
         W = _operand(self.Wt[layer:layer + 1])
         return ops.encoder_fwd(x, W, self.b[layer:layer + 1].contiguous()).reshape(*shp[:-1], self.d_features)
@@ -75,6 +84,8 @@ class Encoder(SerializableModule):
     def forward(self, acts_norm, layer="all"):
         if layer != "all":
             return self.forward_layer(acts_norm, layer)
+        if contractions8_enabled():
+            return custom_ops8.encoder8(acts_norm, self.W, self.b)
         return torch.ops.clt_hip.encoder(acts_norm, self.W, self.b)          # custom_ops.py: dispatcher op + autograd rule
 
     @torch.no_grad()
@@ -128,11 +139,18 @@ class Decoder(_DecoderBase):
         return [self.W]
 
     @torch.no_grad()
-    def forward_layer(self, features, layer: int):
+    def pack8(self) -> "ops8.Block8":
+        """The weights in 8-bit block-scaled form, for forward_layer(packed=...): made once, kept by the caller."""
+        return ops8.quantize8_weights(self.W, transposed=True)
+
+    @torch.no_grad()
+    def forward_layer(self, features, layer: int, packed: Optional["ops8.Block8"] = None):
         from .. import ops
         if features.ndim == 4:
             features = features[:, :, layer, :]
         shp = features.shape
+        if packed is not None:
+            return ops8.linear8(features.reshape(-1, shp[-1]), packed.of_batch(layer), self.b[layer]).reshape(*shp[:-1], self.d_acts)
         f = _operand(features.reshape(-1, 1, shp[-1]))
         r = ops.plt_decoder_fwd(f, _operand(self.W[layer:layer + 1]), self.b[layer:layer + 1].contiguous())
         return r.reshape(*shp[:-1], self.d_acts)
@@ -140,6 +158,8 @@ class Decoder(_DecoderBase):
     def forward(self, features, layer="all"):
         if layer != "all":
             return self.forward_layer(features, layer)
+        if contractions8_enabled():
+            return custom_ops8.plt_decoder8(features, self.W, self.b)
         return torch.ops.clt_hip.plt_decoder(features, self.W, self.b)
 
     @torch.no_grad()
@@ -174,11 +194,18 @@ class CrosslayerDecoder(_DecoderBase):
             self.b.zero_()
 
     @torch.no_grad()
-    def forward_layer(self, features, layer: int):
+    def pack8(self) -> list:
+        """Every target layer's weights in 8-bit block-scaled form, for forward_layer(packed=...): made once, kept by the caller."""
+        return [ops8.quantize8_weights(w.reshape(-1, self.d_acts), transposed=True) for w in self.weights()]
+
+    @torch.no_grad()
+    def forward_layer(self, features, layer: int, packed: Optional[list] = None):
         """Inference: features [batch, seq, from_layer (= layer+1), F] -> [batch, seq, d] (clt.py:304-317)."""
         from .. import ops
         shp = features.shape
         K = (layer + 1) * self.d_features
+        if packed is not None:
+            return ops8.linear8(features.reshape(-1, K), packed[layer], self.b[layer]).reshape(*shp[:-2], self.d_acts)
         f = _operand(features.reshape(-1, 1, K))
         W = _operand(getattr(self, f"W_{layer}").reshape(1, K, self.d_acts))
         r = ops.plt_decoder_fwd(f, W, self.b[layer:layer + 1].contiguous())
@@ -187,6 +214,8 @@ class CrosslayerDecoder(_DecoderBase):
     def forward(self, features, layer="all"):
         if layer != "all":
             return self.forward_layer(features, layer)
+        if contractions8_enabled():
+            return custom_ops8.clt_decoder8(features, self.b, self.weights())
         return torch.ops.clt_hip.clt_decoder(features, self.b, self.weights())
 
     @torch.no_grad()

@@ -172,6 +172,13 @@ def quantize8_tiles(x: torch.Tensor, fmt: str = "e4m3") -> Tuple[Block8, Block8]
     return Block8(q, s, x.shape[1], x.shape[2], fmt), Block8(qt, st, x.shape[2], x.shape[1], fmt)
 
 
+def quantize8_weights(x: torch.Tensor, transposed: bool = False, fmt: str = "e4m3") -> Block8:
+    """One form of quantize8_tiles: a weight matrix [N, K] as linear8 and gemm8 contract it, or (transposed) a [K, N] one."""
+    x = _as3(x)
+    q, s, qt, st, _ = pack8_raw(x, _fmt(fmt), not transposed, transposed, tiles=True)
+    return Block8(qt, st, x.shape[2], x.shape[1], fmt) if transposed else Block8(q, s, x.shape[1], x.shape[2], fmt)
+
+
 def dequantize8(q: Block8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values held, [L, rows, cols], each rounded once to `dtype` (exact in fp32, and in bf16 for normal numbers)."""
     if dtype not in _DT:

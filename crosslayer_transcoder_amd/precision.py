@@ -49,6 +49,33 @@ def precision(p: str):
         set_precision(old)
 
 
+# ---- 8-bit contractions of the module forward --------------------------------------------------------------------------
+_CONTRACTIONS8 = False
+
+
+def set_contractions8(on: bool):
+    """Whether Encoder / Decoder / CrosslayerDecoder.forward contract in 8-bit block-scaled form (custom_ops8.py) and keep their input
+    in 8 bits for the backward pass, instead of in the compute precision.  Off by default: the values differ from the
+    reference's by the rounding to 4 significant bits.  Results have the input's type.  The fused training step does not run
+    the module forward and is unaffected."""
+    global _CONTRACTIONS8
+    _CONTRACTIONS8 = bool(on)
+
+
+def contractions8_enabled() -> bool:
+    return _CONTRACTIONS8
+
+
+@contextlib.contextmanager
+def contractions8(on: bool = True):
+    old = _CONTRACTIONS8
+    set_contractions8(on)
+    try:
+        yield
+    finally:
+        set_contractions8(old)
+
+
 class LossScaler:
     """Dynamic loss scaling of the fp16 mode with torch.amp.GradScaler's rule and defaults (init 2**16, x2 after 2000 clean
     steps, x0.5 after an overflow; Lightning's "16-mixed" plugin creates exactly that scaler).  The overflow flag lives on

@@ -358,7 +358,7 @@ def reference_training(x, W, b, dy, kn):
 
 
 def close(got, ref, tol):
-    err = float((got.cpu().double() - ref).norm())
+    err = float((got.detach().cpu().double() - ref).norm())
     assert err <= tol * float(ref.norm()) + 1e-30, (err, float(ref.norm()))
 
 
@@ -441,6 +441,11 @@ def test_opcheck():
     cases = {"linear8": (x, W, b, True, True, True)}
     kept = torch.ops.clt_hip.linear8(x.detach(), W.detach(), b.detach(), True, True, True)[1]
     cases["linear8_bwd"] = (rnd(9, 2, 30, seed=4, spread=False), kept, 40, True, True, True, torch.float32, True)
+    Ws = [(rnd(l + 1, 40, 30, seed=5 + l, spread=False) * 0.2).requires_grad_() for l in range(2)]
+    feat = torch.relu(x.detach()).requires_grad_()
+    cases["clt_decoder8"] = (feat, b, Ws, True, True)
+    kept = torch.ops.clt_hip.clt_decoder8(feat.detach(), b.detach(), [w.detach() for w in Ws], True, True)[1:]
+    cases["clt_decoder8_bwd"] = (rnd(9, 2, 30, seed=4, spread=False), kept, 40, True, True, torch.float32, True)
     assert set(cases) == set(C.REGISTERED8)
     for name, args in cases.items():
         torch.library.opcheck(getattr(torch.ops.clt_hip, name).default, args)
@@ -491,6 +496,107 @@ def test_two_streams_at_once():
                 got[i].append(ops8.linear8(xs[i], ws[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(y, ref[i]) for i in range(2) for y in got[i])
+
+
+def reference_clt(feat, Ws, b, g):
+    """[recons, dfeat, db, dW_l ...] of the cross-layer decoder in float64 from the values held."""
+    B, L, F = feat.shape
+    d = Ws[0].shape[2]
+    flat = feat.detach().reshape(1, B, L * F)
+    xt = held64(flat.mT)[0][0]                                                    # [L F, B]
+    dfeat, recons, dWs = torch.zeros(B, L * F, dtype=torch.float64), [], []
+    for l, W in enumerate(Ws):
+        K = (l + 1) * F
+        w = held64(W.detach().reshape(1, K, d), tiles=True)[0][0]
+        recons.append(held64(flat[:, :, :K])[0][0] @ w + (b[l].detach().cpu().double() if b is not None else 0.0))
+        dfeat[:, :K] += held64(g[:, l].unsqueeze(0))[0][0] @ w.mT
+        dWs.append((xt[:K] @ held64(g[:, l].unsqueeze(0).mT)[0][0].mT).reshape(l + 1, F, d))
+    return [torch.stack(recons, 1), dfeat.view(B, L, F), g.cpu().double().sum(0)] + dWs
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(5, 3, 40, 30), (130, 2, 256, 70), (64, 4, 128, 110), (33, 1, 300, 64)])
+def test_cross_layer_decoder(shape, dtype):
+    """Dictionaries that are a multiple of 128 (one packing for all target layers) and not; the features' gradient is a sum of L
+    products in fp32, rounded once."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    B, L, F, d = shape
+    feat = torch.relu(rnd(B, L, F, seed=1, dtype=dtype, spread=False)).requires_grad_()
+    Ws = [(rnd(l + 1, F, d, seed=2 + l, spread=False) * 0.1).requires_grad_() for l in range(L)]
+    b, g = rnd(L, d, seed=9, spread=False).requires_grad_(), rnd(B, L, d, seed=10, dtype=dtype, spread=False)
+    y = C.clt_decoder8(feat, b, Ws)
+    assert y.dtype == dtype
+    grads = torch.autograd.grad(y, [feat, b] + Ws, g)
+    ref = reference_clt(feat, Ws, b, g)
+    t = 2.0 ** -18 if dtype == torch.float32 else torch.finfo(dtype).eps / 2 + 2.0 ** -12
+    close(y, ref[0], t), close(grads[0], ref[1], t), close(grads[1], ref[2], 2.0 ** -18)
+    for l in range(L):
+        assert grads[2 + l].shape == Ws[l].shape
+        close(grads[2 + l], ref[3 + l], 2.0 ** -18)
+    z = torch.ops.clt_hip.clt_decoder8(feat, b, Ws, True, True)[0]
+    assert torch.equal(y, z) and all(torch.equal(u, v) for u, v in zip(grads, torch.autograd.grad(z, [feat, b] + Ws, g)))
+
+
+@gpu
+@pytest.mark.parametrize("dec", ["clt", "plt"])
+def test_modules_contract_in_8_bits(dec):
+    """Encoder -> ReLU -> decoder as the modules run them under contractions8(): each stage against 64 bits on what it was given, the
+    chain's gradients against the same formulas, a byte an element of every input kept, and the native forward untouched."""
+    import crosslayer_transcoder_amd as cta
+    from crosslayer_transcoder_amd.model import CrosslayerDecoder, CrossLayerTranscoder, Decoder, Encoder, ReLU
+    L, d, F, B = 3, 96, 256, 64
+    torch.manual_seed(1)
+    m = CrossLayerTranscoder(ReLU(), Encoder(d, F, L), (CrosslayerDecoder if dec == "clt" else Decoder)(d, F, L)).cuda()
+    x = rnd(B, L, d, seed=3, spread=False)
+    native = m(x)[2].detach()
+    with cta.contractions8():
+        pre, feat, recons, _ = m(x)
+    assert torch.equal(m(x)[2], native)
+    g = rnd(B, L, d, seed=4, spread=False)
+    feat.retain_grad(), pre.retain_grad()
+    recons.backward(g)
+    ref = reference_training(x, m.encoder.W.permute(0, 2, 1), m.encoder.b, pre.grad, False)
+    close(pre.detach(), ref[0], 2.0 ** -18), close(m.encoder.W.grad.permute(0, 2, 1), ref[2], 2.0 ** -18), close(m.encoder.b.grad, ref[3], 2.0 ** -18)
+    Ws = m.decoder.weights()
+    if dec == "clt":
+        ref = reference_clt(feat, Ws, m.decoder.b, g)
+        grads = [m.decoder.b.grad] + [w.grad for w in Ws]
+        close(recons.detach(), ref[0], 2.0 ** -18), close(feat.grad, ref[1], 2.0 ** -18)
+        for got, want in zip(grads, ref[2:]):
+            close(got, want, 2.0 ** -18)
+    else:
+        ref = reference_training(feat, m.decoder.W, m.decoder.b, g, True)
+        for got, want in zip((recons.detach(), feat.grad, m.decoder.W.grad, m.decoder.b.grad), ref):
+            close(got, want, 2.0 ** -18)
+    assert same(pre.grad, torch.where(pre > 0, feat.grad, torch.zeros_like(feat.grad)))
+    assert not torch.equal(recons, native)                                           # (the 8-bit path is what ran)
+
+
+@gpu
+def test_layers_with_packed_weights():
+    """forward_layer(packed=pack8()): one token and a batch, every layer, encoder and both decoders."""
+    from crosslayer_transcoder_amd import ops8
+    from crosslayer_transcoder_amd.model import CrosslayerDecoder, Decoder, Encoder
+    L, d, F = 3, 96, 200
+    torch.manual_seed(2)
+    enc, clt, plt = Encoder(d, F, L).cuda(), CrosslayerDecoder(d, F, L).cuda(), Decoder(d, F, L).cuda()
+    for mod in (enc, clt, plt):
+        torch.nn.init.normal_(mod.b)
+    pe, pc, pp = enc.pack8(), clt.pack8(), plt.pack8()
+    assert pe.nbytes() <= enc.W.numel() * 1.4                                       # (rows of 96 are held as 128)
+    for shape in ((1, 1), (2, 3), (5, 40)):
+        for l in range(L):
+            x = rnd(*shape, d, seed=l, dtype=torch.bfloat16, spread=False)
+            y = enc.forward_layer(x, l, packed=pe)
+            assert y.shape == (*shape, F) and y.dtype == torch.bfloat16
+            check_product(y.reshape(1, -1, F), ops8.quantize8(x.reshape(1, -1, d)), pe.of_batch(l), enc.b[l:l + 1])
+            f = torch.relu(rnd(*shape, l + 1, F, seed=l, spread=False))
+            z = clt.forward_layer(f, l, packed=pc)
+            check_product(z.reshape(1, -1, d), ops8.quantize8(f.reshape(1, -1, (l + 1) * F)), pc[l], clt.b[l:l + 1])
+            f = torch.relu(rnd(*shape, L, F, seed=l, spread=False))
+            z = plt.forward_layer(f, l, packed=pp)
+            check_product(z.reshape(1, -1, d), ops8.quantize8(f[:, :, l].reshape(1, -1, F)), pp.of_batch(l), plt.b[l:l + 1])
 
 
 # ---- refusals (host checks: they run on the CPU) -----------------------------------------------------------------------------
@@ -569,6 +675,15 @@ def test_refusals_of_the_training_ops():
         C.encoder8(torch.zeros(4, 2, 8), torch.zeros(3, 8, 3), None)
     with pytest.raises(ValueError):
         C.encoder8(torch.zeros(4, 8), torch.zeros(2, 8, 3), None)
+    w = [torch.zeros(l + 1, 8, 3) for l in range(2)]
+    for args in ((torch.zeros(4, 3, 8), None, w), (torch.zeros(4, 2, 9), None, w), (torch.zeros(4, 2, 8), torch.zeros(2, 4), w),
+                 (torch.zeros(4, 2, 8), None, [w[0], w[1].double()]), (torch.zeros(4, 2, 8), None, w[::-1])):
+        with pytest.raises(ValueError):
+            C.clt_decoder8(*args)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        C.clt_decoder8(torch.zeros(4, 2, 8), None, w)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        C.plt_decoder8(torch.zeros(4, 2, 8), torch.zeros(2, 8, 3), None)
 
 
 @gpu
