@@ -116,8 +116,7 @@ __device__ __forceinline__ int fast_div(int n, int d, uint32_t inv) {
     return q;
 }
 
-// 256 x 256 tiles (gemm8_large.hip): the shapes that take them (0: none; else slices of K), and the launch
-int clt_internal_gemm8_large_slices(int M, int N, int KB, int batch);
+// 256 x 256 tiles (gemm8_large.hip)
 int clt_internal_gemm8_large(const Gemm8Args& g, int fa, int fb, int dtype, hipStream_t st);
 
 // Four consecutive columns of a row of C: one store where the row's alignment allows it (vec), else element by element

@@ -27,7 +27,8 @@ typedef __attribute__((address_space(3))) void lds_void;
 // LDS rows of 128 bytes, 16-byte chunks XOR-swizzled with bits 1..3 of the row.  Row p of a 64-row half is matrix row
 // (p % 16) * 4 + p / 16 (A) or c(p % 16) * 4 + p / 16 (B, c(4 q + i) = 4 i + q): a lane's four fragments are four consecutive rows,
 // so their scales are one dword, and its accumulators of the four B fragments are four consecutive columns.
-// Per block of k: 64 instruction slots of 8 cycles against 96 KB through LDS (768 cycles).  Measured: see DEPTH below.
+// Bound: a block of k is 64 instructions of 32 cycles (four waves: 512 cycles of each SIMD; fp32 results 1024) against 96 KB through
+// LDS (768 cycles); with every CU busy it takes 0.6 us (fp32 results: 1.0).  1024 x 4096 x 4096: 27.5 us = 1250 TFLOP/s.
 constexpr int OPB = 128 * 128, STG = 2 * OPB + 512, DEPTH = 4;
 constexpr int PIECES = 9;                            // DMA instructions of a wave per block of k
 extern __shared__ __attribute__((aligned(1024))) unsigned char t8_smem[];
@@ -194,18 +195,33 @@ template <int DT> __global__ __launch_bounds__(256) void gemm8_fold_kernel(Gemm8
     b8_store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, s, valid, vec, g.accumulate);
 }
 
-// Slices of K: enough blocks for two thirds of the chip, no slice shorter than 8 blocks of k (the second launch and its traffic
-// cost about as much), partial sums of at most 256 MB.
-int slices_of(int M, int N, int KB, int batch) {
-    const long tiles = ((long)(M - 1) / 128 + 1) * ((N - 1) / 128 + 1) * batch;
-    if (tiles >= 160 || KB < 16) return 1;
-    long s = 256 / tiles;
-    if (s > KB / 8) s = KB / 8;
-    const long bytes = (long)batch * M * N * 4;
-    while (s > 1 && s * bytes > (256L << 20)) --s;
-    if (s < 2) return 1;
-    const int per = (int)((KB + s - 1) / s);
-    return (KB + per - 1) / per;
+// Which tiles, and into how many slices K is cut: the least of the times that these measurements add up to (us; a pass is one tile on
+// every CU):
+//                            16-bit results         fp32 results
+//   128 x 128 tiles          7 + 0.6 a block of k   7 + 1.0         a pass
+//   256 x 256 tiles          8 + 1.3                15 + 2.7
+//   slices: the second launch 4, the partial sums 8 bytes an element and slice at 5 TB/s
+// e.g. (M, K, N; small against large tiles, us) 2048 x 1024 x 4096: 23.0 / 17.6 (bf16), 29.4 / 35.2 (fp32); 12 x (768 x 4096 x 768): 64 / 49
+// and 78 / 101; whole against sliced: 128 x 32768 x 768: 132 / 21; 1024 x 4096 x 768: 23 / 18; 1024 x 2048 x 2048: 16.3 / 20.1.
+// A slice keeps 4 blocks (the ring), slices of the large form are equal, partial sums take at most 256 MB.  The large form is not
+// for less than 128 rows on either side: such a tile is more than half empty (12 x (64 x 768 x 32768): 125 / 131).
+struct Plan { bool large; int slices; };
+Plan plan_of(int M, int N, int KB, int batch, bool wide) {
+    const double elements = (double)batch * M * N;
+    Plan best = {false, 1};
+    double least = 1e30;
+    for (int large = 0; large < 2; ++large) {
+        const long side = large ? 256 : 128, tiles = ((M - 1) / side + 1) * ((N - 1) / side + 1) * batch;
+        if (large && (M < 128 || N < 128 || KB < 1 || tiles > 0x3fffffffL)) break;
+        const double block = large ? (wide ? 2.7 : 1.3) : wide ? 1.0 : 0.6, pass = large ? (wide ? 15.0 : 8.0) : 7.0;
+        for (long s = 1; s == 1 || (s * tiles <= 256 && s * 4 <= KB && s * elements * 4.0 <= 268435456.0); ++s) {
+            if (large && s > 1 && (KB % s || 1024L * N > 0x7fffffffL)) continue;       // (offsets of the partial sums: 32 bits)
+            const long per = (KB + s - 1) / s, used = per ? (KB + per - 1) / per : 1;
+            const double t = (double)((tiles * used + 255) / 256) * (per * block + pass) + (used > 1 ? 4.0 + used * elements * 8.0 / 5e6 : 0.0);
+            if (t < least) { least = t; best = {large != 0, (int)used}; }
+        }
+    }
+    return best;
 }
 
 template <int DT, int FA, int FB> int launch_fmt(const Gemm8Args& g, long blocks, hipStream_t st) {
@@ -232,9 +248,9 @@ template <int DT> int launch(const Gemm8Args& g, int fa, int fb, long blocks, hi
 
 extern "C" size_t clt_gemm8_workspace_bytes(int M, int N, int K, int batch) {
     if (M <= 0 || N <= 0 || K <= 0 || batch <= 0) return 0;
-    const int KB = (int)(up128(K) / 128), large = clt_internal_gemm8_large_slices(M, N, KB, batch);
-    const int s = large ? large : slices_of(M, N, KB, batch);
-    return s > 1 ? (size_t)s * batch * M * N * 4 : 0;
+    const int KB = (int)(up128(K) / 128);
+    const int s = plan_of(M, N, KB, batch, false).slices, w = plan_of(M, N, KB, batch, true).slices, most = s > w ? s : w;
+    return most > 1 ? (size_t)most * batch * M * N * 4 : 0;
 }
 
 extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long ldas, long a_batch, long as_batch,
@@ -254,17 +270,16 @@ extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long 
                    static_cast<const uint8_t*>(b_scale), c, bias, lda, ldas, ldb, ldbs, ldc, a_batch, as_batch, b_batch, bs_batch,
                    c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 0u, 0u, 0u, 1, KB, nullptr, 0};
     const hipStream_t st = as_stream(stream);
-    int large = clt_internal_gemm8_large_slices(M, N, KB, batch);
-    // (results whose rows lie further apart than the large form's offsets reach: small tiles, unsliced)
-    const bool far = large == 1 && 256 * ldc * 4 > 0x7fffffffL;
-    g.slices = far ? 1 : large ? large : slices_of(M, N, KB, batch);
-    if (far || (large > 1 && 1024L * N > 0x7fffffffL)) large = 0;
+    Plan plan = plan_of(M, N, KB, batch, c_dtype == CLT_DT_F32);
+    // (results whose rows lie further apart than the large form's 32-bit offsets reach)
+    if (plan.large && plan.slices == 1 && 256 * ldc * 4 > 0x7fffffffL) plan.large = false;
+    g.slices = plan.slices;
     if (g.slices > 1) {
-        if (!workspace || !aligned16(workspace) || workspace_bytes < clt_gemm8_workspace_bytes(M, N, K, batch)) return CLT_ERR_WORKSPACE;
+        if (!workspace || !aligned16(workspace) || workspace_bytes < (size_t)g.slices * batch * M * N * 4) return CLT_ERR_WORKSPACE;
         g.part = static_cast<float*>(workspace);
         g.slice_kb = (KB + g.slices - 1) / g.slices;
     }
-    if (large) {
+    if (plan.large) {
         const int rc = clt_internal_gemm8_large(g, a_format, b_format, c_dtype, st);
         if (rc != CLT_OK || !g.part) return rc;
         return c_dtype == CLT_DT_F32 ? fold<CLT_DT_F32>(g, st) : c_dtype == CLT_DT_BF16 ? fold<CLT_DT_BF16>(g, st) : fold<CLT_DT_F16>(g, st);

@@ -386,7 +386,7 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
         nt = decode_tile(g, svb + (int)gridDim.x);
         // ---- results: for (n, i) a lane has row 4 fr + n of its 64 and eight columns 8 (4 i + fq) .. of its 128
         const int r0 = wa * 64 + fr * 4, c0 = wb * 128 + fq * 8;
-        const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N && !g.accumulate;
+        const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N;
         float* ctile = static_cast<float*>(g.c) + cur.batch * g.bc + cur.slice * g.slice_stride + (long)cur.a0 * g.ldc + cur.b0;
         const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + c0;
         const bool has_bias = g.bias != nullptr;
@@ -400,7 +400,11 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
                 f32x4 hi = f32x4{acc[4][n][i], acc[5][n][i], acc[6][n][i], acc[7][n][i]};
                 if (has_bias) { lo += *reinterpret_cast<const f32x4*>(bl + i * 32); hi += *reinterpret_cast<const f32x4*>(bl + i * 32 + 4); }
                 float* p = reinterpret_cast<float*>(reinterpret_cast<char*>(ctile + (long)n * g.ldc + i * 32) + at);
-                if (interior) { *reinterpret_cast<f32x4_u*>(p) = lo; *reinterpret_cast<f32x4_u*>(p + 4) = hi; }
+                if (interior) {
+                    if (g.accumulate) { lo += *reinterpret_cast<const f32x4_u*>(p); hi += *reinterpret_cast<const f32x4_u*>(p + 4); }
+                    *reinterpret_cast<f32x4_u*>(p) = lo;
+                    *reinterpret_cast<f32x4_u*>(p + 4) = hi;
+                }
                 else if (n < rows)
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
@@ -412,7 +416,7 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
         for (int m = 0; m < 8; ++m)
 #pragma unroll
             for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (!interior) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (!interior || g.accumulate) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
@@ -431,17 +435,6 @@ template <int FA, int FB> int launch_dtype(const Gemm8Args& g, int dtype, bool f
     return launch(gemm8_large_kernel<CLT_DT_F16, FA, FB>, 256, g, total, st);
 }
 }  // namespace
-
-// Slices of K the large form runs a shape in (1: whole; 0: the shape is the small tiles').  Whole where the tiles fill half the chip;
-// fewer tiles (at least 64) and 128 and some are multiplied to about a chip's worth by cutting K, where every slice keeps 32 blocks
-// (50 us: the partial sums and their folding cost a tenth of it) and the cut is even.
-int clt_internal_gemm8_large_slices(int M, int N, int KB, int batch) {
-    const long total = ((long)(M - 1) / 256 + 1) * ((N - 1) / 256 + 1) * batch;
-    if (KB < 1 || M < 128 || N < 128 || total < 64 || total > 0x3fffffffL) return 0;
-    for (int s = (int)(256 / total); s > 1; --s)
-        if (KB % s == 0 && KB / s >= 32) return s;
-    return total >= 128 ? 1 : 0;
-}
 
 // dtype: of the product asked for (it picks the instructions); g.part: partial sums go there, unfolded
 int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, hipStream_t st) {
