@@ -109,6 +109,7 @@ SIGNATURES = {
     "clt_adam_prep_f32": (I, [P, P, P, P, I, I, I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, I, I, P, P, P, P, P, P]),
     "clt_pack8_sums_workspace_bytes": (SZ, [I, I, I]),
     "clt_pack8": (I, [P, I, L, L, I, I, I, I, I, P, P, P, P, P, P, SZ, P]),
+    "clt_pack8_into": (I, [P, I, L, L, I, I, I, I, I, P, P, L, L, L, P, P, L, L, L, P, P, SZ, P]),
     "clt_unpack8": (I, [P, P, I, I, I, I, L, L, L, L, P, I, P]),
     "clt_gemm8_workspace_bytes": (SZ, [I, I, I, I]),
     "clt_gemm8": (I, [P, P, I, L, L, L, L, P, P, I, L, L, L, L, P, I, L, L, P, L, I, I, I, I, I, P, SZ, P]),

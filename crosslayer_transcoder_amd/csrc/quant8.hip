@@ -16,6 +16,7 @@ struct Pack8Args {
     const void* x; long row_stride, batch_stride;
     uint8_t *q, *s;            // row form (or nullptr): codes [L][R][Cp], scale bytes [L][Cp / 128][Rp]
     uint8_t *qt, *st;          // transposed form (or nullptr): codes [L][C][Rp], scale bytes [L][Rp / 128][Cp]
+    long q_pitch, q_batch, s_batch, qt_pitch, qt_batch, st_batch;            // bytes
     float* sums;               // column sums of each 128-row block [L][Rp / 128][C] (or nullptr)
     int R, C, tiles_r, tiles_c;
 };
@@ -124,9 +125,9 @@ template <int DT, int FMT, bool TILES> __global__ __launch_bounds__(256) void pa
             uint2 o;
             o.x = pack_codes<FMT>(v[i][0], v[i][1], v[i][2], v[i][3], f);
             o.y = pack_codes<FMT>(v[i][4], v[i][5], v[i][6], v[i][7], f);
-            if (r < a.R) *reinterpret_cast<uint2*>(a.q + (b * a.R + r) * Cp + c0 + cg * 8) = o;
+            if (r < a.R) *reinterpret_cast<uint2*>(a.q + b * a.q_batch + r * a.q_pitch + c0 + cg * 8) = o;
         }
-        if (cg == 0) *reinterpret_cast<uint2*>(a.s + (b * a.tiles_c + tc) * Rp + r0 + rg * 8) = make_uint2(sb[0], sb[1]);
+        if (cg == 0) *reinterpret_cast<uint2*>(a.s + b * a.s_batch + tc * Rp + r0 + rg * 8) = make_uint2(sb[0], sb[1]);
     }
     if (a.qt) {
         uint32_t sb[2] = {0u, 0u};
@@ -141,14 +142,14 @@ template <int DT, int FMT, bool TILES> __global__ __launch_bounds__(256) void pa
             // 8-byte chunk rg of column c, chunks XOR-swizzled with the column group (the 16 groups of a store hit 16 chunks)
             *reinterpret_cast<uint2*>(tile + c * B8 + ((rg ^ cg) << 3)) = o;
         }
-        if (rg == 0) *reinterpret_cast<uint2*>(a.st + (b * a.tiles_r + tr) * Cp + c0 + cg * 8) = make_uint2(sb[0], sb[1]);
+        if (rg == 0) *reinterpret_cast<uint2*>(a.st + b * a.st_batch + tr * Cp + c0 + cg * 8) = make_uint2(sb[0], sb[1]);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int id = k * 256 + tid, c = id >> 3, p = id & 7, x = c >> 3;
             const uint2 lo = *reinterpret_cast<const uint2*>(tile + c * B8 + (((2 * p) ^ x) << 3));
             const uint2 hi = *reinterpret_cast<const uint2*>(tile + c * B8 + (((2 * p + 1) ^ x) << 3));
-            if (c0 + c < a.C) *reinterpret_cast<uint4*>(a.qt + (b * a.C + c0 + c) * Rp + r0 + p * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            if (c0 + c < a.C) *reinterpret_cast<uint4*>(a.qt + b * a.qt_batch + (c0 + c) * a.qt_pitch + r0 + p * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
     }
 }
@@ -217,11 +218,22 @@ extern "C" size_t clt_pack8_sums_workspace_bytes(int batch, int rows, int cols) 
 extern "C" int clt_pack8(const void* x, int dtype, long row_stride, long batch_stride, int batch, int rows, int cols, int format,
                          int tiles, void* q, void* s, void* qt, void* st, float* column_sums, void* workspace,
                          size_t workspace_bytes, void* stream) {
+    const long Rp = up128(rows), Cp = up128(cols);
+    return clt_pack8_into(x, dtype, row_stride, batch_stride, batch, rows, cols, format, tiles, q, s, Cp, rows * Cp, Cp / B8 * Rp, qt, st,
+                          Rp, cols * Rp, Rp / B8 * Cp, column_sums, workspace, workspace_bytes, stream);
+}
+
+extern "C" int clt_pack8_into(const void* x, int dtype, long row_stride, long batch_stride, int batch, int rows, int cols, int format,
+                              int tiles, void* q, void* s, long q_pitch, long q_batch, long s_batch, void* qt, void* st, long qt_pitch,
+                              long qt_batch, long st_batch, float* column_sums, void* workspace, size_t workspace_bytes, void* stream) {
     if (batch <= 0 || rows <= 0 || cols <= 0 || dtype < 0 || dtype > 2 || format < 0 || format > 1) return CLT_ERR_SHAPE;
     if (!x || !q != !s || !qt != !st || (!q && !qt)) return CLT_ERR_SHAPE;
     const size_t es = dtype == CLT_DT_F32 ? 4 : 2;
     if (((uintptr_t)x & (es - 1)) || !(aligned16(q) && aligned16(s) && aligned16(qt) && aligned16(st))) return CLT_ERR_ALIGN;
+    if ((q && q_pitch < up128(cols)) || (qt && qt_pitch < up128(rows))) return CLT_ERR_SHAPE;
+    if (((q_pitch | q_batch | s_batch | qt_pitch | qt_batch | st_batch) & 15)) return CLT_ERR_ALIGN;
     Pack8Args a;
+    a.q_pitch = q_pitch; a.q_batch = q_batch; a.s_batch = s_batch; a.qt_pitch = qt_pitch; a.qt_batch = qt_batch; a.st_batch = st_batch;
     a.x = x; a.row_stride = row_stride; a.batch_stride = batch_stride;
     a.q = static_cast<uint8_t*>(q); a.s = static_cast<uint8_t*>(s); a.qt = static_cast<uint8_t*>(qt); a.st = static_cast<uint8_t*>(st);
     a.R = rows; a.C = cols; a.tiles_r = (rows - 1) / B8 + 1; a.tiles_c = (cols - 1) / B8 + 1;

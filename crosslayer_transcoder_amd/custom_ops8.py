@@ -8,7 +8,8 @@ the same read (1 byte), and W8 in the orientation the input gradient contracts. 
 the same two forms: dx = g8 W8^T, dW = X8t g8t^T, db = the sum of g itself, taken by the pass that packs it.  These are the
 straight-through gradients: rounding to 8 bits counts as the identity.
 
-y and dx have x's type (dx of the cross-layer decoder is summed in fp32 first), dW has W's, db has b's."""
+y and dx have x's type, dW has W's, db has b's.  A training step can be captured into a graph, forward and backward, as long as no
+eager graph of the same leaves is alive then (torch's own rule: the engine would wait for the stream that graph was made on)."""
 from typing import List, Optional
 
 import torch
@@ -214,10 +215,44 @@ def plt_decoder8(feat: Tensor, W: Tensor, b: Optional[Tensor]) -> Tensor:
 
 
 # ---- cross-layer decoder: recons[:, l] = feat[:, :l+1].flatten(1) @ W_l.flatten(0, 1) + b[l] (reference model/clt.py:334-343) ----------
-# Blocks run along the flattened (source layer, feature) axis.  The features are packed once and every target layer contracts over its
-# first (l + 1) F columns; where F is no multiple of 128 a block would straddle that border, and every prefix is packed by itself.
+# Forward, blocks along the flattened (source layer, feature) axis: the features are packed once and target layer l contracts over the
+# first (l + 1) F columns.  Gradient of source layer s: one product over the flattened (target layer, output) axis from s on,
+#   dfeat[:, s] = [g_s .. g_{L-1}] [W_s[s]; ..; W_{L-1}[s]]^T,
+# whose right operand the packing of each W_l fills in, block of columns by block of columns.  Both need borders between layers that are
+# borders between blocks.  Where d is no multiple of 128 the L products of the targets are added up in fp32 instead (forward and
+# backward of 12 layers, d = 768, 8192 features, 4096 tokens in fp32: 14.8 ms that way, 12.0 ms this way), and where F is none every prefix of the features is packed by itself.
+def _clt_aligned(F, d):
+    return F % ops8.BLOCK == 0 and d % ops8.BLOCK == 0
+
+
+# The right operands of all source layers in [H, F, (L + 1) d], H = (L + 1) // 2: row p holds source layer p (targets p .. L - 1) and behind
+# it source layer L - 1 - p (targets L - 1 - p .. L - 1), which fill it exactly (a middle layer's own row is half empty).
+def _clt_source(s, L, d):
+    """-> (row, first column) of source layer s."""
+    return (s, 0) if s < (L + 1) // 2 else (L - 1 - s, (s + 1) * d)
+
+
+def _clt_pack_weight(W, l, L, kq, ks, tq, ts):
+    """W_l [l + 1, F, d] -> its transpose [d, (l + 1) F] (tq, ts) and its columns of every source layer's operand (kq, ks; or None)."""
+    n, F, d = W.shape
+    H, pitch, K = (L + 1) // 2, (L + 1) * d, (l + 1) * F
+    with ops8._on(W.device):
+        st = ops8._stream(W.device)
+        for s0, s1 in ((0, min(n, H)), (H, n)):              # (the layers of the second half lie the other way round)
+            if s0 >= s1:
+                continue
+            (p, c), step = _clt_source(s0, L, d), 1 if s0 == 0 else -1
+            at = lambda t, rows, p, c: t.data_ptr() + (p * rows * pitch + c) if t is not None else None  # noqa: E731
+            c += (l - s0) * d                                # (one source layer further, this target lies d columns further left or right)
+            q, s = (at(kq, F, p, c), ks.data_ptr() + (p * pitch + c) // 128 * F) if kq is not None else (None, None)
+            _call(lib.clt_pack8_into, W.data_ptr() + s0 * W.stride(0) * W.element_size(), _DT[W.dtype], W.stride(1), W.stride(0), s1 - s0, F, d, _E4M3, 1,
+                  q, s, pitch, step * F * pitch + (-d if s0 == 0 else 0), (step * pitch + (-d if s0 == 0 else 0)) // 128 * F,
+                  tq.data_ptr() + s0 * F, ts.data_ptr() + s0 * F // 128 * d, K, F, F // 128 * d, None, None, 0, st)
+
+
 def _clt_forward(feat, b, Ws, keep_x, keep_w):
-    """-> recons [B, L, d], kept: [x transposed (codes, scale bytes)] + [W_l for the input gradient (codes, scale bytes)] ..."""
+    """-> recons [B, L, d], kept: [x transposed (codes, scale bytes)] + the weights for the input gradient: [codes, scale bytes] of all source
+    layers' operands, or [W_l (codes, scale bytes)] ... where the borders are not the blocks'."""
     feat = ops8._dense(feat, (3,)).contiguous()
     B, L, F = feat.shape
     d = Ws[0].shape[2]
@@ -225,38 +260,57 @@ def _clt_forward(feat, b, Ws, keep_x, keep_w):
         raise ValueError(f"empty map: features {tuple(feat.shape)}, W_0 {tuple(Ws[0].shape)}")
     flat = feat.view(B, L * F)
     out = torch.empty((B, L, d), dtype=feat.dtype, device=feat.device)
-    whole = F % ops8.BLOCK == 0
+    whole, aligned = F % ops8.BLOCK == 0, _clt_aligned(F, d)
     q, s, xt, xs, _ = ops8.pack8_raw(flat.unsqueeze(0), _E4M3, whole, keep_x) if whole or keep_x else (None,) * 5
     kept = [xt, xs] if keep_x else []
     x = ops8.Block8(q, s, B, L * F) if whole else None
+    kq = ks = None
+    if aligned and keep_w:
+        kq, ks = feat.new_empty(((L + 1) // 2, F, (L + 1) * d), dtype=torch.uint8), feat.new_empty(((L + 1) // 2, (L + 1) * d // 128, F), dtype=torch.uint8)
+        kept += [kq, ks]
     for l, W in enumerate(Ws):
         K = (l + 1) * F
-        dq, ds, tq, ts, _ = ops8.pack8_raw(ops8._dense(W, (3,)).reshape(1, K, d), _E4M3, keep_w, True, tiles=True)
-        if keep_w:
-            kept += [dq, ds]
+        W = ops8._dense(W, (3,))
+        if aligned:
+            tq, ts = feat.new_empty((1, d, K), dtype=torch.uint8), feat.new_empty((1, K // 128, d), dtype=torch.uint8)
+            _clt_pack_weight(W, l, L, kq, ks, tq, ts)
+        else:
+            dq, ds, tq, ts, _ = ops8.pack8_raw(W.reshape(1, K, d), _E4M3, keep_w, True, tiles=True)
+            if keep_w:
+                kept += [dq, ds]
         ops8.gemm8(x.first_columns(K) if whole else ops8.quantize8(flat[:, :K]), ops8.Block8(tq, ts, d, K), None if b is None else b[l:l + 1],
                    out=out[:, l].unsqueeze(0))
     return out, kept
 
 
 def _clt_gradients(g, kept, F, has_x, need_dx, w_dtypes, need_db):
-    """-> dfeat fp32 [B, L, F], [dW_l [l + 1, F, d]], db fp32 [L, d]; None where not asked for (w_dtypes empty: no dW)."""
+    """-> dfeat [B, L, F] of g's type, [dW_l [l + 1, F, d]], db fp32 [L, d]; None where not asked for (w_dtypes empty: no dW)."""
     g = ops8._dense(g, (3,))
     B, L, d = g.shape
-    q, s, qt, qs, db = ops8.pack8_raw(g.transpose(0, 1), _E4M3, need_dx or not w_dtypes, bool(w_dtypes), sums=need_db)
+    aligned = _clt_aligned(F, d)
+    # aligned: one matrix [B, L d], whose transpose holds layer l's in rows l d ..; else a matrix [B, d] for each layer
+    m = g.reshape(1, B, L * d) if aligned else g.transpose(0, 1)
+    q, s, qt, qs, db = ops8.pack8_raw(m, _E4M3, need_dx or not w_dtypes, bool(w_dtypes), sums=need_db)
     dx, dWs = None, None
-    if need_dx:
+    ws = kept[2:] if has_x else kept
+    if need_dx and aligned:
+        dx = torch.empty((B, L, F), dtype=g.dtype, device=g.device)
+        gb = ops8.Block8(q, s, B, L * d)
+        for k in range(L):
+            p, c = _clt_source(k, L, d)
+            w = ops8.Block8(ws[0][p:p + 1], ws[1][p:p + 1], F, (L + 1) * d)
+            ops8.gemm8(gb.columns(k * d, (L - k) * d), w.columns(c, (L - k) * d), out=dx[:, k].unsqueeze(0))
+    elif need_dx:
         dx = torch.empty((B, L * F), dtype=torch.float32, device=g.device)
-        ws = kept[2:] if has_x else kept
         for l in range(L - 1, -1, -1):                     # (the last layer reaches every column and writes; the others add)
             K = (l + 1) * F
             ops8.gemm8(ops8.Block8(q[l:l + 1], s[l:l + 1], B, d), ops8.Block8(ws[2 * l], ws[2 * l + 1], K, d), out=dx[:, :K].unsqueeze(0), accumulate=l != L - 1)
-        dx = dx.view(B, L, F)
+        dx = dx.view(B, L, F).to(g.dtype)
     if w_dtypes:
         x = ops8.Block8(kept[0], kept[1], L * F, B)
-        dWs = [ops8.gemm8(x.first_rows((l + 1) * F), ops8.Block8(qt[l:l + 1], qs[l:l + 1], d, B), out_dtype=dt).view(l + 1, F, d)
-               for l, dt in enumerate(w_dtypes)]
-    return dx, dWs, db
+        gt = [ops8.Block8(qt[:, l * d:(l + 1) * d], qs[:, :, l * d:(l + 1) * d], d, B) if aligned else ops8.Block8(qt[l:l + 1], qs[l:l + 1], d, B) for l in range(L)]
+        dWs = [ops8.gemm8(x.first_rows((l + 1) * F), gt[l], out_dtype=dt).view(l + 1, F, d) for l, dt in enumerate(w_dtypes)]
+    return dx, dWs, db.view(L, d) if need_db else None
 
 
 @torch.library.custom_op("clt_hip::clt_decoder8", mutates_args=(), device_types=_DEV)
@@ -272,14 +326,17 @@ def _(feat, b, Ws, keep_x, keep_w):
     d = Ws[0].shape[2]
     form = lambda rows, cols: [feat.new_empty((1, rows, _up(cols)), dtype=torch.uint8), feat.new_empty((1, _up(cols) // 128, _up(rows)), dtype=torch.uint8)]  # noqa: E731
     kept = form(L * F, B) if keep_x else []
-    for l in range(L if keep_w else 0):
-        kept += form((l + 1) * F, d)
+    if keep_w and _clt_aligned(F, d):
+        kept += [feat.new_empty(((L + 1) // 2, F, (L + 1) * d), dtype=torch.uint8), feat.new_empty(((L + 1) // 2, (L + 1) * d // 128, F), dtype=torch.uint8)]
+    elif keep_w:
+        for l in range(L):
+            kept += form((l + 1) * F, d)
     return [feat.new_empty(B, L, d)] + kept
 
 
 @torch.library.custom_op("clt_hip::clt_decoder8_bwd", mutates_args=(), device_types=_DEV)
 def _clt_decoder8_bwd(g: Tensor, kept: List[Tensor], F: int, has_x: bool, need_dx: bool, w_dtype: Optional[torch.dtype], need_db: bool) -> List[Tensor]:
-    """-> [dfeat fp32, db fp32 (empty where not asked for), dW_0, ..., dW_{L-1} (w_dtype None: none)]."""
+    """-> [dfeat of g's type, db fp32 (empty where not asked for), dW_0, ..., dW_{L-1} (w_dtype None: none)]."""
     dx, dWs, db = _clt_gradients(g, kept, F, has_x, need_dx, [w_dtype] * g.shape[1] if w_dtype is not None else [], need_db)
     return [g.new_empty(0) if t is None else t for t in (dx, db)] + (dWs or [])
 
@@ -288,13 +345,13 @@ def _clt_decoder8_bwd(g: Tensor, kept: List[Tensor], F: int, has_x: bool, need_d
 def _(g, kept, F, has_x, need_dx, w_dtype, need_db):
     B, L, d = g.shape
     f32 = torch.float32
-    out = [g.new_empty((B, L, F), dtype=f32) if need_dx else g.new_empty(0), g.new_empty((L, d), dtype=f32) if need_db else g.new_empty(0)]
+    out = [g.new_empty((B, L, F)) if need_dx else g.new_empty(0), g.new_empty((L, d), dtype=f32) if need_db else g.new_empty(0)]
     return out + [g.new_empty((l + 1, F, d), dtype=w_dtype) for l in range(L if w_dtype is not None else 0)]
 
 
 def _clt_setup(ctx, inputs, output):
     feat, b, Ws, ctx.keep_x, ctx.keep_w = inputs
-    ctx.F, ctx.x_dtype, ctx.w_dtype, ctx.b = feat.shape[2], feat.dtype, Ws[0].dtype, None if b is None else (b.dtype, b.shape)
+    ctx.F, ctx.w_dtype, ctx.b = feat.shape[2], Ws[0].dtype, None if b is None else (b.dtype, b.shape)
     ctx.save_for_backward(*output[1:])
 
 
@@ -303,7 +360,7 @@ def _clt_backward(ctx, grads):
     if (need_w and not ctx.keep_x) or (need_x and not ctx.keep_w):
         raise RuntimeError("clt_decoder8 was called without keeping what this gradient needs (keep_x for dW, keep_w for the features')")
     dx, db, *dWs = torch.ops.clt_hip.clt_decoder8_bwd(grads[0], list(ctx.saved_tensors), ctx.F, ctx.keep_x, need_x, ctx.w_dtype if need_w else None, need_b)
-    return dx.to(ctx.x_dtype) if need_x else None, db.to(ctx.b[0]).reshape(ctx.b[1]) if need_b else None, list(dWs) if need_w else None, None, None
+    return dx if need_x else None, db.to(ctx.b[0]).reshape(ctx.b[1]) if need_b else None, list(dWs) if need_w else None, None, None
 
 
 _clt_decoder8_op.register_autograd(_clt_backward, setup_context=_clt_setup)
@@ -315,7 +372,7 @@ class _CltDecoder8(torch.autograd.Function):
         need_w = any(ctx.needs_input_grad[2:])
         out, kept = _clt_forward(feat, b, Ws, need_w, ctx.needs_input_grad[0])
         ctx.save_for_backward(*kept)
-        ctx.F, ctx.x_dtype, ctx.has_x, ctx.w_dtypes = feat.shape[2], feat.dtype, need_w, [w.dtype for w in Ws]
+        ctx.F, ctx.has_x, ctx.w_dtypes = feat.shape[2], need_w, [w.dtype for w in Ws]
         ctx.b = None if b is None else (b.dtype, b.shape)
         return out
 
@@ -325,12 +382,12 @@ class _CltDecoder8(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx, dWs, db = _clt_gradients(g, ctx.saved_tensors, ctx.F, ctx.has_x, need[0], ctx.w_dtypes if any(need[2:]) else [], need[1])
         dWs = [None] * len(ctx.w_dtypes) if dWs is None else [dW if n else None for dW, n in zip(dWs, need[2:])]
-        return (dx.to(ctx.x_dtype) if need[0] else None, db.to(ctx.b[0]).reshape(ctx.b[1]) if need[1] else None, *dWs)
+        return (dx, db.to(ctx.b[0]).reshape(ctx.b[1]) if need[1] else None, *dWs)
 
 
 def clt_decoder8(feat: Tensor, b: Optional[Tensor], Ws: List[Tensor]) -> Tensor:
     """recons [B, L, d] from feat [B, L, F] and Ws[l] [l + 1, F, d], b [L, d] (`clt_hip::clt_decoder`'s arguments)."""
-    if feat.dim() != 3 or len(Ws) != feat.shape[1] or any(W.dim() != 3 or tuple(W.shape) != (l + 1, feat.shape[2], Ws[0].shape[2]) for l, W in enumerate(Ws)):
+    if feat.dim() != 3 or not Ws or len(Ws) != feat.shape[1] or any(W.dim() != 3 or tuple(W.shape) != (l + 1, feat.shape[2], Ws[0].shape[2]) for l, W in enumerate(Ws)):
         raise ValueError(f"features {tuple(feat.shape)} do not match the decoder weights {[tuple(W.shape) for W in Ws]}")
     if any(W.device != feat.device or W.dtype != Ws[0].dtype for W in Ws):
         raise ValueError("the decoder weights are of one type, on the features' device")

@@ -4,7 +4,8 @@ weights, products of packed matrices, and the linear map of a few or many tokens
 A matrix [R, C] is held as 8-bit floats with one power-of-two scale for every row and block of 128 columns (`Block8`).
 Tensors may be fp32, bf16 or fp16, of any size (zero rows included) and with any strides as long as the last dimension is
 dense; everything runs on the tensors' device and on that device's current stream, allocates only through torch's caching
-allocator and can be captured into a graph.  Non-HIP tensors raise: there is no fallback."""
+allocator and can be captured into a graph.  Nothing here is differentiable: custom_ops8.py is.  Non-HIP tensors raise: there is
+no fallback."""
 from __future__ import annotations
 
 import contextlib
@@ -62,7 +63,7 @@ def _dense(x: torch.Tensor, dims=(2, 3)) -> torch.Tensor:
 class Block8:
     """A batch of matrices [L, rows, cols] in 8 bits.  data: uint8 [L, rows, >= cols rounded up to 128], rows 16-byte aligned,
     codes of `fmt` ("e4m3" / "e5m2"), ZERO behind column `cols` up to the next multiple of 128; scale: uint8 [L, >= blocks of 128
-    columns, >= rows], rows 4-byte aligned, byte e + 127 for the scale 2^e of a row's block.  The pack functions below make it; one may be built
+    columns, >= rows], rows 4-byte aligned, byte e + 127 (1 to 254) for the scale 2^e of a row's block.  The pack functions below make it; one may be built
     from kept tensors (a checkpoint of packed weights) as well."""
     __slots__ = ("data", "scale", "rows", "cols", "fmt")
 
@@ -97,9 +98,13 @@ class Block8:
 
     def first_columns(self, n: int) -> "Block8":
         """View of the first n columns, n a multiple of 128 (a block belongs to one contraction)."""
-        if not 0 <= n <= self.cols or (n % BLOCK and n != self.cols):
-            raise ValueError(f"first {n} of {self.cols} columns: a multiple of {BLOCK} is needed")
-        return Block8(self.data, self.scale, self.rows, n, self.fmt)
+        return self.columns(0, n)
+
+    def columns(self, start: int, n: int) -> "Block8":
+        """View of n columns from `start`, a multiple of 128; n too unless they reach the last one."""
+        if not 0 <= start <= start + n <= self.cols or start % BLOCK or (n % BLOCK and start + n != self.cols):
+            raise ValueError(f"columns {start} .. {start + n} of {self.cols}: multiples of {BLOCK} are needed")
+        return Block8(self.data[:, :, start:], self.scale[:, start // BLOCK:], self.rows, n, self.fmt)
 
     def of_batch(self, l: int) -> "Block8":
         """View of one matrix of the batch."""
@@ -209,6 +214,14 @@ def _bias(bias, L, N, device):
     return bias.to(torch.float32).contiguous()
 
 
+def _separate(out):
+    """Whether the rows of out [L, M, N] are dense and no two of them share an element."""
+    (L, M, N), (sb, sr, sc) = out.shape, out.stride()
+    if (N > 1 and sc != 1) or (M > 1 and sr < N) or (L > 1 and sb < N):
+        return False
+    return L == 1 or M == 1 or sb >= (M - 1) * sr + N or sr >= (L - 1) * sb + N
+
+
 def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32,
           out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """out [L, M, N] (+)= a [L, M, K] @ b [L, N, K]^T + bias [L, N].  fp32 results: exact products, fp32 sums; bf16 / fp16 results:
@@ -226,7 +239,7 @@ def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: 
         out = torch.empty((L, M, N), dtype=out_dtype, device=a.device)
     elif out.dtype not in _DT or (accumulate and out.dtype != torch.float32):
         raise TypeError(f"cannot {'add to' if accumulate else 'write'} {out.dtype}")
-    elif tuple(out.shape) != (L, M, N) or out.device != a.device or (N > 1 and out.stride(2) != 1) or (M > 1 and out.stride(1) < N):
+    elif tuple(out.shape) != (L, M, N) or out.device != a.device or (out.numel() and not _separate(out)):
         raise ValueError(f"out must be an [{L}, {M}, {N}] tensor of non-overlapping dense rows on the operands' device")
     bias = _bias(bias, L, N, a.device)
     if out.numel():
@@ -243,7 +256,8 @@ def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: 
 
 def linear8(x: torch.Tensor, w: Block8, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y [T, L, N] = x [T, L, K] @ w^T + bias with kept packed weights w [L, N, K] (x [T, K] -> y [T, N] when L == 1): x is packed in
-    e4m3 with blocks along K on the way.  out_dtype: x's by default."""
+    e4m3 with blocks along K on the way.  out_dtype: x's by default.  Up to FEW_TOKENS the products are exact whatever the type,
+    above that as gemm8's: a token's 16-bit results may differ between the two in the last place."""
     x = _dense(x)
     _hip(w)
     two = x.dim() == 2

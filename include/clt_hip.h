@@ -548,6 +548,12 @@ int clt_sparse_scatter_dense_f32(const uint32_t* col_start, const int32_t* tok, 
 size_t clt_pack8_sums_workspace_bytes(int batch, int rows, int cols);
 int clt_pack8(const void* x, int dtype, long row_stride, long batch_stride, int batch, int rows, int cols, int format, int tiles,
               void* q, void* s, void* qt, void* st, float* column_sums, void* workspace, size_t workspace_bytes, void* stream);
+/* clt_pack8 into parts of larger held matrices: bytes from code row to code row and from matrix to matrix of the batch (negative ones
+ * too), multiples of 16.  Scale rows stay up128(rows) (st: up128(cols)) bytes apart.  The parts may not overlap: a row of codes
+ * is written up to up128 of its length. */
+int clt_pack8_into(const void* x, int dtype, long row_stride, long batch_stride, int batch, int rows, int cols, int format, int tiles,
+                   void* q, void* s, long q_pitch, long q_batch, long s_batch, void* qt, void* st, long qt_pitch, long qt_batch,
+                   long st_batch, float* column_sums, void* workspace, size_t workspace_bytes, void* stream);
 /* out [batch][rows][cols] (contiguous, dtype CLT_DT_*) = 2^e * code, rounded once.  pitch / scale_pitch: bytes per row of q / s. */
 int clt_unpack8(const void* q, const void* s, int format, int batch, int rows, int cols, long pitch, long scale_pitch,
                 long q_batch_stride, long s_batch_stride, void* out, int dtype, void* stream);

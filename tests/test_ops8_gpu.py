@@ -449,6 +449,12 @@ def test_opcheck():
     assert set(cases) == set(C.REGISTERED8)
     for name, args in cases.items():
         torch.library.opcheck(getattr(torch.ops.clt_hip, name).default, args)
+    # sizes that are multiples of 128: the cross-layer decoder keeps its weights by source layer
+    Ws = [(rnd(l + 1, 128, 128, seed=5 + l, spread=False) * 0.2).requires_grad_() for l in range(2)]
+    feat = torch.relu(rnd(9, 2, 128, seed=1, spread=False)).requires_grad_()
+    torch.library.opcheck(torch.ops.clt_hip.clt_decoder8.default, (feat, None, Ws, True, True))
+    kept = torch.ops.clt_hip.clt_decoder8(feat.detach(), None, [w.detach() for w in Ws], True, True)[1:]
+    torch.library.opcheck(torch.ops.clt_hip.clt_decoder8_bwd.default, (rnd(9, 2, 128, seed=4, spread=False), kept, 128, True, True, torch.float32, False))
 
 
 @gpu
@@ -516,10 +522,10 @@ def reference_clt(feat, Ws, b, g):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("shape", [(5, 3, 40, 30), (130, 2, 256, 70), (64, 4, 128, 110), (33, 1, 300, 64)])
+@pytest.mark.parametrize("shape", [(5, 3, 40, 30), (130, 2, 256, 70), (64, 4, 128, 110), (33, 1, 300, 64), (9, 1, 128, 128), (70, 3, 128, 128), (40, 4, 256, 384), (200, 5, 384, 128), (0, 3, 128, 128), (0, 2, 40, 30)])
 def test_cross_layer_decoder(shape, dtype):
-    """Dictionaries that are a multiple of 128 (one packing for all target layers) and not; the features' gradient is a sum of L
-    products in fp32, rounded once."""
+    """Dictionaries that are a multiple of 128 (one packing for all target layers) and not; outputs that are (the features' gradient is
+    one product a source layer) and not (a sum of L products in fp32, rounded once); odd and even numbers of layers; no tokens."""
     from crosslayer_transcoder_amd import custom_ops8 as C
     B, L, F, d = shape
     feat = torch.relu(rnd(B, L, F, seed=1, dtype=dtype, spread=False)).requires_grad_()
@@ -574,6 +580,29 @@ def test_modules_contract_in_8_bits(dec):
 
 
 @gpu
+@pytest.mark.parametrize("F,d", [(128, 128), (96, 64)])
+def test_cross_layer_decoder_parts(F, d):
+    """Each gradient alone equals the one computed with all of them; no gradient at all; a bias of another type."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    feat, b, g = torch.relu(rnd(20, 3, F, seed=1, spread=False)), rnd(3, d, seed=2, spread=False).half(), rnd(20, 3, d, seed=3, spread=False)
+    Ws = [rnd(l + 1, F, d, seed=4 + l, spread=False) * 0.1 for l in range(3)]
+    leaves = [feat, b] + Ws
+    def grads(which):
+        t = [u.detach().requires_grad_(i in which) for i, u in enumerate(leaves)]
+        y = C.clt_decoder8(t[0], t[1], t[2:])
+        return y, torch.autograd.grad(y, [t[i] for i in which], g) if which else ()
+    y, full = grads(range(5))
+    assert full[1].dtype == torch.float16
+    for which in ([0], [1], [3], [0, 4], []):
+        z, part = grads(which)
+        assert torch.equal(y, z) and all(torch.equal(full[i], u) for i, u in zip(which, part))
+    with torch.no_grad():
+        assert torch.equal(C.clt_decoder8(*leaves[:2], leaves[2:]), y)
+    c = torch.compile(lambda f, b, *w: C.clt_decoder8(f, b, list(w)), backend="aot_eager")(*(u.detach().requires_grad_() for u in leaves))
+    assert torch.equal(c, y)
+
+
+@gpu
 def test_layers_with_packed_weights():
     """forward_layer(packed=pack8()): one token and a batch, every layer, encoder and both decoders."""
     from crosslayer_transcoder_amd import ops8
@@ -597,6 +626,16 @@ def test_layers_with_packed_weights():
             f = torch.relu(rnd(*shape, L, F, seed=l, spread=False))
             z = plt.forward_layer(f, l, packed=pp)
             check_product(z.reshape(1, -1, d), ops8.quantize8(f[:, :, l].reshape(1, -1, F)), pp.of_batch(l), plt.b[l:l + 1])
+
+
+def test_results_that_share_elements_are_refused():
+    from crosslayer_transcoder_amd.ops8 import _separate
+    t = torch.empty(400)
+    for good in (t[:24].view(2, 3, 4), t[:24].view(3, 2, 4).transpose(0, 1), t[:40].view(2, 4, 5)[:, :3, :4], t[:4].view(1, 1, 4), t[:6].view(6, 1, 1), t.as_strided((1, 1, 4), (0, 0, 1))):
+        assert _separate(good), (good.shape, good.stride())
+    for bad in (t[:4].view(1, 1, 4).expand(2, 1, 4), t[:12].view(1, 3, 4).expand(2, 3, 4), t.as_strided((2, 3, 4), (4, 4, 1)), t.as_strided((2, 3, 4), (12, 3, 1)),
+                t.as_strided((1, 3, 4), (12, 4, 2)), t.as_strided((3, 2, 4), (4, 8, 1))):
+        assert not _separate(bad), (bad.shape, bad.stride())
 
 
 # ---- refusals (host checks: they run on the CPU) -----------------------------------------------------------------------------
@@ -638,7 +677,9 @@ def test_refusals_of_block8():
         Block8(u(2, 5, 128).float(), u(2, 1, 8), 5, 100)
     q = Block8(u(2, 5, 384), u(2, 3, 128), 5, 300)
     assert q.first_rows(3).rows == 3 and q.first_columns(256).cols == 256 and q.of_batch(1).batch == 1
-    for bad in (lambda: q.first_rows(6), lambda: q.first_columns(200), lambda: q.first_columns(384)):
+    assert q.columns(128, 128).cols == 128 and q.columns(256, 0).cols == 0 and q.columns(128, 172).cols == 172
+    for bad in (lambda: q.first_rows(6), lambda: q.first_columns(200), lambda: q.first_columns(384), lambda: q.columns(64, 64), lambda: q.columns(128, 100),
+                lambda: q.columns(256, 128), lambda: q.columns(-128, 128), lambda: q.columns(128, -128)):
         with pytest.raises(ValueError):
             bad()
 
@@ -656,6 +697,11 @@ def test_refusals_of_the_library():
     assert [pack(r=0), pack(c=-1), pack(b=0), pack(dt=3), pack(f=2), pack(s=None), pack(q=None, s=None), pack(x=None)] == [-1] * 8
     assert [pack(x=p + 2), pack(q=p + 8), pack(s=p + 1)] == [-4] * 3
     assert pack(cs=p) == -3 and pack(cs=p, ws=p, n=255) == -3
+
+    def into(pitch=128, batch=0, qt=None, qt_pitch=0):
+        return lib.clt_pack8_into(p, 0, 64, 0, 1, 4, 64, 0, 0, p, p, pitch, batch, 0, qt, qt, qt_pitch, 0, 0, None, None, 0, None)
+
+    assert [into(pitch=64), into(qt=p), into(pitch=136), into(batch=8), into(qt=p, qt_pitch=132)] == [-1, -1, -4, -4, -4]
 
     def gemm(a=p, lda=128, ldas=128, b=p, ldb=128, ldbs=128, c=p, dt=0, ldc=64, M=4, N=4, K=100, batch=1, acc=0, fa=0, bias=None):
         return lib.clt_gemm8(a, p, fa, lda, ldas, 0, 0, b, p, 0, ldb, ldbs, 0, 0, c, dt, ldc, 0, bias, 0, M, N, K, batch, acc, None, 0, None)
