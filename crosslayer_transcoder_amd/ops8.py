@@ -82,6 +82,13 @@ class Block8:
             raise ValueError("packed rows are dense and start at multiples of 16 bytes (codes) and 4 bytes (scales)")
         self.data, self.scale, self.rows, self.cols, self.fmt = data, scale, rows, cols, fmt
 
+    @classmethod
+    def _made(cls, data, scale, rows, cols, fmt):
+        """Of tensors that a pack function here made (the checks above are 2 us of a 10 us call)."""
+        q = cls.__new__(cls)
+        q.data, q.scale, q.rows, q.cols, q.fmt = data, scale, rows, cols, fmt
+        return q
+
     @property
     def batch(self) -> int:
         return self.data.shape[0]
@@ -153,35 +160,35 @@ def quantize8(x: torch.Tensor, fmt: str = "e4m3") -> Block8:
     """x [R, C] or [L, R, C] held with blocks along its columns (the operand of a contraction over them)."""
     x = _as3(x)
     q, s, *_ = pack8_raw(x, _fmt(fmt), True, False)
-    return Block8(q, s, x.shape[1], x.shape[2], fmt)
+    return Block8._made(q, s, x.shape[1], x.shape[2], fmt)
 
 
 def quantize8_t(x: torch.Tensor, fmt: str = "e4m3") -> Block8:
     """x^T [C, R] held with blocks of 128 rows of x: the 8-bit checkpoint a contraction over the rows (a weight gradient) reads."""
     x = _as3(x)
     _, _, q, s, _ = pack8_raw(x, _fmt(fmt), False, True)
-    return Block8(q, s, x.shape[2], x.shape[1], fmt)
+    return Block8._made(q, s, x.shape[2], x.shape[1], fmt)
 
 
 def quantize8_both(x: torch.Tensor, fmt: str = "e4m3") -> Tuple[Block8, Block8]:
     """(quantize8(x), quantize8_t(x)) from one read of x."""
     x = _as3(x)
     q, s, qt, st, _ = pack8_raw(x, _fmt(fmt), True, True)
-    return Block8(q, s, x.shape[1], x.shape[2], fmt), Block8(qt, st, x.shape[2], x.shape[1], fmt)
+    return Block8._made(q, s, x.shape[1], x.shape[2], fmt), Block8._made(qt, st, x.shape[2], x.shape[1], fmt)
 
 
 def quantize8_tiles(x: torch.Tensor, fmt: str = "e4m3") -> Tuple[Block8, Block8]:
     """A weight matrix and its transpose, one scale per 128 x 128 tile: both hold the same values."""
     x = _as3(x)
     q, s, qt, st, _ = pack8_raw(x, _fmt(fmt), True, True, tiles=True)
-    return Block8(q, s, x.shape[1], x.shape[2], fmt), Block8(qt, st, x.shape[2], x.shape[1], fmt)
+    return Block8._made(q, s, x.shape[1], x.shape[2], fmt), Block8._made(qt, st, x.shape[2], x.shape[1], fmt)
 
 
 def quantize8_weights(x: torch.Tensor, transposed: bool = False, fmt: str = "e4m3") -> Block8:
     """One form of quantize8_tiles: a weight matrix [N, K] as linear8 and gemm8 contract it, or (transposed) a [K, N] one."""
     x = _as3(x)
     q, s, qt, st, _ = pack8_raw(x, _fmt(fmt), not transposed, transposed, tiles=True)
-    return Block8(qt, st, x.shape[2], x.shape[1], fmt) if transposed else Block8(q, s, x.shape[1], x.shape[2], fmt)
+    return Block8._made(qt, st, x.shape[2], x.shape[1], fmt) if transposed else Block8._made(q, s, x.shape[1], x.shape[2], fmt)
 
 
 def dequantize8(q: Block8, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -211,7 +218,7 @@ def _bias(bias, L, N, device):
         raise ValueError(f"bias must be [{L}, {N}] on the operands' device")
     if not bias.dtype.is_floating_point:
         raise TypeError(f"bias must be floating point, got {bias.dtype}")
-    return bias.to(torch.float32).contiguous()
+    return bias if bias.dtype is torch.float32 and bias.is_contiguous() else bias.to(torch.float32).contiguous()
 
 
 def _separate(out):
