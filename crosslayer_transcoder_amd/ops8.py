@@ -115,6 +115,8 @@ class Block8:
 
     def of_batch(self, l: int) -> "Block8":
         """View of one matrix of the batch."""
+        if not 0 <= l < self.batch:
+            raise ValueError(f"matrix {l} of {self.batch}")
         return Block8(self.data[l:l + 1], self.scale[l:l + 1], self.rows, self.cols, self.fmt)
 
     def nbytes(self) -> int:
@@ -233,7 +235,8 @@ def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: 
           out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
     """out [L, M, N] (+)= a [L, M, K] @ b [L, N, K]^T + bias [L, N].  fp32 results: exact products, fp32 sums; bf16 / fp16 results:
     the 8-bit matrix instructions (twice the rate; their loss is far below the result's rounding).  `out`: an [L, M, N] tensor or
-    view with a dense last dimension to write into (its dtype counts); accumulate: add to it (fp32 only)."""
+    view with a dense last dimension to write into (its dtype counts), sharing nothing with the operands; accumulate: add to it (fp32
+    only).  The codes of a row of a or b take at most 8 MB."""
     _hip(a), _hip(b)
     L, M, N, K = a.batch, a.rows, b.rows, a.cols
     if b.batch != L or b.cols != K or b.device != a.device:

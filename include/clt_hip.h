@@ -560,7 +560,9 @@ int clt_unpack8(const void* q, const void* s, int format, int batch, int rows, i
 /* C[M][N] (+)= A[M][K] * B[N][K]^T + bias[N], batched; pitches and batch strides of A, B in bytes, of C and bias in elements.
  * c_dtype bf16 / fp16: 8-bit matrix instructions (products aligned to ~14 bits in groups of 16, fp32 sums, one rounding);
  * c_dtype fp32: exact products (bf16 instructions), fp32 sums; accumulate != 0 (fp32 only): C += . K = 0 gives the bias.
- * Scale rows: 4-byte aligned, readable up to a multiple of 4 bytes.  workspace (16-byte aligned): partial sums where K is cut. */
+ * Scale rows: 4-byte aligned, readable up to a multiple of 4 bytes.  Pitches below 2^23 bytes, an operand's scale bytes below 2^31 (else
+ * CLT_ERR_RANGE).  C shares no memory with the operands, nor its rows with each other.  workspace (16-byte aligned): partial sums
+ * where K is cut. */
 size_t clt_gemm8_workspace_bytes(int M, int N, int K, int batch);
 int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long ldas, long a_batch, long as_batch,
               const void* b, const void* b_scale, int b_format, long ldb, long ldbs, long b_batch, long bs_batch,

@@ -179,7 +179,7 @@ def test_product(shape, out):
 
 #: enough 256 x 256 tiles to fill the chip: whole and partial ones, 1, 2, 3 and many blocks of k, odd rows of results
 LARGE = [(1, 3000, 100, 2901), (12, 700, 256, 1100), (12, 701, 300, 1101), (3, 2048, 1024, 2048), (33, 300, 640, 515), (1, 128, 384, 40000),
-         (1, 2100, 8192, 1801), (2, 1100, 12200, 1700)]            # (and K in two and three slices)
+         (1, 2100, 8192, 1801), (2, 1100, 12200, 1700), (1, 800, 24576, 1900), (2, 600, 20480, 1801)]       # (the last two: and K in slices)
 
 
 @gpu
@@ -679,7 +679,7 @@ def test_refusals_of_block8():
     assert q.first_rows(3).rows == 3 and q.first_columns(256).cols == 256 and q.of_batch(1).batch == 1
     assert q.columns(128, 128).cols == 128 and q.columns(256, 0).cols == 0 and q.columns(128, 172).cols == 172
     for bad in (lambda: q.first_rows(6), lambda: q.first_columns(200), lambda: q.first_columns(384), lambda: q.columns(64, 64), lambda: q.columns(128, 100),
-                lambda: q.columns(256, 128), lambda: q.columns(-128, 128), lambda: q.columns(128, -128)):
+                lambda: q.of_batch(2), lambda: q.of_batch(-1), lambda: q.columns(256, 128), lambda: q.columns(-128, 128), lambda: q.columns(128, -128)):
         with pytest.raises(ValueError):
             bad()
 
