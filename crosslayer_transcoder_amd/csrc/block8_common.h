@@ -106,6 +106,7 @@ struct Gemm8Args {
     uint32_t inv_tiles, inv_panel, inv_rem;  // reciprocals of the large form's tile order (fast_div)
     int slices, slice_kb; float* part;       // K in slices: partial sums [slice][batch][M][N], else nullptr
     long slice_stride;                       // of the results (large form)
+    int first;                               // small tiles: the large form has done this many of its tiles (0: none of them)
 };
 
 // n / d for n < 2^31 with inv = (2^32 - 1) / d from the host: the estimate is at most one too small.  (A division in a kernel costs a
@@ -116,8 +117,35 @@ __device__ __forceinline__ int fast_div(int n, int d, uint32_t inv) {
     return q;
 }
 
-// 256 x 256 tiles (gemm8_large.hip)
-int clt_internal_gemm8_large(const Gemm8Args& g, int fa, int fb, int dtype, hipStream_t st);
+constexpr int B8_PANEL = 4;                          // A tiles of a panel
+struct B8Tile { int batch, slice, a0, b0; };
+// 256 x 256 tile of index vb: every XCD (index mod 8) works on a contiguous range of tiles, walked in panels of 4 A tiles with the A tile
+// fastest, so that the blocks an XCD runs together share operand tiles in its L2
+__device__ __forceinline__ B8Tile b8_tile(const Gemm8Args& g, int vb) {
+    const int nwg = g.tilesA * g.tilesB;
+    B8Tile t;
+    t.batch = fast_div(vb, nwg, g.inv_tiles);
+    int lid = vb - t.batch * nwg;
+    t.slice = 0;
+    if (g.slices > 1) { t.slice = t.batch / g.slices; t.slice = t.batch - t.slice * g.slices; t.batch = (t.batch - t.slice) / g.slices; }
+    const int xcd = lid & 7, q = nwg >> 3, r = nwg & 7;
+    lid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lid >> 3);
+    const int full = g.tilesA / B8_PANEL, rem = g.tilesA - full * B8_PANEL, per = B8_PANEL * g.tilesB;
+    int ta, tb;
+    if (lid < full * per) { const int pn = fast_div(lid, per, g.inv_panel), x = lid - pn * per; tb = x / B8_PANEL; ta = pn * B8_PANEL + (x - tb * B8_PANEL); }
+    else { const int x = lid - full * per; tb = fast_div(x, rem, g.inv_rem); ta = full * B8_PANEL + (x - tb * rem); }
+    t.a0 = ta * 256; t.b0 = tb * 256;
+    return t;
+}
+// for 256 x 256 tiles
+inline void b8_tile_order(Gemm8Args& g) {
+    g.tilesA = (g.M - 1) / 256 + 1; g.tilesB = (g.N - 1) / 256 + 1;
+    const int rem = g.tilesA % B8_PANEL;
+    g.inv_tiles = 0xffffffffu / (uint32_t)(g.tilesA * g.tilesB);
+    g.inv_panel = 0xffffffffu / (uint32_t)(B8_PANEL * g.tilesB);
+    g.inv_rem = rem ? 0xffffffffu / (uint32_t)rem : 0u;
+}
+int clt_internal_gemm8_large(const Gemm8Args& g, int fa, int fb, int dtype, int tiles, hipStream_t st);      // gemm8_large.hip
 
 // Four consecutive columns of a row of C: one store where the row's alignment allows it (vec), else element by element
 template <int DT> __device__ __forceinline__ void b8_store4(void* c, long at, b8_f32x4 v, int valid, bool vec, int accumulate) {

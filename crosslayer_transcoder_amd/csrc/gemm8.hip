@@ -37,12 +37,17 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256, 1) void gemm
     constexpr bool WIDE = DT == CLT_DT_F32;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
     const int wb = w >> 1, wa = w & 1;
-    const int nwg = g.tilesA * g.tilesB;
-    int id = blockIdx.x;
-    const int tile = id % nwg;
-    id /= nwg;
-    const int slice = id % g.slices, batch = id / g.slices;
-    const int a0 = tile % g.tilesA * 128, b0 = tile / g.tilesA * 128;
+    int a0, b0, slice = 0, batch;
+    if (g.first) {                                       // a quarter of one of the large tiles that are left
+        const B8Tile t = b8_tile(g, g.first + (blockIdx.x >> 2));
+        a0 = t.a0 + (blockIdx.x & 1) * 128; b0 = t.b0 + (blockIdx.x >> 1 & 1) * 128;
+        batch = t.batch;
+        if (a0 >= g.M || b0 >= g.N) return;
+    } else {
+        const int nwg = g.tilesA * g.tilesB, tile = blockIdx.x % nwg, id = blockIdx.x / nwg;
+        slice = id % g.slices; batch = id / g.slices;
+        a0 = tile % g.tilesA * 128; b0 = tile / g.tilesA * 128;
+    }
     const int k0 = slice * g.slice_kb, nk = min(g.slice_kb, g.KB - k0);
 
     // DMA: piece i of wave w fills LDS rows (4 i + w) * 8 .. + 7 of an operand.  Ranges end behind the tile's last row: rows past the
@@ -205,20 +210,26 @@ template <int DT> __global__ __launch_bounds__(256) void gemm8_fold_kernel(Gemm8
 // and 78 / 101; whole against sliced: 128 x 32768 x 768: 132 / 21; 1024 x 4096 x 768: 23 / 18; 1024 x 2048 x 2048: 16.3 / 20.1.
 // A slice keeps 4 blocks (the ring), slices of the large form are equal, partial sums take at most 256 MB.  The large form is not
 // for less than 128 rows on either side: such a tile is more than half empty (12 x (64 x 768 x 32768): 125 / 131).
-struct Plan { bool large; int slices; };
+// Large tiles that do not fill their last pass may be left to small ones (a second launch: 3): 4352 x 4096 x 4096 whole / shared 93 / 77
+// and 188 / 139; 12 x (4096 x 8192 x 768): 346 / 326 and 584 / 511.
+struct Plan { long large; int slices; };                 // large tiles (0: small ones only; else the rest are small), slices of K
 Plan plan_of(int M, int N, int KB, int batch, bool wide) {
-    const double elements = (double)batch * M * N;
-    Plan best = {false, 1};
+    const double elements = (double)batch * M * N, small = 7.0 + KB * (wide ? 1.0 : 0.6);
+    Plan best = {0, 1};
     double least = 1e30;
     for (int large = 0; large < 2; ++large) {
-        const long side = large ? 256 : 128, tiles = ((M - 1) / side + 1) * ((N - 1) / side + 1) * batch;
+        const long side = large ? 256 : 128, tiles = ((M - 1) / side + 1) * ((N - 1) / side + 1) * batch, full = tiles / 256 * 256;
         if (large && (M < 128 || N < 128 || KB < 1 || tiles > 0x3fffffffL)) break;
         const double block = large ? (wide ? 2.7 : 1.3) : wide ? 1.0 : 0.6, pass = large ? (wide ? 15.0 : 8.0) : 7.0;
         for (long s = 1; s == 1 || (s * tiles <= 256 && s * 4 <= KB && s * elements * 4.0 <= 268435456.0); ++s) {
             if (large && s > 1 && (KB % s || 1024L * N > 0x7fffffffL)) continue;       // (offsets of the partial sums: 32 bits)
             const long per = (KB + s - 1) / s, used = per ? (KB + per - 1) / per : 1;
             const double t = (double)((tiles * used + 255) / 256) * (per * block + pass) + (used > 1 ? 4.0 + used * elements * 8.0 / 5e6 : 0.0);
-            if (t < least) { least = t; best = {large != 0, (int)used}; }
+            if (t < least) { least = t; best = {large ? tiles : 0, (int)used}; }
+        }
+        if (large && full && full < tiles) {
+            const double t = (double)(full / 256) * (KB * block + pass) + (double)((4 * (tiles - full) + 255) / 256) * small + 3.0;
+            if (t < least) { least = t; best = {full, 1}; }
         }
     }
     return best;
@@ -268,23 +279,28 @@ extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long 
     if (KB && (256 * lda > 0x7fffffffL || 256 * ldb > 0x7fffffffL || KB * ldas > 0x7ffffeffL || KB * ldbs > 0x7ffffeffL)) return CLT_ERR_RANGE;
     Gemm8Args g = {static_cast<const uint8_t*>(a), static_cast<const uint8_t*>(a_scale), static_cast<const uint8_t*>(b),
                    static_cast<const uint8_t*>(b_scale), c, bias, lda, ldas, ldb, ldbs, ldc, a_batch, as_batch, b_batch, bs_batch,
-                   c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 0u, 0u, 0u, 1, KB, nullptr, 0};
+                   c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 0u, 0u, 0u, 1, KB, nullptr, 0, 0};
     const hipStream_t st = as_stream(stream);
     Plan plan = plan_of(M, N, KB, batch, c_dtype == CLT_DT_F32);
     // (results whose rows lie further apart than the large form's 32-bit offsets reach)
-    if (plan.large && plan.slices == 1 && 256 * ldc * 4 > 0x7fffffffL) plan.large = false;
+    if (plan.slices == 1 && 256 * ldc * 4 > 0x7fffffffL) plan.large = 0;
     g.slices = plan.slices;
     if (g.slices > 1) {
         if (!workspace || !aligned16(workspace) || workspace_bytes < (size_t)g.slices * batch * M * N * 4) return CLT_ERR_WORKSPACE;
         g.part = static_cast<float*>(workspace);
         g.slice_kb = (KB + g.slices - 1) / g.slices;
     }
+    long blocks = (long)g.tilesA * g.tilesB * batch * g.slices;
     if (plan.large) {
-        const int rc = clt_internal_gemm8_large(g, a_format, b_format, c_dtype, st);
-        if (rc != CLT_OK || !g.part) return rc;
-        return c_dtype == CLT_DT_F32 ? fold<CLT_DT_F32>(g, st) : c_dtype == CLT_DT_BF16 ? fold<CLT_DT_BF16>(g, st) : fold<CLT_DT_F16>(g, st);
+        b8_tile_order(g);
+        const long tiles = (long)g.tilesA * g.tilesB * batch;
+        const int rc = clt_internal_gemm8_large(g, a_format, b_format, c_dtype, (int)plan.large, st);
+        if (rc != CLT_OK) return rc;
+        if (g.part) return c_dtype == CLT_DT_F32 ? fold<CLT_DT_F32>(g, st) : c_dtype == CLT_DT_BF16 ? fold<CLT_DT_BF16>(g, st) : fold<CLT_DT_F16>(g, st);
+        if (plan.large == tiles) return CLT_OK;
+        g.first = (int)plan.large;
+        blocks = 4 * (tiles - plan.large);
     }
-    const long blocks = (long)g.tilesA * g.tilesB * batch * g.slices;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
     return c_dtype == CLT_DT_F32 ? launch<CLT_DT_F32>(g, a_format, b_format, blocks, st)
            : c_dtype == CLT_DT_BF16 ? launch<CLT_DT_BF16>(g, a_format, b_format, blocks, st)

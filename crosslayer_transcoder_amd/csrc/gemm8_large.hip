@@ -44,26 +44,6 @@ typedef b8_u32x4_u u32x4_u;
 typedef b8_f32x4_u f32x4_u;
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int GA = 4;                                 // A tiles of a panel
-struct Tile { int batch, slice, a0, b0; };
-// block -> tile: every XCD (block index mod 8) works on a contiguous range of tiles, walked in panels of 4 A tiles with the A tile
-// fastest, so that the blocks an XCD runs together share operand tiles in its L2
-__device__ __forceinline__ Tile decode_tile(const Gemm8Args& g, int vb) {
-    const int nwg = g.tilesA * g.tilesB;
-    Tile t;
-    t.batch = fast_div(vb, nwg, g.inv_tiles);
-    int lid = vb - t.batch * nwg;
-    t.slice = 0;
-    if (g.slices > 1) { t.slice = t.batch / g.slices; t.slice = t.batch - t.slice * g.slices; t.batch = (t.batch - t.slice) / g.slices; }
-    const int xcd = lid & 7, q = nwg >> 3, r = nwg & 7;
-    lid = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (lid >> 3);
-    const int full = g.tilesA / GA, rem = g.tilesA - full * GA, per = GA * g.tilesB;
-    int ta, tb;
-    if (lid < full * per) { const int pn = fast_div(lid, per, g.inv_panel), x = lid - pn * per; tb = x / GA; ta = pn * GA + (x - tb * GA); }
-    else { const int x = lid - full * per; tb = fast_div(x, rem, g.inv_rem); ta = full * GA + (x - tb * rem); }
-    t.a0 = ta * 256; t.b0 = tb * 256;
-    return t;
-}
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* p, long records) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)records, 0x00020000);
 }
@@ -73,7 +53,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wb = w >> 1, wa = w & 1, fr = lane & 15, fq = lane >> 4;
     const int nk = g.slice_kb;                            // blocks of k of a tile (K, or a slice of it)
-    auto decode = [&](int vb) { return decode_tile(g, vb); };
+    auto decode = [&](int vb) { return b8_tile(g, vb); };
 
     // ---- DMA: piece i of wave w fills LDS rows (4 i + w) * 8 .. + 7; a lane supplies 16 bytes (chunk XOR-swizzled with bits 1..3 of the
     // row).  Descriptors start at the tile's first row and end behind its last one: rows past the matrix arrive as zeros.
@@ -82,7 +62,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     const int vA = (q8 * 8 + (w >> 1)) * (int)g.lda + ch * 16;
     const int vB = ((((q8 & 3) << 2) | (q8 >> 2)) * 8 + (w >> 1)) * (int)g.ldb + ch * 16;
     __amdgpu_buffer_rsrc_t rA, rB, rS, rBias;
-    auto aim = [&](const Tile& t) {
+    auto aim = [&](const B8Tile& t) {
         // (a slice of K starts slice_kb blocks into the rows: the range ends where the last row does)
         const long k0 = (long)t.slice * g.slice_kb;
         rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda + k0 * 128, (long)min(g.M - t.a0, 256) * g.lda - k0 * 128);
@@ -118,8 +98,8 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
 
     // ---- the stream of k-blocks: staging runs two blocks ahead of the products, across tiles
     int vb = blockIdx.x, svb = vb, skt = 0, sslot = 0, slot = 0, buf = 0;
-    Tile t = decode(vb);
-    auto enter = [&](const Tile& e) {                     // staging enters tile svb = e
+    B8Tile t = decode(vb);
+    auto enter = [&](const B8Tile& e) {                     // staging enters tile svb = e
         if (svb < total) {
             aim(e);
             if (g.bias && w == 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(rBias, (lds_void*)(g8_smem + BIAS_BASE + sslot * 1024), 16, lane * 16, 0, 0, 0);
@@ -127,7 +107,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     };
     // (moved on at the head of a block, where the staging state is needed: control flow behind the matrix instructions would let the
     // compiler sink them, which have no side effects, below everything they are meant to overlap)
-    auto advance = [&](const Tile& next) {
+    auto advance = [&](const B8Tile& next) {
         if (++skt == nk) { skt = 0; svb += (int)gridDim.x; sslot = (sslot + 1) & 3; enter(next); }
     };
     enter(t);
@@ -137,7 +117,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
 #pragma unroll
         for (int i = 0; i < 8; ++i) piece(k, skt, i);
     }
-    Tile nt = decode(svb + (int)gridDim.x);               // the tile staging enters next (decoded off the critical path)
+    B8Tile nt = decode(svb + (int)gridDim.x);               // the tile staging enters next (decoded off the critical path)
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     // Buffer handover: this wave's reads of the block are complete and its pieces of the next block have landed; then all waves'.
     // Vector memory retires in order: in a tile's first block the next block's pieces are older than the previous tile's stores,
@@ -194,7 +174,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
             sa = sa_n; sb = sb_n;
             buf ^= 1;
         }
-        const Tile cur = t;
+        const B8Tile cur = t;
         const int cslot = slot;
         vb += (int)gridDim.x;
         slot = (slot + 1) & 3;
@@ -283,7 +263,7 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
     const int srow = (int)(w & 1 ? g.ldbs : g.ldas);
     __amdgpu_buffer_rsrc_t rA, rB, rS;
     int vb = blockIdx.x, svb = vb, skt = 0, sslot = 0, slot = 0, buf = 0;
-    auto enter = [&](const Tile& t) {
+    auto enter = [&](const B8Tile& t) {
         if (svb < total) {
             const long k0 = (long)t.slice * g.slice_kb;
             rA = rsrc(g.a + t.batch * g.ba + (long)t.a0 * g.lda + k0 * 128, (long)min(g.M - t.a0, 256) * g.lda - k0 * 128);
@@ -296,7 +276,7 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
             }
         } else { rA = rsrc(g.a, 0); rB = rsrc(g.b, 0); rS = rsrc(g.as, 0); }
     };
-    auto advance = [&](const Tile& next) {
+    auto advance = [&](const B8Tile& next) {
         if (++skt == nk) { skt = 0; svb += (int)gridDim.x; sslot = (sslot + 1) & 3; enter(next); }
     };
     auto piece = [&](int b, int kt, int i) {
@@ -313,15 +293,15 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int NST = 32;                               // stores of an interior tile per lane
-    Tile t = decode_tile(g, vb);
+    B8Tile t = b8_tile(g, vb);
     enter(t);
     for (int k = 0; k < 2; ++k) {
-        if (k) advance(decode_tile(g, svb + (int)gridDim.x));
+        if (k) advance(b8_tile(g, svb + (int)gridDim.x));
         scale_piece(k, skt);
 #pragma unroll
         for (int i = 0; i < 4; ++i) piece(k, skt, i);
     }
-    Tile nt = decode_tile(g, svb + (int)gridDim.x);
+    B8Tile nt = b8_tile(g, svb + (int)gridDim.x);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     auto handover = [](int kt) {
         asm volatile("s_cmp_eq_u32 %0, 0\n\ts_cbranch_scc1 1f\n\ts_waitcnt vmcnt(0)\n1:\ts_waitcnt vmcnt(%1) lgkmcnt(0)\n\ts_barrier" ::"s"(kt), "i"(NST) : "scc", "memory");
@@ -377,13 +357,13 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
                 for (int n = 0; n < 4; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb, ha[n], acc[m][n], 0, 0, 0);
             });
         }
-        const Tile cur = t;
+        const B8Tile cur = t;
         const int cslot = slot;
         vb += (int)gridDim.x;
         slot = (slot + 1) & 3;
         const bool more = vb < total;
-        if (more) t = decode_tile(g, vb);
-        nt = decode_tile(g, svb + (int)gridDim.x);
+        if (more) t = b8_tile(g, vb);
+        nt = b8_tile(g, svb + (int)gridDim.x);
         // ---- results: for (n, i) a lane has row 4 fr + n of its 64 and eight columns 8 (4 i + fq) .. of its 128
         const int r0 = wa * 64 + fr * 4, c0 = wb * 128 + fq * 8;
         const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N;
@@ -436,20 +416,17 @@ template <int FA, int FB> int launch_dtype(const Gemm8Args& g, int dtype, bool f
 }
 }  // namespace
 
-// dtype: of the product asked for (it picks the instructions); g.part: partial sums go there, unfolded
-int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, hipStream_t st) {
+// dtype: of the product asked for (it picks the instructions); g.part: partial sums go there, unfolded; tiles: the first ones in the order
+// of b8_tile (slices: all)
+int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, int tiles, hipStream_t st) {
     Gemm8Args g = g0;
     const bool fast = dtype != CLT_DT_F32;
-    g.tilesA = (g.M - 1) / 256 + 1; g.tilesB = (g.N - 1) / 256 + 1;
     if (g.part) {
         g.c = g.part; g.ldc = g.N; g.bc = (long)g.M * g.N; g.slice_stride = g.batch * g.bc;
         g.bias = nullptr; g.accumulate = 0;
         dtype = CLT_DT_F32;
     }
-    const int total = g.tilesA * g.tilesB * g.batch * g.slices, rem = g.tilesA % GA;
-    g.inv_tiles = 0xffffffffu / (uint32_t)(g.tilesA * g.tilesB);
-    g.inv_panel = 0xffffffffu / (uint32_t)(GA * g.tilesB);
-    g.inv_rem = rem ? 0xffffffffu / (uint32_t)rem : 0u;
+    const int total = tiles * g.slices;
     return fa == 0 ? (fb == 0 ? launch_dtype<0, 0>(g, dtype, fast, total, st) : launch_dtype<0, 1>(g, dtype, fast, total, st))
                    : (fb == 0 ? launch_dtype<1, 0>(g, dtype, fast, total, st) : launch_dtype<1, 1>(g, dtype, fast, total, st));
 }
