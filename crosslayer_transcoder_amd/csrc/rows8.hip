@@ -7,8 +7,8 @@
 // four steps ahead in registers; the first steps are requested before x is packed.  Tokens ride the matrix instruction's "N"
 // index (16 of them, repeated where there are fewer), weight rows its "M" index.  Where rows alone give too few blocks, K is cut
 // into slices whose partial sums a second launch adds in order.
-// Measured: 768 -> 32768, 1 token 7.1 us (an empty launch: 3.3); 12 layers of it, 302 MB of weights: 57 us = 5.3 TB/s (1 token), 80 us
-// (32 tokens); 393216 -> 768, 1 token: 73 us = 4.1 TB/s with the second launch.
+// Measured: 768 -> 32768, 1 token 7.1 us (an empty launch: 3.3); 12 layers of it, 302 MB of weights: 57 us = 5.3 TB/s (1 token), 74 us
+// (32 tokens); 393216 -> 768, 1 token: 54 us = 5.6 TB/s with the second launch; 4096 -> 4096: 9.3 us; 8192 -> 768: 7.9 us.
 #include "block8_common.h"
 
 namespace {
@@ -17,7 +17,7 @@ typedef b8_bf16x8 bf16x8;
 constexpr int WAVES = 8, MAX_T = 32;
 constexpr int LDS_CAP = 136 * 1024;                  // packed slice of x at most
 // (64 tokens: packing and the tiled product are as fast or faster, 129 against 138 us for 768 -> 32768 x 12 layers, 47 against 101 for
-// 4096 -> 32768; 32 tokens: 121 against 81 and 24 against 26 for 32768 -> 768)
+// 4096 -> 32768; 32 tokens: 121 against 74)
 
 struct Rows8Args {
     const void* x; long x_token, x_layer;            // strides in elements
@@ -206,29 +206,34 @@ __global__ __launch_bounds__(256) void rows8_fold_kernel(Rows8Args a, long n) {
     store_result(a.y, a.y_dtype, t * a.y_token + layer * a.y_layer + c, f32x4{s, 0.0f, 0.0f, 0.0f}, 1, false);
 }
 
-// How the work is cut: blocks of K per slice, slices, row groups in a wave's hand (G), chunks of rows per block.  Rows first (no
-// partial sums); K is cut where the packed x does not fit LDS or where rows give less than two blocks a CU, down to 16 blocks of
-// k a slice (the second launch costs about as much as a wave's 16 steps).  G grows while every CU keeps two blocks (x is read from
-// LDS once for G row groups); what is left over becomes chunks, so that x is packed once per resident block.
+// How the work is cut: blocks of K per slice, slices, row groups in a wave's hand (G), chunks of rows per block.
+// Slices: at least as many as the packed x needs to fit LDS; up to two blocks a CU the least of the times that these measurements add
+// up to, in units of one step (a block of k, 0.5 us with every CU at work): a pass of blocks over the CUs takes the slice's steps and 1.5
+// (1.3 times that where LDS holds one block of 32 tokens a CU: nothing runs while it packs x), the second launch 6 and 0.3 a slice.
+// One token, 8192 -> 768 in 4 / 8 / 16 slices: 13.1 / 8.9 / 8.0 us; 4096 -> 4096 in 2 / 4 / 8: 13.6 / 10.7 / 9.3; 4096 -> 14336 in 2 / 4 (224 and
+// 448 blocks): 15.7 / 17.8; 1024 -> 1024 in 1 / 2: 6.5 / 7.6; 393216 -> 768 in 42 / 64 / 86 (252, 384 and 516 blocks): 53 / 61 / 57.
+// G grows while every CU keeps two blocks (x is read from LDS once for G row groups).  What is left over becomes chunks, so that x is
+// packed once per resident block: up to 16 tokens above 2048 blocks, above that (a longer packing) above two rounds of the blocks that
+// fit: 12 x (768 -> 32768), 32 tokens: 77 / 72 us in 1536 / 768 blocks, one token 47 / 49; 4096 -> 32768, 32 tokens: 64 / 45 in 512 / 256.
 struct Cut { int slice_kb, slices, g, chunks, row_blocks; };
 Cut cut_rows8(int T, int L, int N, int KB) {
     Cut c;
     const int fit = (LDS_CAP / T - 16) / 256;                            // blocks of k whose x fits LDS (>= 16 for 32 tokens)
     const long rb = (N + WAVES * 16 - 1) / (WAVES * 16), want = 512;
-    long slices = (KB + fit - 1) / fit;
-    if (L * rb * slices < want) {
-        const long by_grid = (want + L * rb - 1) / (L * rb), most = KB / 16 > 0 ? KB / 16 : 1;
-        const long s = by_grid < most ? by_grid : most;
-        if (s > slices) slices = s;
+    auto alone = [&](int slice_kb) { return (long)T * (slice_kb * 256 + 16) > 80 * 1024; };      // one block a CU
+    long least = -1;
+    const long need = (KB + fit - 1) / fit;
+    for (long s = need; s == need || (s * 4 <= KB && L * rb * s <= want); ++s) {
+        const int per = (int)((KB + s - 1) / s), used = (KB + per - 1) / per;
+        const long pass = (L * rb * used + 255) / 256 * (10L * per + 15), t = (alone(per) ? pass * 13 / 10 : pass) + (used > 1 ? 60 + 3 * used : 0);
+        if (least < 0 || t < least) { least = t; c.slice_kb = per; c.slices = used; }
     }
-    c.slice_kb = (int)((KB + slices - 1) / slices);
-    c.slices = (KB + c.slice_kb - 1) / c.slice_kb;
     const long blocks = L * rb * c.slices;                               // at G = 1
     const int most_g = T <= 16 ? 2 : 1;                                  // (two row groups and 32 tokens: one block per CU instead of two, 87 against 80 us)
     c.g = 1;
     while (c.g < most_g && blocks >= 2 * c.g * want) c.g *= 2;
-    const long rows = (long)WAVES * 16 * c.g, per_layer = (N + rows - 1) / rows;
-    c.chunks = (int)(L * per_layer * c.slices / 2048) + 1;
+    const long rows = (long)WAVES * 16 * c.g, per_layer = (N + rows - 1) / rows, round = alone(c.slice_kb) ? 256 : 512;
+    c.chunks = (int)(L * per_layer * c.slices / (T > 16 ? 2 * round : 2048)) + 1;
     if (c.chunks > per_layer) c.chunks = (int)per_layer;
     c.row_blocks = (int)((per_layer + c.chunks - 1) / c.chunks);
     return c;
