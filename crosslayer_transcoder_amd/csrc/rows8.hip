@@ -194,20 +194,26 @@ __global__ __launch_bounds__(256) void rows8_fold_kernel(Rows8Args a, long n) {
     float s = 0.0f;
     const float* p = a.part + i;
     int k = 0;
-    for (; k + 8 <= a.slices; k += 8) {                                  // eight requests at a time, added in order
+    for (; k + 32 <= a.slices; k += 32) {                                // many requests at a time (few threads here), added in order
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = p[(k + j) * n];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s += v[j];
+    }
+    for (; k < a.slices; k += 8) {
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = p[(k + j) * n];
+        for (int j = 0; j < 8; ++j) v[j] = k + j < a.slices ? p[(k + j) * n] : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) s += v[j];
     }
-    for (; k < a.slices; ++k) s += p[k * n];
     if (a.bias) s += a.bias[layer * a.bbias + c];
     store_result(a.y, a.y_dtype, t * a.y_token + layer * a.y_layer + c, f32x4{s, 0.0f, 0.0f, 0.0f}, 1, false);
 }
 
 // How the work is cut: blocks of K per slice, slices, row groups in a wave's hand (G), chunks of rows per block.
-// Slices: at least as many as the packed x needs to fit LDS; up to two blocks a CU the least of the times that these measurements add
+// Slices: at least as many as the packed x needs to fit LDS; from there to two blocks a CU (or twice those slices) the least of the times that these measurements add
 // up to, in units of one step (a block of k, 0.5 us with every CU at work): a pass of blocks over the CUs takes the slice's steps and 1.5
 // (1.3 times that where LDS holds one block of 32 tokens a CU: nothing runs while it packs x), the second launch 6 and 0.3 a slice.
 // One token, 8192 -> 768 in 4 / 8 / 16 slices: 13.1 / 8.9 / 8.0 us; 4096 -> 4096 in 2 / 4 / 8: 13.6 / 10.7 / 9.3; 4096 -> 14336 in 2 / 4 (224 and
@@ -222,8 +228,8 @@ Cut cut_rows8(int T, int L, int N, int KB) {
     const long rb = (N + WAVES * 16 - 1) / (WAVES * 16), want = 512;
     auto alone = [&](int slice_kb) { return (long)T * (slice_kb * 256 + 16) > 80 * 1024; };      // one block a CU
     long least = -1;
-    const long need = (KB + fit - 1) / fit;
-    for (long s = need; s == need || (s * 4 <= KB && L * rb * s <= want); ++s) {
+    const long need = (KB + fit - 1) / fit, most = 2 * L * rb * need > want ? 2 * L * rb * need : want;
+    for (long s = need; s == need || (s * 4 <= KB && L * rb * s <= most); ++s) {
         const int per = (int)((KB + s - 1) / s), used = (KB + per - 1) / per;
         const long pass = (L * rb * used + 255) / 256 * (10L * per + 15), t = (alone(per) ? pass * 13 / 10 : pass) + (used > 1 ? 60 + 3 * used : 0);
         if (least < 0 || t < least) { least = t; c.slice_kb = per; c.slices = used; }
