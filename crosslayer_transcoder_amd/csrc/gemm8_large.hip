@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const f32x4 v = f32x4{acc[4 * j][n][i], acc[4 * j + 1][n][i], acc[4 * j + 2][n][i], acc[4 * j + 3][n][i]};
-                        if (interior) *reinterpret_cast<f32x4_u*>(p + 4 * j) = v;
+                        if (interior || (n < prow && i * 32 + 4 * j + 4 <= pcol)) *reinterpret_cast<f32x4_u*>(p + 4 * j) = v;
                         else if (n < prow)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) if (i * 32 + 4 * j + e < pcol) p[4 * j + e] = v[e];
@@ -229,7 +229,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
             for (int k = 0; k < 4; ++k) {                 // rows (4 k + fq) * 8 + n
                 const u32x4 u = v[k];
                 T* p = reinterpret_cast<T*>(reinterpret_cast<char*>(ctile + (long)(k * 32 + n) * g.ldc) + at);
-                if (interior) __builtin_nontemporal_store((u32x4_u)u, reinterpret_cast<u32x4_u*>(p));
+                if (interior || (k * 32 + n < rows && cols >= 8)) __builtin_nontemporal_store((u32x4_u)u, reinterpret_cast<u32x4_u*>(p));
                 else if (k * 32 + n < rows)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) if (j < cols) p[j] = (T)(u[j >> 1] >> (16 * (j & 1)));
@@ -380,12 +380,11 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
                 f32x4 hi = f32x4{acc[4][n][i], acc[5][n][i], acc[6][n][i], acc[7][n][i]};
                 if (has_bias) { lo += *reinterpret_cast<const f32x4*>(bl + i * 32); hi += *reinterpret_cast<const f32x4*>(bl + i * 32 + 4); }
                 float* p = reinterpret_cast<float*>(reinterpret_cast<char*>(ctile + (long)n * g.ldc + i * 32) + at);
-                if (interior) {
+                if (interior || (n < rows && i * 32 + 8 <= cols)) {
                     if (g.accumulate) { lo += *reinterpret_cast<const f32x4_u*>(p); hi += *reinterpret_cast<const f32x4_u*>(p + 4); }
                     *reinterpret_cast<f32x4_u*>(p) = lo;
                     *reinterpret_cast<f32x4_u*>(p + 4) = hi;
-                }
-                else if (n < rows)
+                } else if (n < rows)
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (i * 32 + j < cols) { const float v = j < 4 ? lo[j & 3] : hi[j & 3]; p[j] = g.accumulate ? p[j] + v : v; }
