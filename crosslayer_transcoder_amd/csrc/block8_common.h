@@ -147,18 +147,19 @@ inline void b8_tile_order(Gemm8Args& g) {
 }
 int clt_internal_gemm8_large(const Gemm8Args& g, int fa, int fb, int dtype, int tiles, hipStream_t st);      // gemm8_large.hip
 
-// Four consecutive columns of a row of C: one store where the row's alignment allows it (vec), else element by element
-template <int DT> __device__ __forceinline__ void b8_store4(void* c, long at, b8_f32x4 v, int valid, bool vec, int accumulate) {
+// Four consecutive columns of a row of C (`valid` of them): one store, aligned to the element only
+typedef uint32_t b8_u32x2_u __attribute__((ext_vector_type(2), aligned(2)));
+template <int DT> __device__ __forceinline__ void b8_store4(void* c, long at, b8_f32x4 v, int valid, int accumulate) {
     typename Elem<DT>::type* p = static_cast<typename Elem<DT>::type*>(c) + at;
     if constexpr (DT == CLT_DT_F32) {
-        if (vec && valid >= 4) {
-            b8_f32x4* q = reinterpret_cast<b8_f32x4*>(p);
+        if (valid >= 4) {
+            b8_f32x4_u* q = reinterpret_cast<b8_f32x4_u*>(p);
             *q = accumulate ? *q + v : v;
         } else
 #pragma unroll
             for (int i = 0; i < 4; ++i) if (i < valid) p[i] = accumulate ? p[i] + v[i] : v[i];
     } else {
-        if (vec && valid >= 4) *reinterpret_cast<uint2*>(p) = make_uint2(pack_out16<DT>(v[0], v[1]), pack_out16<DT>(v[2], v[3]));
+        if (valid >= 4) *reinterpret_cast<b8_u32x2_u*>(p) = b8_u32x2_u{pack_out16<DT>(v[0], v[1]), pack_out16<DT>(v[2], v[3])};
         else
 #pragma unroll
             for (int i = 0; i < 4; ++i) if (i < valid) p[i] = f32_to_elem<DT>(v[i]);

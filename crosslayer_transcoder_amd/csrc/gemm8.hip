@@ -13,6 +13,7 @@
 //
 // This file: the entry point and the form for everything that does not fill the chip with 256 x 256 tiles (gemm8_large.hip): 128 x 128
 // tiles, K cut into slices where tiles are few (partial sums in fp32, added in order by a second launch).
+#include <type_traits>
 #include "block8_common.h"
 
 namespace {
@@ -150,8 +151,6 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256, 1) void gemm
     // for (n, i) a lane has row 4 fr + n and four columns 4 (4 i + fq) ..
     const bool part = g.part != nullptr;
     const float* bias = g.bias && !part ? g.bias + batch * g.bbias : nullptr;
-    const int ldc_part = g.N;
-    const bool vec = part ? g.N % 4 == 0 : ((uintptr_t)g.c % (WIDE ? 16 : 8)) == 0 && g.ldc % 4 == 0 && g.bc % 4 == 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int col = b0 + wb * 64 + (i * 4 + fq) * 4, valid = g.N - col;
@@ -164,8 +163,8 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256, 1) void gemm
             const int row = a0 + wa * 64 + fr * 4 + n;
             if (row >= g.M || valid <= 0) continue;
             const f32x4 v = f32x4{acc[0][n][i], acc[1][n][i], acc[2][n][i], acc[3][n][i]} + bv;
-            if (part) b8_store4<CLT_DT_F32>(g.part, (((long)slice * g.batch + batch) * g.M + row) * ldc_part + col, v, valid, vec, 0);
-            else b8_store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, v, valid, vec, g.accumulate);
+            if (part) b8_store4<CLT_DT_F32>(g.part, (((long)slice * g.batch + batch) * g.M + row) * g.N + col, v, valid, 0);
+            else b8_store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, v, valid, g.accumulate);
         }
     }
 }
@@ -179,25 +178,30 @@ template <int DT> __global__ __launch_bounds__(256) void gemm8_fold_kernel(Gemm8
     const long step = (long)g.batch * g.M * g.N;
     const float* p = g.part + r * g.N + col;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (valid >= 4 && g.N % 4 == 0) {
-        int k = 0;
-        for (; k + 4 <= g.slices; k += 4) {              // four requests at a time, added in order
-            f32x4 v[4];
+    // (a row's last columns: each element by itself, the ones past the end repeated and dropped)
+    const bool whole = valid >= 4;
+    const int c1 = min(1, valid - 1), c2 = min(2, valid - 1);
+    auto sum = [&](int k, auto n) {                      // n requests at a time, added in order
+        constexpr int R = decltype(n)::value;
+        f32x4 v[R];
+        if (whole) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4*>(p + (k + j) * step);
+            for (int j = 0; j < R; ++j) v[j] = *reinterpret_cast<const b8_f32x4_u*>(p + (k + j) * step);
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s += v[j];
+            for (int j = 0; j < R; ++j) { const float* q = p + (k + j) * step; v[j] = f32x4{q[0], q[c1], q[c2], 0.0f}; }
         }
-        for (; k < g.slices; ++k) s += *reinterpret_cast<const f32x4*>(p + k * step);
-    } else
-        for (int k = 0; k < g.slices; ++k)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) if (j < valid) s[j] += p[k * step + j];
+        for (int j = 0; j < R; ++j) s += v[j];
+    };
+    int k = 0;
+    for (; k + 8 <= g.slices; k += 8) sum(k, std::integral_constant<int, 8>{});
+    for (; k + 2 <= g.slices; k += 2) sum(k, std::integral_constant<int, 2>{});
+    if (k < g.slices) sum(k, std::integral_constant<int, 1>{});
     if (g.bias)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[j] += g.bias[batch * g.bbias + min(col + j, g.N - 1)];
-    const bool vec = ((uintptr_t)g.c % (DT == CLT_DT_F32 ? 16 : 8)) == 0 && g.ldc % 4 == 0 && g.bc % 4 == 0;
-    b8_store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, s, valid, vec, g.accumulate);
+    b8_store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, s, valid, g.accumulate);
 }
 
 // Which tiles, and into how many slices K is cut: the least of the times that these measurements add up to (us; a pass is one tile on

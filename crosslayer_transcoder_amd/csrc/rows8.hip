@@ -26,29 +26,16 @@ struct Rows8Args {
     void* y; long y_token, y_layer; int y_dtype;     // results, or
     float* part;                                     // partial sums [slice][layer][token][N] when K is cut
     int T, N, K, KB, slice_kb, slices, chunks, row_blocks, layers;
-    int x_dtype, y_vec;
+    int x_dtype;
 };
 
 extern __shared__ __attribute__((aligned(16))) unsigned char r8_smem[];
 
-// `valid` of four consecutive results; whole: one store (valid >= 4 and the row's alignment allows it)
-__device__ __forceinline__ void store_result(void* y, int dtype, long at, f32x4 v, int valid, bool whole) {
-    if (dtype == CLT_DT_F32) {
-        float* p = static_cast<float*>(y) + at;
-        if (whole) *reinterpret_cast<f32x4*>(p) = v;
-        else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if (i < valid) p[i] = v[i];
-    } else {
-        uint16_t* p = static_cast<uint16_t*>(y) + at;
-        const bool bf = dtype == CLT_DT_BF16;
-        const uint2 u = bf ? make_uint2(pack_out16<CLT_DT_BF16>(v[0], v[1]), pack_out16<CLT_DT_BF16>(v[2], v[3]))
-                           : make_uint2(pack_out16<CLT_DT_F16>(v[0], v[1]), pack_out16<CLT_DT_F16>(v[2], v[3]));
-        if (whole) *reinterpret_cast<uint2*>(p) = u;
-        else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if (i < valid) p[i] = (uint16_t)((i < 2 ? u.x : u.y) >> (16 * (i & 1)));
-    }
+// `valid` of four consecutive results
+__device__ __forceinline__ void store_result(void* y, int dtype, long at, f32x4 v, int valid) {
+    if (dtype == CLT_DT_F32) b8_store4<CLT_DT_F32>(y, at, v, valid, 0);
+    else if (dtype == CLT_DT_BF16) b8_store4<CLT_DT_BF16>(y, at, v, valid, 0);
+    else b8_store4<CLT_DT_F16>(y, at, v, valid, 0);
 }
 
 // MT: groups of 16 tokens; G: groups of 16 weight rows a wave has in hand; FMT: format of the weights.  A step is G x 16 rows x 128 k;
@@ -178,8 +165,8 @@ template <int MT, int G, int FMT> __global__ __launch_bounds__(WAVES * 64, 4) vo
             for (int t = 0; t < MT; ++t) {
                 const int tok = t * 16 + fr;
                 if (tok >= a.T) continue;
-                if (a.part) store_result(a.part, CLT_DT_F32, (((long)slice * a.layers + layer) * a.T + tok) * a.N + n, acc[g][t], valid, valid >= 4 && a.N % 4 == 0);
-                else store_result(a.y, a.y_dtype, tok * a.y_token + layer * a.y_layer + n, acc[g][t] + bv[g], valid, valid >= 4 && a.y_vec);
+                if (a.part) store_result(a.part, CLT_DT_F32, (((long)slice * a.layers + layer) * a.T + tok) * a.N + n, acc[g][t], valid);
+                else store_result(a.y, a.y_dtype, tok * a.y_token + layer * a.y_layer + n, acc[g][t] + bv[g], valid);
             }
         }
     }
@@ -209,7 +196,7 @@ __global__ __launch_bounds__(256) void rows8_fold_kernel(Rows8Args a, long n) {
         for (int j = 0; j < 8; ++j) s += v[j];
     }
     if (a.bias) s += a.bias[layer * a.bbias + c];
-    store_result(a.y, a.y_dtype, t * a.y_token + layer * a.y_layer + c, f32x4{s, 0.0f, 0.0f, 0.0f}, 1, false);
+    store_result(a.y, a.y_dtype, t * a.y_token + layer * a.y_layer + c, f32x4{s, 0.0f, 0.0f, 0.0f}, 1);
 }
 
 // How the work is cut: blocks of K per slice, slices, row groups in a wave's hand (G), chunks of rows per block.
@@ -280,7 +267,6 @@ extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride,
     a.y = y; a.y_token = y_token_stride; a.y_layer = y_layer_stride; a.y_dtype = y_dtype;
     a.part = c.slices > 1 ? static_cast<float*>(workspace) : nullptr;
     a.T = tokens; a.N = N; a.K = K; a.KB = KB; a.slice_kb = c.slice_kb; a.slices = c.slices; a.chunks = c.chunks; a.row_blocks = c.row_blocks; a.layers = layers;
-    a.y_vec = (uintptr_t)y % (4 * ys) == 0 && y_token_stride % 4 == 0 && y_layer_stride % 4 == 0;
     const long blocks = (long)layers * c.slices * c.row_blocks;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
     const int lds = tokens * (c.slice_kb * 256 + 16);
