@@ -290,6 +290,19 @@ def linear8(x: torch.Tensor, w: Block8, bias: Optional[torch.Tensor] = None, out
                   FORMATS[w.fmt], w.data.stride(1), w.scale.stride(1), w.data.stride(0), w.scale.stride(0),
                   bias.data_ptr() if bias is not None else None, N, y.data_ptr(), _DT[dt], L * N, N, T, L, N, K,
                   ws.data_ptr() if nws else None, nws, _stream(x.device))
+    elif T and K and N and L:                               # quantize8 and gemm8 on one buffer (a third of their host time)
+        bias = _bias(bias, L, N, x.device)
+        k, t = _up(K), _up(T)
+        nws = lib.clt_gemm8_workspace_bytes(T, N, K, L)
+        tmp = torch.empty(L * (T * k + k // BLOCK * t) + nws, dtype=torch.uint8, device=x.device)
+        q = tmp.data_ptr()
+        s = q + L * T * k
+        with _on(x.device):
+            st = _stream(x.device)
+            _call(lib.clt_pack8, x.data_ptr(), _DT[x.dtype], x.stride(0), x.stride(1), L, T, K, 0, 0, q, s, None, None, None, None, 0, st)
+            _call(lib.clt_gemm8, q, s, 0, k, t, T * k, k // BLOCK * t, w.data.data_ptr(), w.scale.data_ptr(), FORMATS[w.fmt], w.data.stride(1),
+                  w.scale.stride(1), w.data.stride(0), w.scale.stride(0), y.data_ptr(), _DT[dt], L * N, N,
+                  bias.data_ptr() if bias is not None else None, N, T, N, K, L, 0, s + L * (k // BLOCK) * t if nws else None, nws, st)
     else:
         gemm8(quantize8(x.transpose(0, 1)), w, bias, out=y.transpose(0, 1))
     return y.squeeze(1) if two else y
