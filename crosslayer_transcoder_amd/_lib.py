@@ -115,6 +115,11 @@ SIGNATURES = {
     "clt_gemm8": (I, [P, P, I, L, L, L, L, P, P, I, L, L, L, L, P, I, L, L, P, L, I, I, I, I, I, P, SZ, P]),
     "clt_linear8_rows_workspace_bytes": (SZ, [I, I, I, I]),
     "clt_linear8_rows": (I, [P, I, L, L, P, P, I, L, L, L, L, P, L, P, I, L, L, I, I, I, I, P, SZ, P]),
+    "clt_linear8_kept_bytes": (SZ, [I, I, I, I, I, I]),
+    "clt_linear8_forward_workspace_bytes": (SZ, [I, I, I, I]),
+    "clt_linear8_forward": (I, [P, I, L, L, P, I, L, L, I, P, P, I, I, I, I, I, I, P, P, SZ, P]),
+    "clt_linear8_backward_workspace_bytes": (SZ, [I, I, I, I, I, I, I]),
+    "clt_linear8_backward": (I, [P, I, L, L, P, I, I, I, I, I, I, P, P, I, P, P, SZ, P]),
 }
 
 ABI_VERSION = 21

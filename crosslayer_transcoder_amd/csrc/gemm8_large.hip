@@ -6,8 +6,8 @@
 // reads for 64 matrix instructions of 32 cycles; four waves read 128 KB in those 2048 cycles, half of the LDS's rate, where 8
 // waves of 128 x 64 would need three quarters and wait for it.
 // Operands go global -> LDS by DMA, two buffers of 64 KB, one 128-byte block of k at a time; the scale bytes of the block (256 + 256)
-// and the tile's bias ride along.  The grid is persistent; nothing of the epilogue passes through LDS, so both buffers
-// already receive the next tile's first two blocks while this tile's results are stored.
+// and the tile's bias ride along.  The grid is persistent; the epilogue's LDS is its own, so both buffers already receive the
+// next tile's first two blocks while this tile's results are stored.
 //
 // Row order.  LDS row p of a 128-row half holds matrix row (p % 16) * 8 + p / 16 (A) or c(p % 16) * 8 + p / 16 with
 // c(4 q + i) = 4 i + q (B), so fragment j of a wave is rows 8 * lane + j: (a) the scale bytes of a lane's eight fragments are eight
@@ -16,6 +16,9 @@
 // lanes make 64 / 128 consecutive bytes.  16-bit results pass through a 4 KB slab of LDS a wave, so that 256 bytes of a row leave
 // together, and past the caches, which hold the operands' panels (4096 x 768 x 32768 x 12: 1728 -> 1462 us; without the slab the
 // uncached stores are slower than cached ones, 1765 us).
+// Bound: the matrix units, at what clock the power leaves them (8192^3: 390 .. 437 us over boxes = 2.5 .. 2.8 PFLOP/s; the large library
+// product in 8 bits 2.9); with a short contraction the stores next to them (K = 768, 12 layers, 3.2 GB of results: 1430 us; 1600 us where
+// the rows of a layer lie 786 KB apart).
 #include <type_traits>
 #include "block8_common.h"
 
@@ -250,7 +253,7 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
 // ---- 32-bit results: the codes become bf16 in registers and the products run at the 16-bit rate, so a block of k costs twice the
 // cycles for the same LDS bytes: 8 waves of 128 x 64 (B x A; 192 KB of reads in 4096 cycles), two per SIMD, whose conversions run
 // under each other's matrix instructions.  Tiles, DMA, row order and the stream of blocks as above; A fragments are 4 rows of a
-// 64-row group (row 4 * lane + n).
+// 64-row group (row 4 * lane + n).  8192^3: 795 .. 825 us = 1.33 .. 1.38 PFLOP/s, the rate of the large library product in bf16 (1.32).
 template <int FA, int FB>
 __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, int total) {
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);

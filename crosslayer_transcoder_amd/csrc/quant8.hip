@@ -8,6 +8,9 @@
 // over 4 lanes and, through LDS, 4 waves.  8 x 8 patches because both forms then leave in 8-byte pieces without repacking: a
 // patch row is 8 row-major codes, a patch column 8 transposed ones (these pass through a 16 KB LDS tile to go out as whole
 // 128-byte lines).
+// Measured: 4096 x 12 x 768 bf16, both forms 32 us = 4.7 TB/s (a large copy: 4.75); 4096 x 4 x 32768 bf16, both forms 492 us = 4.4;
+// 12 x 32768 x 768 fp32 weights, one form 280 us = 5.4; 4096 x 12 x 32768 bf16, transposed form and column sums 1310 us = 3.7 (rows of a
+// tile 786 KB apart; other tile orders and uncached stores: 1260 .. 1330); restoring 4096 x 4 x 32768 to bf16 305 us = 5.3.
 #include "block8_common.h"
 
 namespace {

@@ -23,15 +23,15 @@ _DEV = "cuda"
 _E4M3 = ops8.FORMATS["e4m3"]
 
 
-# Bytes of the held forms.  The kept buffer is one allocation: x transposed (codes [L, K, up(T)], scale bytes [L, up(T) / 128, up(K)]),
-# then W for the input gradient (codes [L, K, up(N)], scale bytes [L, up(N) / 128, up(K)]), either part only where it is kept.
-def _held(L, rows, cols):
-    c = _up(cols)
-    return L * rows * c, L * (c // 128) * _up(rows)
-
-
 def _kept_bytes(T, L, K, N, keep_x, keep_w):
-    return (sum(_held(L, K, T)) if keep_x else 0) + (sum(_held(L, K, N)) if keep_w else 0)
+    """clt_linear8_kept_bytes, of symbolic sizes too: codes and scale bytes of x [K, T] and of W [K, N]."""
+    def held(rows, cols):
+        return L * (rows * _up(cols) + _up(cols) // 128 * _up(rows))
+    return (held(K, T) if keep_x else 0) + (held(K, N) if keep_w else 0)
+
+
+def _bytes(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _forward(x, W, b, kn, keep_x, keep_w):
@@ -46,44 +46,13 @@ def _forward(x, W, b, kn, keep_x, keep_w):
         raise ValueError(f"empty map: x {tuple(x.shape)}, W {tuple(W.shape)}")
     b = ops8._bias(b, L, N, dev)
     y = torch.empty((T, L, N), dtype=x.dtype, device=dev)
-    kept = torch.empty(_kept_bytes(T, L, K, N, keep_x, keep_w), dtype=torch.uint8, device=dev)
-    if not T and not keep_w:
-        return y, kept
-    (nq, ns), (nf, nfs) = _held(L, T, K), _held(L, N, K)
-    tmp = torch.empty(nq + ns + nf + nfs, dtype=torch.uint8, device=dev)
-    q = tmp.data_ptr()
-    s, f = q + nq, q + nq + ns
-    fs = f + nf
-    xt = wk = xs = ws = None
-    at = kept.data_ptr()
-    if keep_x:
-        n, ns_ = _held(L, K, T)
-        xt, xs = at, at + n
-        at += n + ns_
-    if keep_w:
-        wk, ws = at, at + _held(L, K, N)[0]
-    # the contraction over K reads the [N, K] form, the input gradient the [K, N] form
-    d, ds, t, ts = (wk, ws, f, fs) if kn else (f, fs, wk, ws)
+    kept = _bytes(lib.clt_linear8_kept_bytes(T, L, K, N, keep_x, keep_w), dev)
+    nws = lib.clt_linear8_forward_workspace_bytes(T, L, K, N)
+    ws = _bytes(nws, dev)
     with ops8._on(dev):
-        st = ops8._stream(dev)
-        R, C = W.shape[1:]
-        _call(lib.clt_pack8, W.data_ptr(), _DT[W.dtype], W.stride(1), W.stride(0), L, R, C, _E4M3, 1, d, ds, t, ts, None, None, 0, st)
-        if T:
-            _call(lib.clt_pack8, x.data_ptr(), _DT[x.dtype], x.stride(0), x.stride(1), L, T, K, _E4M3, 0, q, s, xt, xs, None, None, 0, st)
-            _gemm((q, s, L, T), (f, fs, L, N), K, y, L * N, N, b, N, st)
+        _call(lib.clt_linear8_forward, x.data_ptr(), _DT[x.dtype], x.stride(0), x.stride(1), W.data_ptr(), _DT[W.dtype], W.stride(1), W.stride(0), kn,
+              b.data_ptr() if b is not None else None, y.data_ptr(), T, L, K, N, keep_x, keep_w, kept.data_ptr(), ws.data_ptr(), nws, ops8._stream(dev))
     return y, kept
-
-
-def _gemm(a, b, K, out, ldc, cb, bias, nbias, st):
-    """clt_gemm8 of densely held e4m3 operands (codes, scale bytes, batch, rows) contracting over K."""
-    (aq, as_, L, M), (bq, bs, _, N) = a, b
-    k = _up(K)
-    sa, sb = _up(M), _up(N)
-    nws = lib.clt_gemm8_workspace_bytes(M, N, K, L)
-    ws = torch.empty(nws, dtype=torch.uint8, device=out.device) if nws else None
-    _call(lib.clt_gemm8, aq, as_, _E4M3, k, sa, M * k, k // 128 * sa, bq, bs, _E4M3, k, sb, N * k, k // 128 * sb, out.data_ptr(),
-          _DT[out.dtype], ldc, cb, bias.data_ptr() if bias is not None else None, nbias, M, N, K, L, 0,
-          ws.data_ptr() if nws else None, nws, st)
 
 
 def _gradients(dy, kept, K, kn, has_x, need_dx, w_dtype, need_db):
@@ -97,31 +66,13 @@ def _gradients(dy, kept, K, kn, has_x, need_dx, w_dtype, need_db):
     db = torch.empty((L, N), dtype=torch.float32, device=dev) if need_db else None
     if need_db and not T:
         db.zero_()
-    (nq, ns), (nt, nts) = _held(L, T, N), _held(L, N, T)
-    nws = lib.clt_pack8_sums_workspace_bytes(L, T, N) if need_db and T else 0
-    along = need_dx or not need_dw                     # (the bias gradient rides along with a pack; alone it still takes one)
-    tmp = torch.empty((nq + ns if along else 0) + (nt + nts if need_dw else 0) + nws, dtype=torch.uint8, device=dev)
-    at = tmp.data_ptr()
-    q = s = qt = qs = None
-    if along:
-        q, s = at, at + nq
-        at += nq + ns
-    if need_dw:
-        qt, qs = at, at + nt
-        at += nt + nts
-    xt = kept.data_ptr()
-    xs = xt + _held(L, K, T)[0]
-    wk = xt + (sum(_held(L, K, T)) if has_x else 0)
-    with ops8._on(dev):
-        st = ops8._stream(dev)
-        if T:
-            _call(lib.clt_pack8, dy.data_ptr(), _DT[dy.dtype], dy.stride(0), dy.stride(1), L, T, N, _E4M3, 0, q, s, qt, qs,
-                  db.data_ptr() if need_db else None, at if nws else None, nws, st)
-            if need_dx:
-                _gemm((q, s, L, T), (wk, wk + _held(L, K, N)[0], L, K), N, dx, L * K, K, None, 0, st)
-        if need_dw:
-            xk, gk = (xt, xs, L, K), (qt, qs, L, N)
-            _gemm(*((xk, gk) if kn else (gk, xk)), T, dW, dW.shape[2], dW.shape[1] * dW.shape[2], None, 0, st)
+    if need_dx or need_dw or need_db:
+        nws = lib.clt_linear8_backward_workspace_bytes(T, L, K, N, need_dx, need_dw, need_db)
+        ws = _bytes(nws, dev)
+        with ops8._on(dev):
+            _call(lib.clt_linear8_backward, dy.data_ptr(), _DT[dy.dtype], dy.stride(0), dy.stride(1), kept.data_ptr(), has_x, kn, T, L, K, N,
+                  dx.data_ptr() if need_dx else None, dW.data_ptr() if need_dw else None, _DT[w_dtype] if need_dw else 0,
+                  db.data_ptr() if need_db else None, ws.data_ptr(), nws, ops8._stream(dev))
     return dx, dW, db
 
 

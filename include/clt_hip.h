@@ -576,6 +576,22 @@ int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride, long x_lay
                      int y_dtype, long y_token_stride, long y_layer_stride, int tokens, int layers, int N, int K, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/* A linear map and its gradients, batched over layers: y[t][l][:] = x[t][l][:] * w[l] + bias[l] with x packed in e4m3 along K and w in
+ * e4m3 tiles; w is [N][K] a layer, kn != 0: [K][N] (strides in elements, unit last stride).  y [T][L][N] has x's type.  kept (16-byte
+ * aligned, clt_linear8_kept_bytes): x transposed in blocks of 128 tokens where keep_x, w for the input gradient where keep_w, for
+ * the backward call.  T = 0: no results. */
+size_t clt_linear8_kept_bytes(int T, int L, int K, int N, int keep_x, int keep_w);
+size_t clt_linear8_forward_workspace_bytes(int T, int L, int K, int N);
+int clt_linear8_forward(const void* x, int x_dtype, long x_token_stride, long x_layer_stride, const void* w, int w_dtype, long w_row_stride,
+                        long w_batch_stride, int kn, const float* bias, void* y, int T, int L, int K, int N, int keep_x, int keep_w,
+                        void* kept, void* workspace, size_t workspace_bytes, void* stream);
+/* dy [T][L][N] -> dx [T][L][K] (dy's type), dw (w's layout, dw_dtype), db fp32 [L][N]; NULL where not asked for.  kept: as the forward call
+ * wrote it, has_x its keep_x (dw needs keep_x, dx keep_w).  db = 0 for T = 0 is the caller's. */
+size_t clt_linear8_backward_workspace_bytes(int T, int L, int K, int N, int need_dx, int need_dw, int need_db);
+int clt_linear8_backward(const void* dy, int dtype, long token_stride, long layer_stride, const void* kept, int has_x, int kn, int T, int L,
+                         int K, int N, void* dx, void* dw, int dw_dtype, float* db, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

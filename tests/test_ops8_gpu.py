@@ -710,6 +710,18 @@ def test_refusals_of_the_library():
     assert [gemm(M=0), gemm(N=0), gemm(K=-1), gemm(batch=0), gemm(dt=3), gemm(dt=1, acc=1), gemm(lda=112), gemm(ldbs=3), gemm(ldc=3), gemm(fa=2), gemm(c=None), gemm(a=None)] == [-1] * 12
     assert [gemm(a=p + 8), gemm(lda=136), gemm(c=p + 2), gemm(bias=p + 1), gemm(ldas=130)] == [-4] * 5
     assert gemm(K=5000, lda=5120, ldb=5120) == -3 and gemm(lda=1 << 24) == -6
+    def fwd(x=p, dt=0, w=p, T=4, L=2, K=100, N=30, kx=1, kw=1, kept=p, ws=p, n=1 << 20):
+        return lib.clt_linear8_forward(x, dt, 200, 100, w, 0, 100, 3000, 0, None, p, T, L, K, N, kx, kw, kept, ws, n, None)
+
+    def bwd(dy=p, kept=p, T=4, N=30, dx=p, dw=p, db=p, ws=p, n=1 << 20):
+        return lib.clt_linear8_backward(dy, 0, 60, 30, kept, 1, 0, T, 2, 100, N, dx, dw, 0, db, ws, n, None)
+
+    assert [fwd(T=-1), fwd(L=0), fwd(K=0), fwd(N=0), fwd(x=p, w=None), fwd(dt=7, w=None)] == [-1] * 6
+    assert [fwd(kept=None), fwd(kept=p + 8), fwd(ws=None), fwd(ws=p + 4), fwd(n=100)] == [-3] * 5
+    assert fwd(T=0, kw=0) == 0                                                   # nothing to do
+    assert [bwd(T=-1), bwd(N=0), bwd(dx=None, dw=None, db=None), bwd(dy=None)] == [-1] * 4
+    assert [bwd(kept=None), bwd(ws=None), bwd(n=100)] == [-3] * 3
+    assert lib.clt_linear8_kept_bytes(4, 2, 100, 30, 1, 1) == 2 * (100 * 128 + 128) * 2 and lib.clt_linear8_kept_bytes(4, 2, 100, 30, 0, 0) == 0
     assert lib.clt_unpack8(p, p, 0, 1, 4, 100, 112, 128, 0, 0, p, 0, None) == -1
     assert lib.clt_unpack8(p, p, 0, 1, 4, 100, 136, 128, 0, 0, p, 0, None) == -4
 
