@@ -16,7 +16,7 @@
 // lanes make 64 / 128 consecutive bytes.  16-bit results pass through a 4 KB slab of LDS a wave, so that 256 bytes of a row leave
 // together, and past the caches, which hold the operands' panels (4096 x 768 x 32768 x 12: 1728 -> 1462 us; without the slab the
 // uncached stores are slower than cached ones, 1765 us).
-// Bound: the matrix units, at what clock the power leaves them (8192^3: 390 .. 437 us over boxes = 2.5 .. 2.8 PFLOP/s; the large library
+// Bound: the matrix units, at what clock the power leaves them (8192^3: 390 .. 437 us from card to card = 2.5 .. 2.8 PFLOP/s; the large library
 // product in 8 bits 2.9); with a short contraction the stores next to them (K = 768, 12 layers, 3.2 GB of results: 1430 us; 1600 us where
 // the rows of a layer lie 786 KB apart).
 #include <type_traits>

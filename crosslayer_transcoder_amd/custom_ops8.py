@@ -93,6 +93,11 @@ def _(x, W, b, kn, keep_x, keep_w):
 @torch.library.custom_op("clt_hip::linear8_bwd", mutates_args=(), device_types=_DEV)
 def linear8_bwd(dy: Tensor, kept: Tensor, K: int, kn: bool, has_x: bool, need_dx: bool, w_dtype: Optional[torch.dtype], need_db: bool) -> List[Tensor]:
     """-> [dx [T, L, K], dW (shape of W), db fp32 [L, N]], empty where not asked for (w_dtype None: no dW)."""
+    T, L, N = dy.shape
+    if kept.dtype != torch.uint8 or not kept.is_contiguous() or kept.device != dy.device or kept.numel() < _kept_bytes(T, L, K, N, has_x, need_dx):
+        raise ValueError("`kept` is not what linear8 kept for this gradient")
+    if w_dtype is not None and not has_x:
+        raise ValueError("the weights' gradient needs the input that linear8 keeps with keep_x")
     return [dy.new_empty(0) if t is None else t for t in _gradients(dy, kept, K, kn, has_x, need_dx, w_dtype, need_db)]
 
 

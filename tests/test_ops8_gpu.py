@@ -138,8 +138,8 @@ def values(q):
     return ops8.dequantize8(q).cpu().double()
 
 
-def check_product(y, a, b, bias=None, base=None):
-    """y [L, M, N] against the 64-bit product of the values held."""
+def check_product(y, a, b, bias=None, base=None, whole=2.0 ** -20):
+    """y [L, M, N] against the 64-bit product of the values held; whole: the tolerance of fp32 results' norm."""
     A, B = values(a), values(b)
     ref, mag = A @ B.mT, A.abs() @ B.abs().mT
     if bias is not None:
@@ -155,7 +155,7 @@ def check_product(y, a, b, bias=None, base=None):
     worst = float((d - bound).max())
     assert worst <= 0, worst
     # and as a whole: the alignment loss of normal data is about 2^-16, the rounding at most eps / 2 a value
-    tol = 2.0 ** -20 if y.dtype == torch.float32 else torch.finfo(y.dtype).eps / 2 + 2.0 ** -12
+    tol = whole if y.dtype == torch.float32 else torch.finfo(y.dtype).eps / 2 + 2.0 ** -12
     assert float(d.norm()) <= tol * float(ref.norm()) + 1e-30
 
 
@@ -503,6 +503,95 @@ def test_two_streams_at_once():
                 got[i].append(ops8.linear8(xs[i], ws[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(y, ref[i]) for i in range(2) for y in got[i])
+
+
+@gpu
+def test_captured_products_equal_eager_on_every_replay():
+    """One graph with the few-token form and products whose K is cut (their workspaces share the graph's pool), replayed on changed inputs
+    with eager calls of the same functions in between."""
+    from crosslayer_transcoder_amd import ops8
+    w, v = ops8.quantize8_weights(rnd(1, 70, 9000, seed=1, spread=False)), ops8.quantize8_weights(rnd(1, 1900, 20480, seed=2, spread=False))
+    xs = [rnd(1, 9000, seed=10, spread=False), rnd(100, 9000, seed=11, spread=False), rnd(800, 20480, seed=12, dtype=torch.bfloat16, spread=False)]
+
+    def calls():
+        return [ops8.linear8(xs[0], w), ops8.linear8(xs[1], w), ops8.linear8(xs[2], v)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = calls()
+    for k in range(4):
+        for i, x in enumerate(xs):
+            x.copy_(rnd(*x.shape, seed=20 + 3 * k + i, dtype=x.dtype, spread=False))
+        expected = [y.clone() for y in calls()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, expected)), k
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """More than 2^31 elements in the input, the codes, the results and the weights: the last rows and columns."""
+    from crosslayer_transcoder_amd import ops8
+    R, C, last = 66000, 33000, 66000 // 128 * 128                                   # (last: first row of the last, partial block)
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.empty(R, C, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    q, t = ops8.quantize8_both(x)
+    a, b = ops8.quantize8_both(x[last:])
+    assert torch.equal(q.data[:, last:], a.data) and torch.equal(t.data[:, :, last:], b.data) and torch.equal(t.scale[:, -1], b.scale[:, -1])
+    assert torch.equal(q.scale[:, :, last:R], a.scale[:, :, :R - last])
+    assert same(ops8.dequantize8(q, torch.bfloat16)[:, last:], ops8.dequantize8(a, torch.bfloat16))
+    del x, t, b
+    m, n = q.first_columns(256), ops8.quantize8(rnd(1, C, 256, seed=1, spread=False))
+    tail = ops8.Block8(n.data[:, C - 300:], n.scale[:, :, C - 300:], 300, 256)
+    for dtype in (torch.bfloat16, torch.float32):
+        y = ops8.gemm8(m, n, out_dtype=dtype)
+        check_product(y[:, last:, C - 300:], a.first_columns(256), tail)
+        del y
+    del q, m
+    K, N = 131072, 33000
+    w = ops8.Block8(torch.randint(0, 100, (1, N, K), dtype=torch.uint8, device="cuda", generator=gen), torch.full((1, K // 128, N), 120, dtype=torch.uint8, device="cuda"), N, K)
+    end = ops8.Block8(w.data[:, N - 64:], w.scale[:, :, N - 64:], 64, K)
+    for T in (1, 40):
+        v = rnd(T, K, seed=3, spread=False)
+        # K additions one after another, each off by at most 2^-23 of the sum so far; sums of terms of random sign grow as sqrt(j / K) of
+        # the last one, and errors of random sign add by squares: 2^-23 sqrt(sum_j j / K) = 2^-23 sqrt(K / 2) of the result's norm
+        check_product(ops8.linear8(v, w)[None, :, N - 64:], ops8.quantize8(v), end, whole=2.0 ** -23 * math.sqrt(K / 2))
+
+
+@gpu
+def test_broadcast_inputs():
+    """Tensors expanded over tokens or layers (strides of zero), as inputs and as gradients."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    from crosslayer_transcoder_amd import ops8
+    x, W = rnd(1, 1, 300, seed=1, spread=False).expand(140, 2, 300), rnd(2, 300, 70, seed=2, spread=False)
+    q, t = ops8.quantize8_both(x.transpose(0, 1))
+    a, b = ops8.quantize8_both(x.transpose(0, 1).contiguous())
+    assert torch.equal(q.data, a.data) and torch.equal(t.data, b.data) and torch.equal(t.scale, b.scale)
+    w = ops8.quantize8_weights(W, transposed=True)
+    assert same(ops8.linear8(x, w), ops8.linear8(x.contiguous(), w)) and same(ops8.linear8(x[:3], w), ops8.linear8(x[:3].contiguous(), w))
+    leaves = [x.contiguous().requires_grad_(), W.clone().requires_grad_()]
+    for dy in (torch.ones((), device="cuda").expand(140, 2, 70), rnd(1, 1, 70, seed=3, spread=False).expand(140, 2, 70), rnd(140, 1, 70, seed=4, spread=False).expand(140, 2, 70)):
+        got = torch.autograd.grad(C.plt_decoder8(*leaves, None), leaves, dy)
+        want = torch.autograd.grad(C.plt_decoder8(*leaves, None), leaves, dy.contiguous())
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+@gpu
+def test_kept_bytes_that_do_not_fit_are_refused():
+    x, W, dy = rnd(9, 2, 40, seed=1, spread=False), rnd(2, 40, 30, seed=2, spread=False), rnd(9, 2, 30, seed=3, spread=False)
+    _, both = torch.ops.clt_hip.linear8(x, W, None, True, True, True)
+    _, only_w = torch.ops.clt_hip.linear8(x, W, None, True, False, True)
+    bwd = torch.ops.clt_hip.linear8_bwd
+    assert torch.equal(bwd(dy, both, 40, True, True, True, None, False)[0], bwd(dy, only_w, 40, True, False, True, None, False)[0])
+    for args in ((both[:-1], 40, True, True, True, None, False), (only_w, 40, True, True, True, None, False), (both.cpu(), 40, True, True, True, None, False),
+                 (only_w, 40, True, False, True, torch.float32, False), (both.view(torch.int8), 40, True, True, True, None, False), (both, 400, True, True, True, None, False)):
+        with pytest.raises((ValueError, RuntimeError)):
+            bwd(dy, *args)
 
 
 def reference_clt(feat, Ws, b, g):
