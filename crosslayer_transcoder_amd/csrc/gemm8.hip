@@ -23,29 +23,36 @@ typedef b8_bf16x8 bf16x8;
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-// One block of 4 waves of 64 x 64.  Blocks of k (16 KB of A, 16 KB of B, their scale bytes) arrive by DMA in a ring of four LDS
-// buffers, three ahead; a block's fragments are read while the previous block's products run, one barrier a block.
+// One block of 4 waves of 64 x 64.  Blocks of k (16 KB of A, 16 KB of B, their scale bytes) arrive by DMA in a ring of DEPTH LDS
+// buffers; a block's fragments are read while the previous block's products run, one barrier a block.  DEPTH 4 where a CU has one
+// tile, 2 (two tiles a CU, one's loads and stores under the other's products) where there are more than 256: 2048 x 4096 x 4096 with fp32
+// results 73 / 62 us, 12 x (64 x 768 x 32768) 125 / 100, but 1536 x 4096 x 1792 (168 tiles) 24 / 34.
 // LDS rows of 128 bytes, 16-byte chunks XOR-swizzled with bits 1..3 of the row.  Row p of a 64-row half is matrix row
 // (p % 16) * 4 + p / 16 (A) or c(p % 16) * 4 + p / 16 (B, c(4 q + i) = 4 i + q): a lane's four fragments are four consecutive rows,
 // so their scales are one dword, and its accumulators of the four B fragments are four consecutive columns.
 // Bound: a block of k is 64 instructions of 32 cycles (four waves: 512 cycles of each SIMD; fp32 results 1024) against 96 KB through
-// LDS (768 cycles); with every CU busy it takes 0.6 us (fp32 results: 1.0).  1024 x 4096 x 4096: 27.5 us = 1250 TFLOP/s.
-constexpr int OPB = 128 * 128, STG = 2 * OPB + 512, DEPTH = 4;
+// LDS (768 cycles); with every CU busy it takes 0.6 us (fp32 results: 1.0), two together 0.85 (1.6).  2048 x 4096 x 4096: 39 us = 1760
+// TFLOP/s.
+constexpr int OPB = 128 * 128, STG = 2 * OPB + 512;
 constexpr int PIECES = 9;                            // DMA instructions of a wave per block of k
 extern __shared__ __attribute__((aligned(1024))) unsigned char t8_smem[];
 
-template <int DT, int FA, int FB> __global__ __launch_bounds__(256, 1) void gemm8_kernel(Gemm8Args g) {
+template <int DT, int FA, int FB, int DEPTH> __global__ __launch_bounds__(256, DEPTH == 2 ? 2 : 1) void gemm8_kernel(Gemm8Args g) {
     constexpr bool WIDE = DT == CLT_DT_F32;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
     const int wb = w >> 1, wa = w & 1;
+    // every XCD (block index mod 8) works on a contiguous range of tiles, so that its L2 holds their operands once (12 x (768 x 4096 x 768):
+    // 61 -> 39 us); not where K is cut: the columns of one slice lie in a few of an L2's channels (512 x 8192 x 768: 18 -> 21 us)
+    const int xcd = blockIdx.x & 7, per = gridDim.x >> 3, more = gridDim.x & 7;
+    const int lid = g.slices > 1 ? blockIdx.x : (xcd < more ? xcd * (per + 1) : more + xcd * per) + (blockIdx.x >> 3);
     int a0, b0, slice = 0, batch;
     if (g.first) {                                       // a quarter of one of the large tiles that are left
-        const B8Tile t = b8_tile(g, g.first + (blockIdx.x >> 2));
-        a0 = t.a0 + (blockIdx.x & 1) * 128; b0 = t.b0 + (blockIdx.x >> 1 & 1) * 128;
+        const B8Tile t = b8_tile(g, g.first + (lid >> 2));
+        a0 = t.a0 + (lid & 1) * 128; b0 = t.b0 + (lid >> 1 & 1) * 128;
         batch = t.batch;
         if (a0 >= g.M || b0 >= g.N) return;
     } else {
-        const int nwg = g.tilesA * g.tilesB, tile = blockIdx.x % nwg, id = blockIdx.x / nwg;
+        const int nwg = g.tilesA * g.tilesB, tile = lid % nwg, id = lid / nwg;
         slice = id % g.slices; batch = id / g.slices;
         a0 = tile % g.tilesA * 128; b0 = tile / g.tilesA * 128;
     }
@@ -129,9 +136,9 @@ template <int DT, int FA, int FB> __global__ __launch_bounds__(256, 1) void gemm
             }
         }
     };
-    // this wave's pieces of the next block have landed (the two blocks behind it may be on their way) and its reads are complete
-#define G8_NEXT() asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(2 * PIECES) : "memory")
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(3 * PIECES) : "memory");
+    // this wave's pieces of the next block have landed (the blocks behind it may be on their way) and its reads are complete
+#define G8_NEXT() asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((DEPTH - 2) * PIECES) : "memory")
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((DEPTH - 1) * PIECES) : "memory");
     fragments(0, 0);
     int k = 0;
     for (; k + 1 < nk; k += 2) {
@@ -204,47 +211,59 @@ template <int DT> __global__ __launch_bounds__(256) void gemm8_fold_kernel(Gemm8
     b8_store4<DT>(g.c, batch * g.bc + (long)row * g.ldc + col, s, valid, g.accumulate);
 }
 
-// Which tiles, and into how many slices K is cut: the least of the times that these measurements add up to (us; a pass is one tile on
-// every CU):
-//                            16-bit results         fp32 results
-//   128 x 128 tiles          7 + 0.6 a block of k   7 + 1.0         a pass
-//   256 x 256 tiles          8 + 1.3                15 + 2.7
+// Which tiles, and into how many slices K is cut: the least of the times that these measurements add up to (us):
+//                                             16-bit results          fp32 results
+//   128 x 128 tiles, up to 256                7 + 0.6 a block of k    7 + 1.0
+//     a pass of up to 512, two a CU          10.5 + 0.85              9 + 1.6
+//     up to 256 that are left                 5 + 0.8                 5 + 0.95
+//   256 x 256 tiles, a pass of up to 256      9 + 1.3                15 + 2.9
 //   slices: the second launch 4, the partial sums 8 bytes an element and slice at 5 TB/s
-// e.g. (M, K, N; small against large tiles, us) 2048 x 1024 x 4096: 23.0 / 17.6 (bf16), 29.4 / 35.2 (fp32); 12 x (768 x 4096 x 768): 64 / 49
-// and 78 / 101; whole against sliced: 128 x 32768 x 768: 132 / 21; 1024 x 4096 x 768: 23 / 18; 1024 x 2048 x 2048: 16.3 / 20.1.
+// e.g. (M, K, N; small against large tiles, us) 2048 x 4096 x 4096: 39 / 46 (bf16), 62 / 98 (fp32); 2304 x 4096 x 4096: 67 / 47 and 92 / 98;
+// 4096 x 4096 x 4096: 78 / 54 and 131 / 111; whole against sliced: 128 x 32768 x 768: 132 / 21; 1024 x 4096 x 768: 23 / 18;
+// 1024 x 2048 x 2048: 16.3 / 20.1.
 // A slice keeps 4 blocks (the ring), slices of the large form are equal, partial sums take at most 256 MB.  The large form is not
-// for less than 128 rows on either side: such a tile is more than half empty (12 x (64 x 768 x 32768): 125 / 131).
+// for less than 128 rows on either side: such a tile is more than half empty.
 // Large tiles that do not fill their last pass may be left to small ones (a second launch: 3): 4352 x 4096 x 4096 whole / shared 93 / 77
 // and 188 / 139; 12 x (4096 x 8192 x 768): 346 / 326 and 584 / 511.
 struct Plan { long large; int slices; };                 // large tiles (0: small ones only; else the rest are small), slices of K
+double small_time(long tiles, double kb, bool wide) {
+    if (tiles <= 256) return 7.0 + kb * (wide ? 1.0 : 0.6);
+    const double pass = wide ? 9.0 + 1.6 * kb : 10.5 + 0.85 * kb, rest = 5.0 + kb * (wide ? 0.95 : 0.8);
+    const long left = tiles % 512;
+    return (double)(tiles / 512) * pass + (left > 256 ? pass : left ? rest : 0.0);
+}
 Plan plan_of(int M, int N, int KB, int batch, bool wide) {
-    const double elements = (double)batch * M * N, small = 7.0 + KB * (wide ? 1.0 : 0.6);
+    const double elements = (double)batch * M * N;
     Plan best = {0, 1};
     double least = 1e30;
     for (int large = 0; large < 2; ++large) {
         const long side = large ? 256 : 128, tiles = ((M - 1) / side + 1) * ((N - 1) / side + 1) * batch, full = tiles / 256 * 256;
         if (large && (M < 128 || N < 128 || KB < 1 || tiles > 0x3fffffffL)) break;
-        const double block = large ? (wide ? 2.7 : 1.3) : wide ? 1.0 : 0.6, pass = large ? (wide ? 15.0 : 8.0) : 7.0;
+        auto pass = [&](double kb) { return wide ? 15.0 + 2.9 * kb : 9.0 + 1.3 * kb; };
         for (long s = 1; s == 1 || (s * tiles <= 256 && s * 4 <= KB && s * elements * 4.0 <= 268435456.0); ++s) {
             if (large && s > 1 && (KB % s || 1024L * N > 0x7fffffffL)) continue;       // (offsets of the partial sums: 32 bits)
             const long per = (KB + s - 1) / s, used = per ? (KB + per - 1) / per : 1;
-            const double t = (double)((tiles * used + 255) / 256) * (per * block + pass) + (used > 1 ? 4.0 + used * elements * 8.0 / 5e6 : 0.0);
+            const double t = (large ? (double)((tiles * used + 255) / 256) * pass(per) : small_time(tiles * used, per, wide)) +
+                             (used > 1 ? 4.0 + used * elements * 8.0 / 5e6 : 0.0);
             if (t < least) { least = t; best = {large ? tiles : 0, (int)used}; }
         }
         if (large && full && full < tiles) {
-            const double t = (double)(full / 256) * (KB * block + pass) + (double)((4 * (tiles - full) + 255) / 256) * small + 3.0;
+            const double t = (double)(full / 256) * pass(KB) + small_time(4 * (tiles - full), KB, wide) + 3.0;
             if (t < least) { least = t; best = {full, 1}; }
         }
     }
     return best;
 }
 
-template <int DT, int FA, int FB> int launch_fmt(const Gemm8Args& g, long blocks, hipStream_t st) {
-    const auto f = gemm8_kernel<DT, FA, FB>;
+template <int DT, int FA, int FB, int DEPTH> int launch_depth(const Gemm8Args& g, long blocks, hipStream_t st) {
+    const auto f = gemm8_kernel<DT, FA, FB, DEPTH>;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, DEPTH * STG) != hipSuccess) return CLT_ERR_LAUNCH;
     f<<<dim3((unsigned)blocks), dim3(256), DEPTH * STG, st>>>(g);
     CLT_LAUNCH_CHECK();
     return CLT_OK;
+}
+template <int DT, int FA, int FB> int launch_fmt(const Gemm8Args& g, long blocks, hipStream_t st) {
+    return blocks > 256 ? launch_depth<DT, FA, FB, 2>(g, blocks, st) : launch_depth<DT, FA, FB, 4>(g, blocks, st);
 }
 template <int DT> int fold(const Gemm8Args& g, hipStream_t st) {
     const int quads = (g.N - 1) / 4 + 1;
