@@ -16,8 +16,8 @@ typedef b8_f32x4 f32x4;
 typedef b8_bf16x8 bf16x8;
 constexpr int WAVES = 8, MAX_T = 32;
 constexpr int LDS_CAP = 136 * 1024;                  // packed slice of x at most
-// (64 tokens: packing and the tiled product are as fast or faster, 129 against 138 us for 768 -> 32768 x 12 layers, 47 against 101 for
-// 4096 -> 32768; 32 tokens: 121 against 74)
+// (beyond 32 tokens packing and the tiled product are faster: 64 tokens, 12 layers of 768 -> 32768 102 against 138 us; 32 tokens: 102 against
+// 78, 4096 -> 4096 20 against 13, 393216 -> 768 107 against 105)
 
 struct Rows8Args {
     const void* x; long x_token, x_layer;            // strides in elements

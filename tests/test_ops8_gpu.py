@@ -180,7 +180,8 @@ def test_product(shape, out):
 #: enough 256 x 256 tiles to fill the chip: whole and partial ones, 1, 2, 3 and many blocks of k, odd rows of results
 LARGE = [(1, 3000, 100, 2901), (12, 700, 256, 1100), (12, 701, 300, 1101), (3, 2048, 1024, 2048), (33, 300, 640, 515), (1, 128, 384, 40000),
          (1, 2100, 8192, 1801), (2, 1100, 12200, 1700), (1, 800, 24576, 1900), (2, 600, 20480, 1801),        # (these two: and K in slices)
-         (1, 4100, 300, 4500), (3, 3000, 640, 2901)]                # (and a rest of small tiles)
+         (1, 4100, 300, 4500), (3, 3000, 640, 2901),                # (and a rest of small tiles)
+         (2, 2100, 300, 3501), (4, 1000, 640, 3900)]
 
 
 @gpu
