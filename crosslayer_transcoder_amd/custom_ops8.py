@@ -188,52 +188,78 @@ def _clt_source(s, L, d):
     return (s, 0) if s < (L + 1) // 2 else (L - 1 - s, (s + 1) * d)
 
 
-def _clt_pack_weight(W, l, L, kq, ks, tq, ts):
-    """W_l [l + 1, F, d] -> its transpose [d, (l + 1) F] (tq, ts) and its columns of every source layer's operand (kq, ks; or None)."""
+def _clt_kept_shapes(B, L, F, d, keep_x, keep_w):
+    """Shapes of the kept uint8 tensors: [x transposed (codes, scale bytes)] + [codes, scale bytes] of all source layers' operands, or of every
+    W_l where the borders are not the blocks'."""
+    def form(rows, cols):
+        return [(1, rows, _up(cols)), (1, _up(cols) // 128, _up(rows))]
+    shapes = form(L * F, B) if keep_x else []
+    if keep_w and _clt_aligned(F, d):
+        shapes += [((L + 1) // 2, F, (L + 1) * d), ((L + 1) // 2, (L + 1) * d // 128, F)]
+    elif keep_w:
+        for l in range(L):
+            shapes += form((l + 1) * F, d)
+    return shapes
+
+
+def _clt_pack_weight(W, l, L, kq, ks, tq, ts, st):
+    """W_l [l + 1, F, d] -> its transpose [d, (l + 1) F] (at tq, ts) and its columns of every source layer's operand (at kq, ks; or None)."""
     n, F, d = W.shape
     H, pitch, K = (L + 1) // 2, (L + 1) * d, (l + 1) * F
-    with ops8._on(W.device):
-        st = ops8._stream(W.device)
-        for s0, s1 in ((0, min(n, H)), (H, n)):              # (the layers of the second half lie the other way round)
-            if s0 >= s1:
-                continue
-            (p, c), step = _clt_source(s0, L, d), 1 if s0 == 0 else -1
-            at = lambda t, rows, p, c: t.data_ptr() + (p * rows * pitch + c) if t is not None else None  # noqa: E731
-            c += (l - s0) * d                                # (one source layer further, this target lies d columns further left or right)
-            q, s = (at(kq, F, p, c), ks.data_ptr() + (p * pitch + c) // 128 * F) if kq is not None else (None, None)
-            _call(lib.clt_pack8_into, W.data_ptr() + s0 * W.stride(0) * W.element_size(), _DT[W.dtype], W.stride(1), W.stride(0), s1 - s0, F, d, _E4M3, 1,
-                  q, s, pitch, step * F * pitch + (-d if s0 == 0 else 0), (step * pitch + (-d if s0 == 0 else 0)) // 128 * F,
-                  tq.data_ptr() + s0 * F, ts.data_ptr() + s0 * F // 128 * d, K, F, F // 128 * d, None, None, 0, st)
+    for s0, s1 in ((0, min(n, H)), (H, n)):                  # (the layers of the second half lie the other way round)
+        if s0 >= s1:
+            continue
+        p, c = _clt_source(s0, L, d)
+        c += (l - s0) * d                                    # (one source layer further, this target lies d columns further left or right)
+        step, left = (1, d) if s0 == 0 else (-1, 0)
+        _call(lib.clt_pack8_into, W.data_ptr() + s0 * W.stride(0) * W.element_size(), _DT[W.dtype], W.stride(1), W.stride(0), s1 - s0, F, d, _E4M3, 1,
+              kq + p * F * pitch + c if kq else None, ks + (p * pitch + c) // 128 * F if kq else None, pitch, step * F * pitch - left,
+              (step * pitch - left) // 128 * F, tq + s0 * F, ts + s0 * F // 128 * d, K, F, F // 128 * d, None, None, 0, st)
+
+
+def _product(a, b, K, c, dtype, ldc, bias, device, st):
+    """One clt_gemm8 of operands (codes, scale bytes, their pitches, rows) into c, all addresses."""
+    (aq, as_, lda, ldas, M), (bq, bs, ldb, ldbs, N) = a, b
+    nws = lib.clt_gemm8_workspace_bytes(M, N, K, 1)
+    ws = _bytes(nws, device) if nws else None
+    _call(lib.clt_gemm8, aq, as_, _E4M3, lda, ldas, 0, 0, bq, bs, _E4M3, ldb, ldbs, 0, 0, c, dtype, ldc, 0, bias, 0, M, N, K, 1, 0,
+          ws.data_ptr() if nws else None, nws, st)
 
 
 def _clt_forward(feat, b, Ws, keep_x, keep_w):
-    """-> recons [B, L, d], kept: [x transposed (codes, scale bytes)] + the weights for the input gradient: [codes, scale bytes] of all source
-    layers' operands, or [W_l (codes, scale bytes)] ... where the borders are not the blocks'."""
+    """-> recons [B, L, d], the kept tensors."""
     feat = ops8._dense(feat, (3,)).contiguous()
     B, L, F = feat.shape
     d = Ws[0].shape[2]
     if not (L and F and d):
         raise ValueError(f"empty map: features {tuple(feat.shape)}, W_0 {tuple(Ws[0].shape)}")
+    dev = feat.device
     flat = feat.view(B, L * F)
-    out = torch.empty((B, L, d), dtype=feat.dtype, device=feat.device)
-    whole, aligned = F % ops8.BLOCK == 0, _clt_aligned(F, d)
+    out = torch.empty((B, L, d), dtype=feat.dtype, device=dev)
+    b = ops8._bias(b, L, d, dev)
+    whole = F % ops8.BLOCK == 0
     q, s, xt, xs, _ = ops8.pack8_raw(flat.unsqueeze(0), _E4M3, whole, keep_x) if whole or keep_x else (None,) * 5
     kept = [xt, xs] if keep_x else []
+    if _clt_aligned(F, d):
+        k = [_bytes(shape, dev) for shape in _clt_kept_shapes(B, L, F, d, False, keep_w)]
+        kq, ks = (t.data_ptr() for t in k) if keep_w else (None, None)
+        tmp = _bytes(d * L * F + L * F // 128 * d, dev)      # one target layer's operand after the other
+        tq, ts, es = tmp.data_ptr(), tmp.data_ptr() + d * L * F, out.element_size()
+        with ops8._on(dev):
+            st = ops8._stream(dev)
+            for l, W in enumerate(Ws):
+                K = (l + 1) * F
+                _clt_pack_weight(ops8._dense(W, (3,)), l, L, kq, ks, tq, ts, st)
+                if B:
+                    _product((q.data_ptr(), s.data_ptr(), L * F, _up(B), B), (tq, ts, K, d, d), K, out.data_ptr() + l * d * es, _DT[out.dtype], L * d,
+                             b.data_ptr() + 4 * l * d if b is not None else None, dev, st)
+        return out, kept + k
     x = ops8.Block8(q, s, B, L * F) if whole else None
-    kq = ks = None
-    if aligned and keep_w:
-        kq, ks = feat.new_empty(((L + 1) // 2, F, (L + 1) * d), dtype=torch.uint8), feat.new_empty(((L + 1) // 2, (L + 1) * d // 128, F), dtype=torch.uint8)
-        kept += [kq, ks]
     for l, W in enumerate(Ws):
         K = (l + 1) * F
-        W = ops8._dense(W, (3,))
-        if aligned:
-            tq, ts = feat.new_empty((1, d, K), dtype=torch.uint8), feat.new_empty((1, K // 128, d), dtype=torch.uint8)
-            _clt_pack_weight(W, l, L, kq, ks, tq, ts)
-        else:
-            dq, ds, tq, ts, _ = ops8.pack8_raw(W.reshape(1, K, d), _E4M3, keep_w, True, tiles=True)
-            if keep_w:
-                kept += [dq, ds]
+        dq, ds, tq, ts, _ = ops8.pack8_raw(ops8._dense(W, (3,)).reshape(1, K, d), _E4M3, keep_w, True, tiles=True)
+        if keep_w:
+            kept += [dq, ds]
         ops8.gemm8(x.first_columns(K) if whole else ops8.quantize8(flat[:, :K]), ops8.Block8(tq, ts, d, K), None if b is None else b[l:l + 1],
                    out=out[:, l].unsqueeze(0))
     return out, kept
@@ -243,30 +269,40 @@ def _clt_gradients(g, kept, F, has_x, need_dx, w_dtypes, need_db):
     """-> dfeat [B, L, F] of g's type, [dW_l [l + 1, F, d]], db fp32 [L, d]; None where not asked for (w_dtypes empty: no dW)."""
     g = ops8._dense(g, (3,))
     B, L, d = g.shape
-    aligned = _clt_aligned(F, d)
-    # aligned: one matrix [B, L d], whose transpose holds layer l's in rows l d ..; else a matrix [B, d] for each layer
-    m = g.reshape(1, B, L * d) if aligned else g.transpose(0, 1)
-    q, s, qt, qs, db = ops8.pack8_raw(m, _E4M3, need_dx or not w_dtypes, bool(w_dtypes), sums=need_db)
-    dx, dWs = None, None
+    dev = g.device
     ws = kept[2:] if has_x else kept
-    if need_dx and aligned:
-        dx = torch.empty((B, L, F), dtype=g.dtype, device=g.device)
-        gb = ops8.Block8(q, s, B, L * d)
-        for k in range(L):
-            p, c = _clt_source(k, L, d)
-            w = ops8.Block8(ws[0][p:p + 1], ws[1][p:p + 1], F, (L + 1) * d)
-            ops8.gemm8(gb.columns(k * d, (L - k) * d), w.columns(c, (L - k) * d), out=dx[:, k].unsqueeze(0))
-    elif need_dx:
-        dx = torch.empty((B, L * F), dtype=torch.float32, device=g.device)
+    dx, dWs = None, None
+    if _clt_aligned(F, d):
+        # one matrix [B, L d]; its transpose holds layer l's in rows l d ..
+        q, s, qt, qs, db = ops8.pack8_raw(g.reshape(1, B, L * d), _E4M3, need_dx or not w_dtypes, bool(w_dtypes), sums=need_db)
+        t, pitch = _up(B), (L + 1) * d
+        with ops8._on(dev):
+            st = ops8._stream(dev)
+            if need_dx:
+                dx = torch.empty((B, L, F), dtype=g.dtype, device=dev)
+                wq, wsc = ws[0].data_ptr(), ws[1].data_ptr()
+                for k in range(L if B else 0):
+                    p, c = _clt_source(k, L, d)
+                    _product((q.data_ptr() + k * d, s.data_ptr() + k * d // 128 * t, L * d, t, B),
+                             (wq + p * F * pitch + c, wsc + (p * pitch + c) // 128 * F, pitch, F, F), (L - k) * d,
+                             dx.data_ptr() + k * F * dx.element_size(), _DT[g.dtype], L * F, None, dev, st)
+            if w_dtypes:
+                dWs = [torch.empty((l + 1, F, d), dtype=dt, device=dev) for l, dt in enumerate(w_dtypes)]
+                for l, dW in enumerate(dWs):
+                    _product((kept[0].data_ptr(), kept[1].data_ptr(), t, L * F, (l + 1) * F), (qt.data_ptr() + l * d * t, qs.data_ptr() + l * d, t, L * d, d), B,
+                             dW.data_ptr(), _DT[dW.dtype], d, None, dev, st)
+        return dx, dWs, db.view(L, d) if need_db else None
+    q, s, qt, qs, db = ops8.pack8_raw(g.transpose(0, 1), _E4M3, need_dx or not w_dtypes, bool(w_dtypes), sums=need_db)
+    if need_dx:
+        dx = torch.empty((B, L * F), dtype=torch.float32, device=dev)
         for l in range(L - 1, -1, -1):                     # (the last layer reaches every column and writes; the others add)
             K = (l + 1) * F
             ops8.gemm8(ops8.Block8(q[l:l + 1], s[l:l + 1], B, d), ops8.Block8(ws[2 * l], ws[2 * l + 1], K, d), out=dx[:, :K].unsqueeze(0), accumulate=l != L - 1)
         dx = dx.view(B, L, F).to(g.dtype)
     if w_dtypes:
         x = ops8.Block8(kept[0], kept[1], L * F, B)
-        gt = [ops8.Block8(qt[:, l * d:(l + 1) * d], qs[:, :, l * d:(l + 1) * d], d, B) if aligned else ops8.Block8(qt[l:l + 1], qs[l:l + 1], d, B) for l in range(L)]
-        dWs = [ops8.gemm8(x.first_rows((l + 1) * F), gt[l], out_dtype=dt).view(l + 1, F, d) for l, dt in enumerate(w_dtypes)]
-    return dx, dWs, db.view(L, d) if need_db else None
+        dWs = [ops8.gemm8(x.first_rows((l + 1) * F), ops8.Block8(qt[l:l + 1], qs[l:l + 1], d, B), out_dtype=dt).view(l + 1, F, d) for l, dt in enumerate(w_dtypes)]
+    return dx, dWs, db
 
 
 @torch.library.custom_op("clt_hip::clt_decoder8", mutates_args=(), device_types=_DEV)
@@ -280,20 +316,19 @@ def _clt_decoder8_op(feat: Tensor, b: Optional[Tensor], Ws: List[Tensor], keep_x
 def _(feat, b, Ws, keep_x, keep_w):
     B, L, F = feat.shape
     d = Ws[0].shape[2]
-    form = lambda rows, cols: [feat.new_empty((1, rows, _up(cols)), dtype=torch.uint8), feat.new_empty((1, _up(cols) // 128, _up(rows)), dtype=torch.uint8)]  # noqa: E731
-    kept = form(L * F, B) if keep_x else []
-    if keep_w and _clt_aligned(F, d):
-        kept += [feat.new_empty(((L + 1) // 2, F, (L + 1) * d), dtype=torch.uint8), feat.new_empty(((L + 1) // 2, (L + 1) * d // 128, F), dtype=torch.uint8)]
-    elif keep_w:
-        for l in range(L):
-            kept += form((l + 1) * F, d)
-    return [feat.new_empty(B, L, d)] + kept
+    return [feat.new_empty(B, L, d)] + [feat.new_empty(shape, dtype=torch.uint8) for shape in _clt_kept_shapes(B, L, F, d, keep_x, keep_w)]
 
 
 @torch.library.custom_op("clt_hip::clt_decoder8_bwd", mutates_args=(), device_types=_DEV)
 def _clt_decoder8_bwd(g: Tensor, kept: List[Tensor], F: int, has_x: bool, need_dx: bool, w_dtype: Optional[torch.dtype], need_db: bool) -> List[Tensor]:
     """-> [dfeat of g's type, db fp32 (empty where not asked for), dW_0, ..., dW_{L-1} (w_dtype None: none)]."""
-    dx, dWs, db = _clt_gradients(g, kept, F, has_x, need_dx, [w_dtype] * g.shape[1] if w_dtype is not None else [], need_db)
+    B, L, d = g.shape
+    shapes = _clt_kept_shapes(B, L, F, d, has_x, need_dx)
+    if [tuple(t.shape) for t in kept[:len(shapes)]] != shapes or any(t.dtype != torch.uint8 or not t.is_contiguous() or t.device != g.device for t in kept):
+        raise ValueError("`kept` is not what clt_decoder8 kept for this gradient")
+    if w_dtype is not None and not has_x:
+        raise ValueError("the weights' gradient needs the features that clt_decoder8 keeps with keep_x")
+    dx, dWs, db = _clt_gradients(g, kept, F, has_x, need_dx, [w_dtype] * L if w_dtype is not None else [], need_db)
     return [g.new_empty(0) if t is None else t for t in (dx, db)] + (dWs or [])
 
 

@@ -595,6 +595,21 @@ def test_kept_bytes_that_do_not_fit_are_refused():
             bwd(dy, *args)
 
 
+@gpu
+@pytest.mark.parametrize("F,d", [(128, 128), (40, 30)])
+def test_kept_tensors_that_do_not_fit_are_refused(F, d):
+    feat, Ws, g = rnd(9, 2, F, seed=1, spread=False), [rnd(l + 1, F, d, seed=2 + l, spread=False) for l in range(2)], rnd(9, 2, d, seed=5, spread=False)
+    kept = torch.ops.clt_hip.clt_decoder8(feat, None, Ws, True, True)[1:]
+    only_w = torch.ops.clt_hip.clt_decoder8(feat, None, Ws, False, True)[1:]
+    bwd = torch.ops.clt_hip.clt_decoder8_bwd
+    assert torch.equal(bwd(g, kept, F, True, True, None, False)[0], bwd(g, only_w, F, False, True, None, False)[0])
+    for args in ((kept, F + 128, True, True, None, False), (only_w, F, True, True, None, False), (kept[:2], F, True, True, None, False),
+                 ([t.cpu() for t in kept], F, True, True, None, False), (only_w, F, False, True, torch.float32, False),
+                 ([t.view(torch.int8) for t in kept], F, True, True, None, False)):
+        with pytest.raises((ValueError, RuntimeError)):
+            bwd(g, *args)
+
+
 def reference_clt(feat, Ws, b, g):
     """[recons, dfeat, db, dW_l ...] of the cross-layer decoder in float64 from the values held."""
     B, L, F = feat.shape
