@@ -1,6 +1,6 @@
 // A linear map and its gradients in 8-bit block-scaled form, each as one call over clt_pack8 and clt_gemm8.  Why: with few tokens a training
 // step costs what the host needs between launches.  Inside a step of 16 tokens and 2 layers of 110 -> 32: forward 41 us and
-// backward 51 us with a call from Python for every launch, 33 and 41 us so (the step, autograd's own 64 us included: 170 and 150).
+// backward 51 us with a call from Python for every launch, 32 and 37 us so (the step, autograd's own 60 us included: 170 and 142).
 //
 // Bytes kept between the two: x transposed (codes [L][K][up(T)], scale bytes [L][up(T) / 128][up(K)]), then W for the input gradient (codes
 // [L][K][up(N)], scale bytes [L][up(N) / 128][up(K)]), either part only where it is kept.  All parts are multiples of 128 bytes.

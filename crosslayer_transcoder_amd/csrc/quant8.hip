@@ -214,8 +214,9 @@ template <int DT> int launch_pack(const Pack8Args& a, int fmt, bool tiles, long 
 }
 }  // namespace
 
+// (up to 128 rows: the one block of rows writes the sums themselves)
 extern "C" size_t clt_pack8_sums_workspace_bytes(int batch, int rows, int cols) {
-    return batch > 0 && rows > 0 && cols > 0 ? (size_t)batch * ((rows + B8 - 1) / B8) * cols * 4 : 0;
+    return batch > 0 && rows > B8 && cols > 0 ? (size_t)batch * ((rows - 1) / B8 + 1) * cols * 4 : 0;
 }
 
 extern "C" int clt_pack8(const void* x, int dtype, long row_stride, long batch_stride, int batch, int rows, int cols, int format,
@@ -241,15 +242,15 @@ extern "C" int clt_pack8_into(const void* x, int dtype, long row_stride, long ba
     a.q = static_cast<uint8_t*>(q); a.s = static_cast<uint8_t*>(s); a.qt = static_cast<uint8_t*>(qt); a.st = static_cast<uint8_t*>(st);
     a.R = rows; a.C = cols; a.tiles_r = (rows - 1) / B8 + 1; a.tiles_c = (cols - 1) / B8 + 1;
     const size_t need = clt_pack8_sums_workspace_bytes(batch, rows, cols);
-    if (column_sums && (!workspace || workspace_bytes < need)) return CLT_ERR_WORKSPACE;
-    a.sums = column_sums ? static_cast<float*>(workspace) : nullptr;
+    if (column_sums && need && (!workspace || workspace_bytes < need)) return CLT_ERR_WORKSPACE;
+    a.sums = !column_sums ? nullptr : need ? static_cast<float*>(workspace) : column_sums;
     const long blocks = (long)batch * a.tiles_r * a.tiles_c;
     if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
     const hipStream_t hs = as_stream(stream);
     const int rc = dtype == CLT_DT_F32 ? launch_pack<CLT_DT_F32>(a, format, tiles != 0, blocks, hs)
                    : dtype == CLT_DT_BF16 ? launch_pack<CLT_DT_BF16>(a, format, tiles != 0, blocks, hs)
                                           : launch_pack<CLT_DT_F16>(a, format, tiles != 0, blocks, hs);
-    if (rc != CLT_OK || !column_sums) return rc;
+    if (rc != CLT_OK || !column_sums || !need) return rc;
     const long n = (long)batch * cols;
     fold_sums_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, hs>>>(a.sums, column_sums, a.tiles_r, cols, n);
     CLT_LAUNCH_CHECK();

@@ -802,7 +802,7 @@ def test_refusals_of_the_library():
 
     assert [pack(r=0), pack(c=-1), pack(b=0), pack(dt=3), pack(f=2), pack(s=None), pack(q=None, s=None), pack(x=None)] == [-1] * 8
     assert [pack(x=p + 2), pack(q=p + 8), pack(s=p + 1)] == [-4] * 3
-    assert pack(cs=p) == -3 and pack(cs=p, ws=p, n=255) == -3
+    assert pack(cs=p, r=200) == -3 and pack(cs=p, r=200, ws=p, n=511) == -3
 
     def into(pitch=128, batch=0, qt=None, qt_pitch=0):
         return lib.clt_pack8_into(p, 0, 64, 0, 1, 4, 64, 0, 0, p, p, pitch, batch, 0, qt, qt, qt_pitch, 0, 0, None, None, 0, None)
