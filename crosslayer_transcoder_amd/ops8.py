@@ -37,7 +37,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(device):
     """The tensors' device made current for a launch (a no-op when it is already)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _stream(device):
@@ -69,16 +69,18 @@ class Block8:
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, rows: int, cols: int, fmt: str = "e4m3"):
         _fmt(fmt)
-        if data.dtype != torch.uint8 or scale.dtype != torch.uint8:
+        if data.dtype is not torch.uint8 or scale.dtype is not torch.uint8:
             raise TypeError("codes and scale bytes are uint8 tensors")
         if data.device != scale.device:
             raise ValueError("codes and scale bytes are on different devices")
-        if data.dim() != 3 or scale.dim() != 3 or data.shape[0] != scale.shape[0]:
+        shape, held = data.shape, scale.shape
+        if len(shape) != 3 or len(held) != 3 or shape[0] != held[0]:
             raise ValueError("codes [L, rows, bytes] and scale bytes [L, blocks, rows] have three dimensions")
-        if rows < 0 or cols < 0 or data.shape[1] != rows or data.shape[2] < _up(cols) or scale.shape[1] < _up(cols) // BLOCK or scale.shape[2] < rows:
-            raise ValueError(f"codes {tuple(data.shape)} / scale bytes {tuple(scale.shape)} do not hold a [{rows}, {cols}] matrix")
-        if data.numel() and (data.stride(2) != 1 or scale.stride(2) != 1 or data.stride(1) % 16 or data.stride(0) % 16 or data.data_ptr() % 16
-                             or scale.stride(1) % 4 or scale.stride(0) % 4 or scale.data_ptr() % 4):
+        wide = _up(cols)
+        if rows < 0 or cols < 0 or shape[1] != rows or shape[2] < wide or held[1] < wide // BLOCK or held[2] < rows:
+            raise ValueError(f"codes {tuple(shape)} / scale bytes {tuple(held)} do not hold a [{rows}, {cols}] matrix")
+        (d0, d1, d2), (s0, s1, s2) = data.stride(), scale.stride()
+        if data.numel() and (d2 != 1 or s2 != 1 or (d0 | d1 | data.data_ptr()) & 15 or (s0 | s1 | scale.data_ptr()) & 3):
             raise ValueError("packed rows are dense and start at multiples of 16 bytes (codes) and 4 bytes (scales)")
         self.data, self.scale, self.rows, self.cols, self.fmt = data, scale, rows, cols, fmt
 
