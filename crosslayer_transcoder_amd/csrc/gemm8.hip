@@ -3,12 +3,15 @@
 //   C[m][n] = sum over blocks kb of 2^(ea[kb][m] + eb[kb][n]) * (sum over the block's 128 k of a * b)
 //
 // Two inner products, by the type of the result (gfx950's 8-bit matrix instructions align the products of a group of 16 at the
-// largest one and keep about 14 bits below it — measured 1.0e-5 .. 1.5e-5 relative on normal data, whichever 8-bit instruction
-// and shape; their sums over groups and blocks are fp32):
-//   16-bit results: v_mfma_scale_f32_16x16x128_f8f6f4, one instruction per 16 x 16 tile and block of 128, scales as operands —
-//     the alignment loss is far below the result's own rounding (2^-9 bf16, 2^-12 fp16).
-//   32-bit results: the codes become bf16 in registers (2^e x code is exact in bf16) and go through v_mfma_f32_16x16x32_bf16:
-//     exact products, fp32 sums, at the 16-bit rate.
+// largest one and keep about 14 bits below it, whichever 8-bit instruction and shape; their sums over groups and blocks are fp32):
+//   bf16 results: v_mfma_scale_f32_16x16x128_f8f6f4, one instruction per 16 x 16 tile and block of 128, scales as operands.  A group is
+//     off by less than 16 * 2^-13 of its largest product, which is less than 2^-9 of the sum of |a b| over all of them.  Against 64 bits,
+//     2048 x 768 x 4096: on normal data 1.1e-5 of the result's norm (rounding to bf16: 1.66e-3), 1 % of the values are the neighbour of
+//     the rounded sum and a near-cancelled one may be off by many of its own places; with two columns 100 times larger than the rest that
+//     cancel each other 2.2e-4 of the norm, 9 % neighbours.
+//   fp16 and fp32 results: the codes become bf16 in registers (2^e x code is exact in bf16) and go through v_mfma_f32_16x16x32_bf16:
+//     exact products, fp32 sums, at the 16-bit rate.  fp16 too: its rounding is 2e-4 of the norm, no more than the alignment may lose
+//     (the cancelling columns: 3.1e-4 in all, 35 % of the values neighbours).
 // B rows ride the instruction's "M" index and A rows its "N" index, so a lane's accumulators are consecutive columns of a row of C.
 //
 // This file: the entry point and the form for everything that does not fill the chip with 256 x 256 tiles (gemm8_large.hip): 128 x 128
@@ -30,15 +33,15 @@ typedef __attribute__((address_space(3))) void lds_void;
 // LDS rows of 128 bytes, 16-byte chunks XOR-swizzled with bits 1..3 of the row.  Row p of a 64-row half is matrix row
 // (p % 16) * 4 + p / 16 (A) or c(p % 16) * 4 + p / 16 (B, c(4 q + i) = 4 i + q): a lane's four fragments are four consecutive rows,
 // so their scales are one dword, and its accumulators of the four B fragments are four consecutive columns.
-// Bound: a block of k is 64 instructions of 32 cycles (four waves: 512 cycles of each SIMD; fp32 results 1024) against 96 KB through
-// LDS (768 cycles); with every CU busy it takes 0.6 us (fp32 results: 1.0), two together 0.85 (1.6).  2048 x 4096 x 4096: 39 us = 1760
+// Bound: a block of k is 64 instructions of 32 cycles (four waves: 512 cycles of each SIMD; exact products 1024) against 96 KB through
+// LDS (768 cycles); with every CU busy it takes 0.6 us (exact products: 1.0), two together 0.85 (1.6).  2048 x 4096 x 4096: 39 us = 1760
 // TFLOP/s.
 constexpr int OPB = 128 * 128, STG = 2 * OPB + 512;
 constexpr int PIECES = 9;                            // DMA instructions of a wave per block of k
 extern __shared__ __attribute__((aligned(1024))) unsigned char t8_smem[];
 
 template <int DT, int FA, int FB, int DEPTH> __global__ __launch_bounds__(256, DEPTH == 2 ? 2 : 1) void gemm8_kernel(Gemm8Args g) {
-    constexpr bool WIDE = DT == CLT_DT_F32;
+    constexpr bool WIDE = DT != CLT_DT_BF16;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), fr = lane & 15, fq = lane >> 4;
     const int wb = w >> 1, wa = w & 1;
     // every XCD (block index mod 8) works on a contiguous range of tiles, so that its L2 holds their operands once (12 x (768 x 4096 x 768):
@@ -212,7 +215,7 @@ template <int DT> __global__ __launch_bounds__(256) void gemm8_fold_kernel(Gemm8
 }
 
 // Which tiles, and into how many slices K is cut: the least of the times that these measurements add up to (us):
-//                                             16-bit results          fp32 results
+//                                             bf16 results            exact products (fp32 results)
 //   128 x 128 tiles, up to 256                7 + 0.6 a block of k    7 + 1.0
 //     a pass of up to 512, two a CU          10.5 + 0.85              9 + 1.6
 //     up to 256 that are left                 5 + 0.8                 5 + 0.95
@@ -304,7 +307,7 @@ extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long 
                    static_cast<const uint8_t*>(b_scale), c, bias, lda, ldas, ldb, ldbs, ldc, a_batch, as_batch, b_batch, bs_batch,
                    c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 0u, 0u, 0u, 1, KB, nullptr, 0, 0};
     const hipStream_t st = as_stream(stream);
-    Plan plan = plan_of(M, N, KB, batch, c_dtype == CLT_DT_F32);
+    Plan plan = plan_of(M, N, KB, batch, c_dtype != CLT_DT_BF16);
     // (results whose rows lie further apart than the large form's 32-bit offsets reach)
     if (plan.slices == 1 && 256 * ldc * 4 > 0x7fffffffL) plan.large = 0;
     g.slices = plan.slices;

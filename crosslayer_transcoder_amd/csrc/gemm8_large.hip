@@ -13,7 +13,7 @@
 // c(4 q + i) = 4 i + q (B), so fragment j of a wave is rows 8 * lane + j: (a) the scale bytes of a lane's eight fragments are eight
 // consecutive bytes — one 8-byte read per operand and block, the instruction picks its byte by op_sel; (b) a lane's
 // accumulators of the eight B fragments are eight consecutive columns of C — 16 bytes of 16-bit results, 32 of fp32 — and four
-// lanes make 64 / 128 consecutive bytes.  16-bit results pass through a 4 KB slab of LDS a wave, so that 256 bytes of a row leave
+// lanes make 64 / 128 consecutive bytes.  bf16 results pass through a 4 KB slab of LDS a wave, so that 256 bytes of a row leave
 // together, and past the caches, which hold the operands' panels (4096 x 768 x 32768 x 12: 1728 -> 1462 us; without the slab the
 // uncached stores are slower than cached ones, 1765 us).
 // Bound: the matrix units, at what clock the power leaves them (8192^3: 390 .. 437 us from card to card = 2.5 .. 2.8 PFLOP/s; the large library
@@ -250,12 +250,13 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // no DMA into this block's LDS outlives it
 }
 
-// ---- 32-bit results: the codes become bf16 in registers and the products run at the 16-bit rate, so a block of k costs twice the
+// ---- exact products (fp32 and fp16 results): the codes become bf16 in registers and the products run at the 16-bit rate, so a block of k costs twice the
 // cycles for the same LDS bytes: 8 waves of 128 x 64 (B x A; 192 KB of reads in 4096 cycles), two per SIMD, whose conversions run
 // under each other's matrix instructions.  Tiles, DMA, row order and the stream of blocks as above; A fragments are 4 rows of a
 // 64-row group (row 4 * lane + n).  8192^3: 795 .. 825 us = 1.33 .. 1.38 PFLOP/s, the rate of the large library product in bf16 (1.32).
-template <int FA, int FB>
-__global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, int total) {
+template <int DT, int FA, int FB>
+__global__ __launch_bounds__(512, 2) void gemm8_large_exact_kernel(Gemm8Args g, int total) {
+    typedef typename Elem<DT>::type T;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wb = w >> 2, wa = w & 3, fr = lane & 15, fq = lane >> 4;
     const int nk = g.slice_kb;                            // blocks of k of a tile (K, or a slice of it)
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
     for (int m = 0; m < 8; ++m)
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int NST = 32;                               // stores of an interior tile per lane
+    constexpr int NST = DT == CLT_DT_F32 ? 32 : 16;       // stores of an interior tile per lane
     B8Tile t = b8_tile(g, vb);
     enter(t);
     for (int k = 0; k < 2; ++k) {
@@ -370,11 +371,11 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
         // ---- results: for (n, i) a lane has row 4 fr + n of its 64 and eight columns 8 (4 i + fq) .. of its 128
         const int r0 = wa * 64 + fr * 4, c0 = wb * 128 + fq * 8;
         const bool interior = cur.a0 + 256 <= g.M && cur.b0 + 256 <= g.N;
-        float* ctile = static_cast<float*>(g.c) + cur.batch * g.bc + cur.slice * g.slice_stride + (long)cur.a0 * g.ldc + cur.b0;
+        T* ctile = static_cast<T*>(g.c) + cur.batch * g.bc + cur.slice * g.slice_stride + (long)cur.a0 * g.ldc + cur.b0;
         const float* bl = reinterpret_cast<const float*>(g8_smem + BIAS_BASE + cslot * 1024) + c0;
         const bool has_bias = g.bias != nullptr;
         const int rows = g.M - cur.a0 - r0, cols = g.N - cur.b0 - c0;
-        const unsigned at = (unsigned)(r0 * (int)g.ldc + c0) * 4u;
+        const unsigned at = (unsigned)(r0 * (int)g.ldc + c0) * (unsigned)sizeof(T);
 #pragma unroll
         for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -382,8 +383,14 @@ __global__ __launch_bounds__(512, 2) void gemm8_large_f32_kernel(Gemm8Args g, in
                 f32x4 lo = f32x4{acc[0][n][i], acc[1][n][i], acc[2][n][i], acc[3][n][i]};
                 f32x4 hi = f32x4{acc[4][n][i], acc[5][n][i], acc[6][n][i], acc[7][n][i]};
                 if (has_bias) { lo += *reinterpret_cast<const f32x4*>(bl + i * 32); hi += *reinterpret_cast<const f32x4*>(bl + i * 32 + 4); }
-                float* p = reinterpret_cast<float*>(reinterpret_cast<char*>(ctile + (long)n * g.ldc + i * 32) + at);
-                if (interior || (n < rows && i * 32 + 8 <= cols)) {
+                T* p = reinterpret_cast<T*>(reinterpret_cast<char*>(ctile + (long)n * g.ldc + i * 32) + at);
+                if constexpr (DT != CLT_DT_F32) {
+                    const u32x4 u = {pack_out16<DT>(lo[0], lo[1]), pack_out16<DT>(lo[2], lo[3]), pack_out16<DT>(hi[0], hi[1]), pack_out16<DT>(hi[2], hi[3])};
+                    if (interior || (n < rows && i * 32 + 8 <= cols)) *reinterpret_cast<u32x4_u*>(p) = u;
+                    else if (n < rows)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) if (i * 32 + j < cols) p[j] = (T)(u[j >> 1] >> (16 * (j & 1)));
+                } else if (interior || (n < rows && i * 32 + 8 <= cols)) {
                     if (g.accumulate) { lo += *reinterpret_cast<const f32x4_u*>(p); hi += *reinterpret_cast<const f32x4_u*>(p + 4); }
                     *reinterpret_cast<f32x4_u*>(p) = lo;
                     *reinterpret_cast<f32x4_u*>(p + 4) = hi;
@@ -409,12 +416,12 @@ template <class F> int launch(F f, int threads, const Gemm8Args& g, int total, h
     CLT_LAUNCH_CHECK();
     return CLT_OK;
 }
-// fast: 8-bit instructions (16-bit results, or the partial sums of their slices)
+// fast: 8-bit instructions (bf16 results, or the partial sums of their slices)
 template <int FA, int FB> int launch_dtype(const Gemm8Args& g, int dtype, bool fast, int total, hipStream_t st) {
-    if (dtype == CLT_DT_F32 && !fast) return launch(gemm8_large_f32_kernel<FA, FB>, 512, g, total, st);
-    if (dtype == CLT_DT_F32) return launch(gemm8_large_kernel<CLT_DT_F32, FA, FB>, 256, g, total, st);
-    if (dtype == CLT_DT_BF16) return launch(gemm8_large_kernel<CLT_DT_BF16, FA, FB>, 256, g, total, st);
-    return launch(gemm8_large_kernel<CLT_DT_F16, FA, FB>, 256, g, total, st);
+    if (fast && dtype == CLT_DT_F32) return launch(gemm8_large_kernel<CLT_DT_F32, FA, FB>, 256, g, total, st);
+    if (fast) return launch(gemm8_large_kernel<CLT_DT_BF16, FA, FB>, 256, g, total, st);
+    if (dtype == CLT_DT_F32) return launch(gemm8_large_exact_kernel<CLT_DT_F32, FA, FB>, 512, g, total, st);
+    return launch(gemm8_large_exact_kernel<CLT_DT_F16, FA, FB>, 512, g, total, st);
 }
 }  // namespace
 
@@ -422,7 +429,7 @@ template <int FA, int FB> int launch_dtype(const Gemm8Args& g, int dtype, bool f
 // of b8_tile (slices: all)
 int clt_internal_gemm8_large(const Gemm8Args& g0, int fa, int fb, int dtype, int tiles, hipStream_t st) {
     Gemm8Args g = g0;
-    const bool fast = dtype != CLT_DT_F32;
+    const bool fast = dtype == CLT_DT_BF16;
     if (g.part) {
         g.c = g.part; g.ldc = g.N; g.bc = (long)g.M * g.N; g.slice_stride = g.batch * g.bc;
         g.bias = nullptr; g.accumulate = 0;

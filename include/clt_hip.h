@@ -558,8 +558,9 @@ int clt_pack8_into(const void* x, int dtype, long row_stride, long batch_stride,
 int clt_unpack8(const void* q, const void* s, int format, int batch, int rows, int cols, long pitch, long scale_pitch,
                 long q_batch_stride, long s_batch_stride, void* out, int dtype, void* stream);
 /* C[M][N] (+)= A[M][K] * B[N][K]^T + bias[N], batched; pitches and batch strides of A, B in bytes, of C and bias in elements.
- * c_dtype bf16 / fp16: 8-bit matrix instructions (products aligned to ~14 bits in groups of 16, fp32 sums, one rounding);
- * c_dtype fp32: exact products (bf16 instructions), fp32 sums; accumulate != 0 (fp32 only): C += . K = 0 gives the bias.
+ * c_dtype bf16: 8-bit matrix instructions (products aligned to ~14 bits below the largest of a group of 16: less than 2^-9 of the sum
+ * of |a b| in all; fp32 sums, one rounding); c_dtype fp32 / fp16: exact products (bf16 instructions), fp32 sums, one rounding;
+ * accumulate != 0 (fp32 only): C += . K = 0 gives the bias.
  * Scale rows: 4-byte aligned, readable up to a multiple of 4 bytes.  Pitches below 2^23 bytes, an operand's scale bytes below 2^31 (else
  * CLT_ERR_RANGE).  C shares no memory with the operands, nor its rows with each other.  workspace (16-byte aligned): partial sums
  * where K is cut. */

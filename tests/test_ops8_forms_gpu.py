@@ -1,0 +1,62 @@
+"""8-bit block-scaled operators: every form that a product can take, and the calls next to the documented ones (the operators' own tests:
+test_ops8_gpu.py).  Bounds are that file's; where every product and every partial sum is a whole number below 2^24, results are
+compared to the bit."""
+import math
+
+import pytest
+import torch
+
+from tests.test_ops8_gpu import check_product, close, held64, reference_clt, reference_training, rnd, same, up, values
+
+gpu = pytest.mark.gpu
+
+
+def cancelling(L, R, K, seed):
+    """Whole numbers of -1 .. 1 and, every 64 columns, two neighbours of 256: with weights_of below their products cancel, and a unit that
+    aligns products to 14 bits below the largest of a few loses the small ones."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-1, 2, (L, R, K), generator=g).float()
+    for k in range(0, K - 1, 64):
+        x[:, :, k] = x[:, :, k + 1] = 256.0
+    return x.cuda()
+
+
+def weights_of(L, N, K, seed):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randint(-1, 2, (L, N, K), generator=g).float()
+    for k in range(0, K - 1, 64):
+        w[:, :, k], w[:, :, k + 1] = 256.0, -256.0
+    return w.cuda()
+
+
+#: small tiles, K in slices, large tiles, large tiles with a rest of small ones
+CANCELLING = [(1, 200, 768, 300), (1, 100, 9000, 130), (1, 2048, 768, 8192), (1, 4100, 300, 4500), (1, 130, 128, 40000)]
+
+
+@gpu
+@pytest.mark.parametrize("shape", CANCELLING)
+def test_fp16_and_fp32_results_keep_what_cancelling_products_leave(shape):
+    """Sums below 2^11 are exact in fp16 and fp32; bf16 results stay within their documented bound."""
+    from crosslayer_transcoder_amd import ops8
+    L, M, K, N = shape
+    a, b = cancelling(L, M, K, 1), weights_of(L, N, K, 2)
+    ref = (a @ b.mT.contiguous()).cpu()                              # (exact: whole numbers, partial sums below 2^24)
+    assert float(ref.abs().max()) <= 2048
+    q, w = ops8.quantize8(a), ops8.quantize8(b)
+    assert same(ops8.gemm8(q, w), ref) and same(ops8.gemm8(q, w, out_dtype=torch.float16), ref)
+    assert same(ops8.linear8(a.transpose(0, 1).half(), w).transpose(0, 1), ref)
+    y = ops8.gemm8(q, w, out_dtype=torch.bfloat16).cpu().float()
+    assert bool(((y - ref).abs() <= 2.0 ** -9 * (a.abs() @ b.abs().mT.contiguous()).cpu() + 2.0 ** -8 * ref.abs()).all())
+
+
+@gpu
+def test_fp16_training_keeps_what_cancelling_products_leave():
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    x, w = cancelling(1, 300, 256, 1).transpose(0, 1).half(), weights_of(1, 384, 256, 2)
+    y = C.encoder8(x, w.permute(0, 2, 1), None)
+    assert same(y.transpose(0, 1), (x.transpose(0, 1).float() @ w.mT.contiguous()).cpu())
+    # dx = g W^T: the gradient's neighbours of 256 meet +256 and -256 again
+    g, W = cancelling(1, 300, 384, 3).transpose(0, 1).half(), weights_of(1, 256, 384, 4)             # W [L, K, N], blocks along N
+    x = torch.zeros(300, 1, 256, dtype=torch.float16, device="cuda").requires_grad_()
+    dx, = torch.autograd.grad(C.plt_decoder8(x, W, None), x, g)
+    assert same(dx.transpose(0, 1), (g.transpose(0, 1).float() @ W.mT.contiguous()).cpu())
