@@ -35,14 +35,24 @@ def _bytes(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
+def _check(x, W, b, kn):
+    """Refuses what does not fit: the kernels take x's sizes for W's (the op's body, its fake and the eager functions all come here)."""
+    if x.dim() != 3 or W.dim() != 3 or W.shape[0] != x.shape[1] or W.shape[1 if kn else 2] != x.shape[2]:
+        raise ValueError(f"x {tuple(x.shape)} ([tokens, layers, features]) does not match W {tuple(W.shape)}")
+    N = W.shape[2 if kn else 1]
+    if b is not None and (b.numel() != W.shape[0] * N or (b.dim() > 1 and tuple(b.shape) != (W.shape[0], N))):
+        raise ValueError(f"bias {tuple(b.shape)} does not match {W.shape[0]} layers of {N}")
+    if W.device != x.device or (b is not None and b.device != x.device):
+        raise ValueError("x, W and the bias are on different devices")
+
+
 def _forward(x, W, b, kn, keep_x, keep_w):
     """x [T, L, K], W [L, N, K] (kn: [L, K, N]) -> y [T, L, N], the kept buffer."""
+    _check(x, W, b, kn)
     x, W = ops8._dense(x, (3,)), ops8._dense(W, (3,))
     T, L, K = x.shape
     N = W.shape[2] if kn else W.shape[1]
     dev = x.device
-    if W.device != dev:
-        raise ValueError("x and W are on different devices")
     if not (L and K and N):
         raise ValueError(f"empty map: x {tuple(x.shape)}, W {tuple(W.shape)}")
     b = ops8._bias(b, L, N, dev)
@@ -86,9 +96,15 @@ def linear8(x: Tensor, W: Tensor, b: Optional[Tensor], kn: bool, keep_x: bool, k
 
 @linear8.register_fake
 def _(x, W, b, kn, keep_x, keep_w):
+    _check(x, W, b, kn)
     T, L, K = x.shape
     N = W.shape[2] if kn else W.shape[1]
     return [x.new_empty(T, L, N), x.new_empty(_kept_bytes(T, L, K, N, keep_x, keep_w), dtype=torch.uint8)]
+
+
+def _check_type(w_dtype):
+    if w_dtype is not None and w_dtype not in _DT:
+        raise TypeError(f"weight gradients are float32, bfloat16 or float16, got {w_dtype}")
 
 
 @torch.library.custom_op("clt_hip::linear8_bwd", mutates_args=(), device_types=_DEV)
@@ -99,6 +115,7 @@ def linear8_bwd(dy: Tensor, kept: Tensor, K: int, kn: bool, has_x: bool, need_dx
         raise ValueError("`kept` is not what linear8 kept for this gradient")
     if w_dtype is not None and not has_x:
         raise ValueError("the weights' gradient needs the input that linear8 keeps with keep_x")
+    _check_type(w_dtype)
     return [dy.new_empty(0) if t is None else t for t in _gradients(dy, kept, K, kn, has_x, need_dx, w_dtype, need_db)]
 
 
@@ -148,8 +165,6 @@ class _Linear8(torch.autograd.Function):
 
 
 def _linear(x, W, b, kn):
-    if x.dim() != 3 or W.dim() != 3 or W.shape[0] != x.shape[1] or W.shape[1 if kn else 2] != x.shape[2]:
-        raise ValueError(f"x {tuple(x.shape)} ([tokens, layers, features]) does not match W {tuple(W.shape)}")
     if torch.compiler.is_compiling():
         grad = torch.is_grad_enabled()
         return torch.ops.clt_hip.linear8(x, W, b, kn, grad and W.requires_grad, grad and x.requires_grad)[0]
@@ -227,8 +242,19 @@ def _product(a, b, K, c, dtype, ldc, bias, device, st):
           ws.data_ptr() if nws else None, nws, st)
 
 
+def _clt_check(feat, b, Ws):
+    """As _check: every W_l is addressed with its place in the features' layout."""
+    if feat.dim() != 3 or not Ws or len(Ws) != feat.shape[1] or any(W.dim() != 3 or tuple(W.shape) != (l + 1, feat.shape[2], Ws[0].shape[2]) for l, W in enumerate(Ws)):
+        raise ValueError(f"features {tuple(feat.shape)} do not match the decoder weights {[tuple(W.shape) for W in Ws]}")
+    if any(W.device != feat.device or W.dtype != Ws[0].dtype for W in Ws):
+        raise ValueError("the decoder weights are of one type, on the features' device")
+    if b is not None and (tuple(b.shape) != (len(Ws), Ws[0].shape[2]) or b.device != feat.device):
+        raise ValueError(f"bias {tuple(b.shape)} does not match {len(Ws)} layers of {Ws[0].shape[2]} on the features' device")
+
+
 def _clt_forward(feat, b, Ws, keep_x, keep_w):
     """-> recons [B, L, d], the kept tensors."""
+    _clt_check(feat, b, Ws)
     feat = ops8._dense(feat, (3,)).contiguous()
     B, L, F = feat.shape
     d = Ws[0].shape[2]
@@ -315,6 +341,7 @@ def _clt_decoder8_op(feat: Tensor, b: Optional[Tensor], Ws: List[Tensor], keep_x
 
 @_clt_decoder8_op.register_fake
 def _(feat, b, Ws, keep_x, keep_w):
+    _clt_check(feat, b, Ws)
     B, L, F = feat.shape
     d = Ws[0].shape[2]
     return [feat.new_empty(B, L, d)] + [feat.new_empty(shape, dtype=torch.uint8) for shape in _clt_kept_shapes(B, L, F, d, keep_x, keep_w)]
@@ -329,6 +356,7 @@ def _clt_decoder8_bwd(g: Tensor, kept: List[Tensor], F: int, has_x: bool, need_d
         raise ValueError("`kept` is not what clt_decoder8 kept for this gradient")
     if w_dtype is not None and not has_x:
         raise ValueError("the weights' gradient needs the features that clt_decoder8 keeps with keep_x")
+    _check_type(w_dtype)
     dx, dWs, db = _clt_gradients(g, kept, F, has_x, need_dx, [w_dtype] * L if w_dtype is not None else [], need_db)
     return [g.new_empty(0) if t is None else t for t in (dx, db)] + (dWs or [])
 
@@ -379,12 +407,6 @@ class _CltDecoder8(torch.autograd.Function):
 
 def clt_decoder8(feat: Tensor, b: Optional[Tensor], Ws: List[Tensor]) -> Tensor:
     """recons [B, L, d] from feat [B, L, F] and Ws[l] [l + 1, F, d], b [L, d] (`clt_hip::clt_decoder`'s arguments)."""
-    if feat.dim() != 3 or not Ws or len(Ws) != feat.shape[1] or any(W.dim() != 3 or tuple(W.shape) != (l + 1, feat.shape[2], Ws[0].shape[2]) for l, W in enumerate(Ws)):
-        raise ValueError(f"features {tuple(feat.shape)} do not match the decoder weights {[tuple(W.shape) for W in Ws]}")
-    if any(W.device != feat.device or W.dtype != Ws[0].dtype for W in Ws):
-        raise ValueError("the decoder weights are of one type, on the features' device")
-    if b is not None and tuple(b.shape) != (len(Ws), Ws[0].shape[2]):
-        raise ValueError(f"bias {tuple(b.shape)} does not match {len(Ws)} layers of {Ws[0].shape[2]}")
     if torch.compiler.is_compiling():
         grad = torch.is_grad_enabled()
         return torch.ops.clt_hip.clt_decoder8(feat, b, list(Ws), grad and any(W.requires_grad for W in Ws), grad and feat.requires_grad)[0]

@@ -60,3 +60,55 @@ def test_fp16_training_keeps_what_cancelling_products_leave():
     x = torch.zeros(300, 1, 256, dtype=torch.float16, device="cuda").requires_grad_()
     dx, = torch.autograd.grad(C.plt_decoder8(x, W, None), x, g)
     assert same(dx.transpose(0, 1), (g.transpose(0, 1).float() @ W.mT.contiguous()).cpu())
+
+
+# ---- calls of the registered ops with tensors that do not fit: refused before any address is taken --------------------------------
+def wrong_linear(t):
+    """(x, W, b, kn) that do not belong together; t makes a tensor of a shape."""
+    x = t(4, 2, 8)
+    return [(x, t(1, 8, 3), None, True), (x, t(3, 8, 3), None, True), (x, t(2, 7, 3), None, True), (x, t(2, 3, 7), None, False), (x, t(2, 8, 3), None, False),
+            (x, t(8, 3), None, True), (t(4, 8), t(2, 8, 3), None, True), (x, t(2, 8, 3), t(2, 4), True), (x, t(2, 8, 3), t(5), True), (x, t(2, 8, 3), t(3, 2), True)]
+
+
+def wrong_clt(t):
+    """(features, b, Ws): too many and too few matrices, one with more source layers, features or outputs than its place holds."""
+    f = t(4, 2, 8)
+    W = lambda *F: [t(l + 1, n, 3) for l, n in enumerate(F)]          # noqa: E731
+    return [(f, None, W(8, 8, 8)), (f, None, W(8)), (f, None, []), (f, None, W(8, 9)), (f, None, W(9, 8)), (f, None, W(9, 9)), (f, None, [t(2, 8, 3), t(2, 8, 3)]),
+            (f, None, [t(1, 8, 3), t(2, 8, 4)]), (f, None, [t(1, 8, 3), t(2, 24)]), (f, t(2, 4), W(8, 8)), (f, t(6), W(8, 8)), (t(4, 16), None, W(8, 8))]
+
+
+@pytest.mark.parametrize("device", ["meta", "cpu", pytest.param("cuda", marks=gpu)])
+def test_registered_ops_refuse_what_does_not_fit(device):
+    """meta: what a tracer asks; cpu: the functions that the ops' bodies call; cuda: the ops themselves."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    t = lambda *s: torch.zeros(*s, device=device)                      # noqa: E731
+    body = device == "cpu"
+    for x, W, b, kn in wrong_linear(t):
+        with pytest.raises(ValueError):
+            C._forward(x, W, b, kn, True, True) if body else torch.ops.clt_hip.linear8(x, W, b, kn, True, True)
+    for f, b, Ws in wrong_clt(t):
+        with pytest.raises(ValueError):
+            C._clt_forward(f, b, Ws, True, True) if body else torch.ops.clt_hip.clt_decoder8(f, b, Ws, True, True)
+    if device != "cpu":                                               # what fits passes
+        assert torch.ops.clt_hip.linear8(t(4, 2, 8), t(2, 8, 3), t(2, 3), True, True, True)[0].shape == (4, 2, 3)
+        assert torch.ops.clt_hip.linear8(t(4, 2, 8), t(2, 3, 8), t(6), False, True, True)[0].shape == (4, 2, 3)
+        assert torch.ops.clt_hip.clt_decoder8(t(4, 2, 8), t(2, 3), [t(1, 8, 3), t(2, 8, 3)], True, True)[0].shape == (4, 2, 3)
+
+
+@gpu
+def test_registered_ops_refuse_other_devices_and_types():
+    t = lambda *s, **k: torch.zeros(*s, **{"device": "cuda", **k})     # noqa: E731
+    ops = torch.ops.clt_hip
+    for args in ((t(4, 2, 8), t(2, 8, 3, device="cpu"), None), (t(4, 2, 8), t(2, 8, 3), t(2, 3, device="cpu")), (t(4, 2, 8), t(2, 8, 3, dtype=torch.float64), None)):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            ops.linear8(*args, True, True, True)
+    Ws = [t(1, 8, 3), t(2, 8, 3)]
+    for args in ((t(4, 2, 8), None, [Ws[0], Ws[1].cpu()]), (t(4, 2, 8), t(2, 3, device="cpu"), Ws), (t(4, 2, 8), None, [Ws[0], Ws[1].half()])):
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.clt_decoder8(*args, True, True)
+    kept, kepts = ops.linear8(t(4, 2, 8), t(2, 8, 3), None, True, True, True)[1], ops.clt_decoder8(t(4, 2, 8), None, Ws, True, True)[1:]
+    with pytest.raises(TypeError):
+        ops.linear8_bwd(t(4, 2, 3), kept, 8, True, True, True, torch.float64, False)
+    with pytest.raises(TypeError):
+        ops.clt_decoder8_bwd(t(4, 2, 3), kepts, 8, True, True, torch.float64, False)
