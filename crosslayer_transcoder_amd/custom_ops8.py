@@ -380,7 +380,8 @@ def _clt_backward(ctx, grads):
     if (need_w and not ctx.keep_x) or (need_x and not ctx.keep_w):
         raise RuntimeError("clt_decoder8 was called without keeping what this gradient needs (keep_x for dW, keep_w for the features')")
     dx, db, *dWs = torch.ops.clt_hip.clt_decoder8_bwd(grads[0], list(ctx.saved_tensors), ctx.F, ctx.keep_x, need_x, ctx.w_dtype if need_w else None, need_b)
-    return dx if need_x else None, db.to(ctx.b[0]).reshape(ctx.b[1]) if need_b else None, list(dWs) if need_w else None, None, None
+    # (a list argument's gradients are a list, of None where none is asked for)
+    return dx if need_x else None, db.to(ctx.b[0]).reshape(ctx.b[1]) if need_b else None, list(dWs) if need_w else [None] * grads[0].shape[1], None, None
 
 
 _clt_decoder8_op.register_autograd(_clt_backward, setup_context=_clt_setup)

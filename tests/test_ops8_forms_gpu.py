@@ -112,3 +112,22 @@ def test_registered_ops_refuse_other_devices_and_types():
         ops.linear8_bwd(t(4, 2, 3), kept, 8, True, True, True, torch.float64, False)
     with pytest.raises(TypeError):
         ops.clt_decoder8_bwd(t(4, 2, 3), kepts, 8, True, True, torch.float64, False)
+
+
+@gpu
+@pytest.mark.parametrize("F,d", [(128, 128), (40, 30)])
+def test_registered_cross_layer_decoder_with_some_gradients(F, d):
+    """The op that torch.compile captures: each gradient alone (kept weights among them) equals the one of the eager function."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    leaves = [torch.relu(rnd(20, 2, F, seed=1, spread=False)), rnd(2, d, seed=2, spread=False)] + [rnd(l + 1, F, d, seed=3 + l, spread=False) * 0.1 for l in range(2)]
+    g = rnd(20, 2, d, seed=9, spread=False)
+    for which in ([0], [1], [2], [3], [0, 1], [0, 3], [2, 3], [0, 1, 2, 3]):
+        got = []
+        for f in (C.clt_decoder8, lambda feat, b, Ws: torch.ops.clt_hip.clt_decoder8(feat, b, Ws, any(i > 1 for i in which), 0 in which)[0]):
+            t = [u.detach().clone().requires_grad_(i in which) for i, u in enumerate(leaves)]
+            got.append(torch.autograd.grad(f(t[0], t[1], t[2:]), [t[i] for i in which], g))
+        assert all(torch.equal(u, v) for u, v in zip(*got)), which
+    c = torch.compile(lambda feat, b, *Ws: C.clt_decoder8(feat, b, list(Ws)), backend="aot_eager")
+    feat = leaves[0].clone().requires_grad_()
+    want = torch.autograd.grad(C.clt_decoder8(feat, leaves[1], leaves[2:]), feat, g)[0]
+    assert torch.equal(torch.autograd.grad(c(feat, *leaves[1:]), feat, g)[0], want)
