@@ -143,9 +143,19 @@ def _backward(ctx, grads):
 linear8.register_autograd(_backward, setup_context=_setup)
 
 
+_PLAIN = (Tensor, torch.nn.Parameter)
+
+
+def _dispatched(*tensors):
+    """Whether a call has to be the registered op: something compiles, traces, transforms or watches what runs (none of them would see a
+    launch on an address), or a tensor is of a class with its own dispatch."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 or torch._C._get_tracing_state() is not None or
+            torch._C._functorch.peek_interpreter_stack() is not None or any(type(t) not in _PLAIN for t in tensors if t is not None))
+
+
 class _Linear8(torch.autograd.Function):
-    """The same two functions without the dispatcher's Python layers, for eager calls (a forward and backward of a few tokens:
-    400 us of host time through the registered ops)."""
+    """The same two functions without the dispatcher's Python layers, for eager calls that nothing watches (a forward and backward of
+    a few tokens: 400 us of host time through the registered ops)."""
 
     @staticmethod
     def forward(ctx, x, W, b, kn):
@@ -165,7 +175,7 @@ class _Linear8(torch.autograd.Function):
 
 
 def _linear(x, W, b, kn):
-    if torch.compiler.is_compiling():
+    if _dispatched(x, W, b):
         grad = torch.is_grad_enabled()
         return torch.ops.clt_hip.linear8(x, W, b, kn, grad and W.requires_grad, grad and x.requires_grad)[0]
     if not torch.is_grad_enabled():
@@ -408,7 +418,7 @@ class _CltDecoder8(torch.autograd.Function):
 
 def clt_decoder8(feat: Tensor, b: Optional[Tensor], Ws: List[Tensor]) -> Tensor:
     """recons [B, L, d] from feat [B, L, F] and Ws[l] [l + 1, F, d], b [L, d] (`clt_hip::clt_decoder`'s arguments)."""
-    if torch.compiler.is_compiling():
+    if _dispatched(feat, b, *Ws):
         grad = torch.is_grad_enabled()
         return torch.ops.clt_hip.clt_decoder8(feat, b, list(Ws), grad and any(W.requires_grad for W in Ws), grad and feat.requires_grad)[0]
     if not torch.is_grad_enabled():

@@ -4,8 +4,8 @@ weights, products of packed matrices, and the linear map of a few or many tokens
 A matrix [R, C] is held as 8-bit floats with one power-of-two scale for every row and block of 128 columns (`Block8`).
 Tensors may be fp32, bf16 or fp16, of any size (zero rows included) and with any strides as long as the last dimension is
 dense; everything runs on the tensors' device and on that device's current stream, allocates only through torch's caching
-allocator and can be captured into a graph.  Nothing here is differentiable: custom_ops8.py is.  Non-HIP tensors raise: there is
-no fallback."""
+allocator and can be captured into a graph.  Nothing here is differentiable or seen by a tracer (make_fx, torch.jit.trace: refused):
+custom_ops8.py is.  Non-HIP tensors raise: there is no fallback."""
 from __future__ import annotations
 
 import contextlib
@@ -26,7 +26,19 @@ def _up(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK * BLOCK
 
 
+_RECORDERS = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE, torch._C._TorchDispatchModeKey.FUNCTIONAL)
+
+
+def _recorded():
+    """Whether a tracer is taking down the calls around this one.  Inside the body of a registered op none is."""
+    return torch._C._get_tracing_state() is not None or (
+        torch._C._len_torch_dispatch_stack() > 0 and any(torch._C._get_dispatch_mode(k) is not None for k in _RECORDERS))
+
+
 def _call(fn, *args):
+    if _recorded():
+        raise RuntimeError(f"{fn.__name__}: a tracer does not see launches on addresses; trace the functions of custom_ops8 or the modules' forward, "
+                           "which are dispatcher ops")
     rc = fn(*args)
     if rc:
         raise CltError(fn.__name__, rc)

@@ -131,3 +131,99 @@ def test_registered_cross_layer_decoder_with_some_gradients(F, d):
     feat = leaves[0].clone().requires_grad_()
     want = torch.autograd.grad(C.clt_decoder8(feat, leaves[1], leaves[2:]), feat, g)[0]
     assert torch.equal(torch.autograd.grad(c(feat, *leaves[1:]), feat, g)[0], want)
+
+
+# ---- tracers and modes: the calls are dispatcher ops wherever something records them ---------------------------------------------
+class Seen(torch.utils._python_dispatch.TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+def tracing_cases(t):
+    """name -> (function of the inputs, inputs, the op it has to show)."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    W, b, Ws = t(2, 130, 70), t(2, 70), [t(1, 130, 70), t(2, 130, 70)]
+    enc = t(2, 70, 130).permute(0, 2, 1)
+    return {"plt_decoder8": (lambda x: C.plt_decoder8(x, W, b), t(40, 2, 130), "clt_hip.linear8"),
+            "encoder8": (lambda x: C.encoder8(x, enc, b), t(40, 2, 130), "clt_hip.linear8"),
+            "clt_decoder8": (lambda x: C.clt_decoder8(x, b, Ws), t(40, 2, 130), "clt_hip.clt_decoder8")}
+
+
+@pytest.mark.parametrize("name", ["plt_decoder8", "encoder8", "clt_decoder8"])
+def test_traced_calls_are_dispatcher_ops(name):
+    """With fake tensors, on the CPU: the graph holds the op, not the allocations around a launch."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    f, x, op = tracing_cases(lambda *s: torch.zeros(*s))[name]
+    with torch.no_grad():
+        code = make_fx(f, tracing_mode="fake", _allow_non_fake_inputs=True)(x).code
+    assert op in code, code
+
+
+@gpu
+@pytest.mark.parametrize("name", ["plt_decoder8", "encoder8", "clt_decoder8"])
+def test_traced_calls_equal_eager_ones(name):
+    """make_fx on real tensors, without and with gradients, and torch.jit.trace, run on other inputs; a dispatch mode sees the op."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    n = iter(range(100))
+    f, x, op = tracing_cases(lambda *s: rnd(*s, seed=next(n), spread=False))[name]
+    z = rnd(*x.shape, seed=50, spread=False)
+    with torch.no_grad():
+        want = f(z)
+        for traced in (make_fx(f)(x), torch.jit.trace(f, (x,), check_trace=False)):
+            assert torch.equal(traced(z), want)
+    with Seen() as mode:
+        assert torch.equal(f(z), want)
+    assert any(op in s for s in mode.names), mode.names
+
+    def both(x):
+        y = f(x)
+        return y.detach(), torch.autograd.grad(y.square().sum(), x)[0]
+
+    x, z = x.requires_grad_(), z.requires_grad_()
+    traced = make_fx(both)(x)
+    assert op + "_bwd" in traced.code
+    assert all(torch.equal(u, v) for u, v in zip(traced(z), both(z)))
+    assert torch.equal(torch.jit.trace(f, (x,), check_trace=False)(z), f(z))
+
+
+@gpu
+def test_traced_model_equals_the_eager_one():
+    import crosslayer_transcoder_amd as cta
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from crosslayer_transcoder_amd.model import CrosslayerDecoder, CrossLayerTranscoder, Encoder, ReLU
+    torch.manual_seed(0)
+    m = CrossLayerTranscoder(ReLU(), Encoder(96, 256, 2), CrosslayerDecoder(96, 256, 2)).cuda()
+    x, z = rnd(20, 2, 96, seed=1, spread=False), rnd(20, 2, 96, seed=2, spread=False)
+    with cta.contractions8(), torch.no_grad():
+        want = m(z)[2]
+        assert torch.equal(make_fx(lambda x: m(x)[2])(x)(z), want)
+
+
+@gpu
+def test_functions_of_ops8_refuse_tracers():
+    """They are no dispatcher ops: a trace would hold their allocations and nothing of what fills them."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from crosslayer_transcoder_amd import ops8
+    from crosslayer_transcoder_amd.model import Encoder
+    w = ops8.quantize8_weights(rnd(1, 70, 130, seed=1, spread=False))
+    q = ops8.quantize8(rnd(1, 9, 130, seed=2, spread=False))
+    enc = Encoder(130, 70, 1).cuda().requires_grad_(False)               # (torch.jit.trace takes no closed-over leaves)
+    packed = enc.pack8()
+    x = rnd(40, 130, seed=3, spread=False)
+    calls = [lambda x: ops8.linear8(x, w), lambda x: ops8.linear8(x[:3], w), lambda x: ops8.quantize8(x).data, lambda x: ops8.quantize8_t(x).data,
+             lambda x: ops8.quantize8_tiles(x)[0].data, lambda x: ops8.dequantize8(q) + x[0, 0], lambda x: ops8.gemm8(q, w) + x[0, 0],
+             lambda x: enc.forward_layer(x, 0, packed=packed)]
+    with torch.no_grad():
+        for f in calls:
+            want = f(x)
+            for trace in (lambda: make_fx(f)(x), lambda: torch.jit.trace(f, (x,), check_trace=False)):
+                with pytest.raises(RuntimeError, match="tracer"):
+                    trace()
+            with Seen():                                              # (a mode that only watches: nothing is recorded, nothing refused)
+                assert torch.equal(f(x), want)
+            assert torch.equal(torch.compile(f, backend="aot_eager")(x), want)
