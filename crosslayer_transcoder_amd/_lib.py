@@ -112,8 +112,10 @@ SIGNATURES = {
     "clt_pack8_into": (I, [P, I, L, L, I, I, I, I, I, P, P, L, L, L, P, P, L, L, L, P, P, SZ, P]),
     "clt_unpack8": (I, [P, P, I, I, I, I, L, L, L, L, P, I, P]),
     "clt_gemm8_workspace_bytes": (SZ, [I, I, I, I]),
+    "clt_gemm8_plan": (I, [I, I, I, I, I, L, P]),
     "clt_gemm8": (I, [P, P, I, L, L, L, L, P, P, I, L, L, L, L, P, I, L, L, P, L, I, I, I, I, I, P, SZ, P]),
     "clt_linear8_rows_workspace_bytes": (SZ, [I, I, I, I]),
+    "clt_linear8_rows_plan": (I, [I, I, I, I, P]),
     "clt_linear8_rows": (I, [P, I, L, L, P, P, I, L, L, L, L, P, L, P, I, L, L, I, I, I, I, P, SZ, P]),
     "clt_linear8_kept_bytes": (SZ, [I, I, I, I, I, I]),
     "clt_linear8_forward_workspace_bytes": (SZ, [I, I, I, I]),
@@ -122,7 +124,7 @@ SIGNATURES = {
     "clt_linear8_backward": (I, [P, I, L, L, P, I, I, I, I, I, I, P, P, I, P, P, SZ, P]),
 }
 
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 
 class CltError(RuntimeError):

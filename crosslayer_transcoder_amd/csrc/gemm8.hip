@@ -258,6 +258,13 @@ Plan plan_of(int M, int N, int KB, int batch, bool wide) {
     return best;
 }
 
+// of a call: where the rows of C lie further apart than the large form's 32-bit offsets reach, small tiles
+Plan plan_of_call(int M, int N, int KB, int batch, int c_dtype, long ldc) {
+    Plan p = plan_of(M, N, KB, batch, c_dtype != CLT_DT_BF16);
+    if (p.slices == 1 && 256 * ldc * 4 > 0x7fffffffL) p.large = 0;
+    return p;
+}
+
 template <int DT, int FA, int FB, int DEPTH> int launch_depth(const Gemm8Args& g, long blocks, hipStream_t st) {
     const auto f = gemm8_kernel<DT, FA, FB, DEPTH>;
     if (hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, DEPTH * STG) != hipSuccess) return CLT_ERR_LAUNCH;
@@ -290,6 +297,13 @@ extern "C" size_t clt_gemm8_workspace_bytes(int M, int N, int K, int batch) {
     return most > 1 ? (size_t)most * batch * M * N * 4 : 0;
 }
 
+extern "C" int clt_gemm8_plan(int M, int N, int K, int batch, int c_dtype, long ldc, int64_t* plan) {
+    if (M <= 0 || N <= 0 || K < 0 || batch <= 0 || c_dtype < 0 || c_dtype > 2 || ldc < N || !plan) return CLT_ERR_SHAPE;
+    const Plan p = plan_of_call(M, N, (int)(up128(K) / 128), batch, c_dtype, ldc);
+    plan[0] = ((M - 1) / 256 + 1L) * ((N - 1) / 256 + 1) * batch; plan[1] = p.large; plan[2] = p.slices;
+    return CLT_OK;
+}
+
 extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long ldas, long a_batch, long as_batch,
                          const void* b, const void* b_scale, int b_format, long ldb, long ldbs, long b_batch, long bs_batch,
                          void* c, int c_dtype, long ldc, long c_batch, const float* bias, long bias_batch, int M, int N, int K,
@@ -307,9 +321,7 @@ extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long 
                    static_cast<const uint8_t*>(b_scale), c, bias, lda, ldas, ldb, ldbs, ldc, a_batch, as_batch, b_batch, bs_batch,
                    c_batch, bias_batch, M, N, KB, (M - 1) / 128 + 1, (N - 1) / 128 + 1, accumulate, batch, 0u, 0u, 0u, 1, KB, nullptr, 0, 0};
     const hipStream_t st = as_stream(stream);
-    Plan plan = plan_of(M, N, KB, batch, c_dtype != CLT_DT_BF16);
-    // (results whose rows lie further apart than the large form's 32-bit offsets reach)
-    if (plan.slices == 1 && 256 * ldc * 4 > 0x7fffffffL) plan.large = 0;
+    const Plan plan = plan_of_call(M, N, KB, batch, c_dtype, ldc);
     g.slices = plan.slices;
     if (g.slices > 1) {
         if (!workspace || !aligned16(workspace) || workspace_bytes < (size_t)g.slices * batch * M * N * 4) return CLT_ERR_WORKSPACE;

@@ -247,6 +247,13 @@ extern "C" size_t clt_linear8_rows_workspace_bytes(int tokens, int layers, int N
     return c.slices > 1 ? (size_t)c.slices * layers * tokens * N * 4 : 0;
 }
 
+extern "C" int clt_linear8_rows_plan(int tokens, int layers, int N, int K, int64_t* plan) {
+    if (tokens <= 0 || tokens > MAX_T || layers <= 0 || N <= 0 || K <= 0 || !plan) return CLT_ERR_SHAPE;
+    const Cut c = cut_rows8(tokens, layers, N, (int)(up128(K) / 128));
+    plan[0] = c.slice_kb; plan[1] = c.slices; plan[2] = c.g; plan[3] = c.chunks; plan[4] = c.row_blocks;
+    return CLT_OK;
+}
+
 extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride, long x_layer_stride, const void* w, const void* w_scale,
                                 int w_format, long ldw, long ldws, long w_batch, long ws_batch, const float* bias, long bias_batch,
                                 void* y, int y_dtype, long y_token_stride, long y_layer_stride, int tokens, int layers, int N, int K,

@@ -565,6 +565,9 @@ int clt_unpack8(const void* q, const void* s, int format, int batch, int rows, i
  * CLT_ERR_RANGE).  C shares no memory with the operands, nor its rows with each other.  workspace (16-byte aligned): partial sums
  * where K is cut. */
 size_t clt_gemm8_workspace_bytes(int M, int N, int K, int batch);
+/* plan[3]: how clt_gemm8 would run (host only): 256 x 256 tiles that cover C, how many of them the large form computes (the rest, or all, are
+ * 128 x 128 ones), slices of K. */
+int clt_gemm8_plan(int M, int N, int K, int batch, int c_dtype, long ldc, int64_t* plan);
 int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long ldas, long a_batch, long as_batch,
               const void* b, const void* b_scale, int b_format, long ldb, long ldbs, long b_batch, long bs_batch,
               void* c, int c_dtype, long ldc, long c_batch, const float* bias, long bias_batch, int M, int N, int K, int batch,
@@ -572,6 +575,9 @@ int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long l
 /* y[t][l][:] = x[t][l][:] * w[l]^T + bias[l] for few tokens (at most 32; returns 1 for more: clt_pack8 + clt_gemm8), x packed on the
  * way (e4m3, blocks along K), exact products, fp32 sums.  x, y: unit stride in K / N, token and layer strides in elements. */
 size_t clt_linear8_rows_workspace_bytes(int tokens, int layers, int N, int K);
+/* plan[5]: how clt_linear8_rows would run (host only): blocks of 128 k a slice, slices, groups of 16 rows a wave holds, chunks of rows a
+ * block walks, blocks a layer and slice. */
+int clt_linear8_rows_plan(int tokens, int layers, int N, int K, int64_t* plan);
 int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride, long x_layer_stride, const void* w, const void* w_scale,
                      int w_format, long ldw, long ldws, long w_batch, long ws_batch, const float* bias, long bias_batch, void* y,
                      int y_dtype, long y_token_stride, long y_layer_stride, int tokens, int layers, int N, int K, void* workspace,

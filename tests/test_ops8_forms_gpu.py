@@ -227,3 +227,168 @@ def test_functions_of_ops8_refuse_tracers():
             with Seen():                                              # (a mode that only watches: nothing is recorded, nothing refused)
                 assert torch.equal(f(x), want)
             assert torch.equal(torch.compile(f, backend="aot_eager")(x), want)
+
+
+# ---- every form that the rules choose, asked of the rules themselves ------------------------------------------------------------------
+DT = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+FORMATS = [("e4m3", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e4m3"), ("e5m2", "e5m2")]
+
+
+def gemm_plan(L, M, K, N, out):
+    """-> (tiles of 256 x 256 that cover C, those the large form computes, slices of K)."""
+    import ctypes
+    from crosslayer_transcoder_amd._lib import lib
+    plan = (ctypes.c_int64 * 3)()
+    assert lib.clt_gemm8_plan(M, N, K, L, DT[out], N * L, plan) == 0
+    return tuple(plan)
+
+
+def rows_plan(T, L, K, N):
+    """-> (blocks of k a slice, slices, row groups in hand, chunks of rows a block walks, blocks)."""
+    import ctypes
+    from crosslayer_transcoder_amd._lib import lib
+    plan = (ctypes.c_int64 * 5)()
+    assert lib.clt_linear8_rows_plan(T, L, N, K, plan) == 0
+    return tuple(plan)
+
+
+def check_large(y, a, b, bias=None, base=None, exact=None):
+    """check_product's bounds with the 64-bit products on the GPU, a matrix at a time; fp16 results are exact up to the fp32 sums and one rounding."""
+    from crosslayer_transcoder_amd import ops8
+    fi = torch.finfo(y.dtype)
+    exact = y.dtype != torch.bfloat16 if exact is None else exact
+    for l in range(a.batch):
+        A, B = ops8.dequantize8(a.of_batch(l))[0].double(), ops8.dequantize8(b.of_batch(l))[0].double().T.contiguous()
+        ref, mag = A @ B, A.abs() @ B.abs()
+        if bias is not None:
+            ref, mag = ref + bias[l].double(), mag + bias[l].double().abs()
+        if base is not None:
+            ref, mag = ref + base[l].double(), mag + base[l].double().abs()
+        d = (y[l].double() - ref).abs()
+        lost = ((a.cols + 2) * 2.0 ** -23 if exact else 2.0 ** -9) * mag
+        # one rounding of the sum as computed: half a step of its magnitude, of the smallest normal number's below that
+        bound = lost if y.dtype == torch.float32 else lost + fi.eps / 2 * (ref.abs() + lost).clamp(min=fi.smallest_normal)
+        assert float((d - bound).max()) <= 0, float((d - bound).max())
+        # as a whole: fp32 sums of random sign stay below sqrt(K) 2^-23, aligned products below 2^-12, a rounding below half a step
+        tol = math.sqrt(a.cols + 2) * 2.0 ** -23 if exact else 2.0 ** -12
+        if y.dtype != torch.float32:
+            tol += fi.eps / 2
+        assert float(d.norm()) <= tol * float(ref.norm()) + 1e-30
+        del A, B, ref, mag, d, bound
+
+
+#: (L, M, K, N): whole and partial tiles; 1, 2 and 3 blocks of k, over which the staging of the next tiles runs ahead; many of them; slices;
+#: a rest of small tiles
+LARGE_FORMS = [(1, 4096, 128, 12288), (1, 4000, 100, 12201), (1, 4096, 256, 12288), (1, 4000, 300, 12201), (1, 4096, 4096, 12288), (1, 4000, 4100, 12201),
+               (1, 800, 24576, 1900), (1, 4100, 4100, 4500)]
+
+
+@gpu
+@pytest.mark.parametrize("formats", FORMATS)
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", LARGE_FORMS)
+def test_large_form(shape, out, formats):
+    """Three tiles and more a block of the large form, for every type of results and pair of formats, with a bias and added to."""
+    from crosslayer_transcoder_amd import ops8
+    L, M, K, N = shape
+    tiles, large, slices = gemm_plan(L, M, K, N, out)
+    if K == 24576:
+        assert large == tiles and slices > 1
+    elif (M, K) == (4100, 4100):
+        assert 0 < large < tiles and slices == 1
+    else:
+        assert large == tiles >= 768 and slices == 1
+    a = ops8.quantize8(rnd(L, M, K, seed=1, spread=False), formats[0])
+    b = ops8.quantize8(rnd(L, N, K, seed=2, spread=False), formats[1])
+    bias = rnd(L, N, seed=3, spread=False)
+    y = ops8.gemm8(a, b, bias, out_dtype=out)
+    check_large(y, a, b, bias)
+    if out == torch.float32:
+        z = y.clone()
+        ops8.gemm8(a, b, out=z, accumulate=True)
+        check_large(z, a, b, base=y)
+    assert torch.equal(y, ops8.gemm8(a, b, bias, out_dtype=out))                 # (the order of the sums is fixed)
+
+
+@gpu
+@pytest.mark.parametrize("formats", FORMATS)
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape,sliced,many", [((3, 500, 300, 901), False, False), ((1, 100, 9000, 130), True, False), ((33, 300, 640, 515), False, True)])
+def test_small_form(shape, sliced, many, out, formats):
+    """Up to 256 tiles (one a CU), K in slices, more than 256 (two a CU)."""
+    from crosslayer_transcoder_amd import ops8
+    L, M, K, N = shape
+    tiles, large, slices = gemm_plan(L, M, K, N, out)
+    assert large == 0 and (slices > 1) == sliced and (-(-M // 128) * -(-N // 128) * L * slices > 256) == many, (tiles, large, slices)
+    a, b = ops8.quantize8(rnd(L, M, K, seed=1, spread=False), formats[0]), ops8.quantize8(rnd(L, N, K, seed=2, spread=False), formats[1])
+    bias = rnd(L, N, seed=3, spread=False)
+    check_large(ops8.gemm8(a, b, bias, out_dtype=out), a, b, bias)
+
+
+@gpu
+def test_weight_gradient_of_a_short_batch():
+    """Up to 128 tokens: one block of k, enough tiles for the large form."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    from crosslayer_transcoder_amd import ops8
+    T, K, N = 70, 4096, 8192
+    assert gemm_plan(1, K, T, N, torch.float32) == (512, 512, 1)
+    x, W, dy = rnd(T, 1, K, seed=1, spread=False), (rnd(1, K, N, seed=2, spread=False) * 0.01).requires_grad_(), rnd(T, 1, N, seed=3, spread=False)
+    dW, = torch.autograd.grad(C.plt_decoder8(x, W, None), W, dy)
+    check_large(dW, ops8.quantize8_t(x.transpose(0, 1)), ops8.quantize8_t(dy.transpose(0, 1)))
+
+
+#: (T, L, K, N) -> what the rule has to choose for them (blocks of k a slice >=, slices > 1, groups in hand, chunks > 1)
+ROWS_FORMS = [((20, 12, 130, 32001), (1, False, 1, True)),       # 17 .. 32 tokens: blocks that walk several chunks of rows, the last one ragged
+              ((32, 3, 130, 66001), (1, False, 1, True)),
+              ((3, 12, 130, 50001), (1, False, 2, True)),        # up to 16 tokens: two row groups, several chunks
+              ((9, 5, 1200, 130000), (10, False, 2, True)),      # the same with long rows
+              ((32, 1, 9000, 200), (5, True, 1, False)),         # slices of 32 tokens
+              ((17, 2, 20000, 33), (6, True, 1, False)),
+              ((24, 12, 1300, 12345), (11, False, 1, True)),     # long slices of 17 .. 32 tokens: the loop in steps, one block a CU
+              ((17, 12, 1500, 20001), (12, False, 1, True)),
+              ((32, 4, 2000, 20000), (8, True, 1, True)),        # slices and chunks
+              ((1, 4, 70000, 1000), (60, True, 1, False)),
+              ((16, 1, 768, 1000), (6, False, 1, False))]
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+@pytest.mark.parametrize("shape,form", ROWS_FORMS)
+def test_few_token_forms(shape, form, fmt):
+    from crosslayer_transcoder_amd import ops8
+    T, L, K, N = shape
+    slice_kb, slices, g, chunks, _ = rows_plan(T, L, K, N)
+    assert slice_kb >= form[0] and (slices > 1, g, chunks > 1) == form[1:], (slice_kb, slices, g, chunks)
+    x, bias = rnd(T, L, K, seed=1, spread=False), rnd(L, N, seed=3, spread=False)
+    w = ops8.quantize8(rnd(L, N, K, seed=2, spread=False), fmt)
+    y = ops8.linear8(x, w, bias)
+    check_large(y.transpose(0, 1), ops8.quantize8(x.transpose(0, 1)), w, bias)
+    z = ops8.linear8(x.half(), w, bias)
+    check_large(z.transpose(0, 1), ops8.quantize8(x.half().transpose(0, 1)), w, bias)
+    z = ops8.linear8(x.bfloat16(), w)
+    check_large(z.transpose(0, 1), ops8.quantize8(x.bfloat16().transpose(0, 1)), w, exact=True)
+    assert torch.equal(y, ops8.linear8(x, w, bias))
+
+
+@gpu
+@pytest.mark.parametrize("K,slices", [(301, False), (9000, True)])
+def test_a_token_does_not_depend_on_its_batch(K, slices):
+    """Each of 27 tokens by itself, against 64 bits (test_ops8_gpu.py compares only within a few percent); to the bit where neither call cuts K:
+    the same products in the same order."""
+    from crosslayer_transcoder_amd import ops8
+    x, w = rnd(27, 2, K, seed=1, spread=False), ops8.quantize8_weights(rnd(2, 70, K, seed=2, spread=False))
+    assert (rows_plan(27, 2, K, 70)[1] > 1) == slices and (rows_plan(1, 2, K, 70)[1] > 1) == slices
+    y, one = ops8.linear8(x, w), torch.cat([ops8.linear8(x[t:t + 1], w) for t in range(27)])
+    check_large(one.transpose(0, 1), ops8.quantize8(x.transpose(0, 1)), w)
+    assert slices or torch.equal(one, y)
+
+
+def test_plans_are_refused_for_no_sizes():
+    import ctypes
+    from crosslayer_transcoder_amd._lib import lib
+    p = (ctypes.c_int64 * 5)()
+    assert [lib.clt_gemm8_plan(0, 1, 1, 1, 0, 1, p), lib.clt_gemm8_plan(1, 2, 1, 1, 0, 1, p), lib.clt_gemm8_plan(1, 1, 1, 1, 3, 1, p), lib.clt_gemm8_plan(1, 1, 1, 1, 0, 1, None)] == [-1] * 4
+    assert [lib.clt_linear8_rows_plan(0, 1, 1, 1, p), lib.clt_linear8_rows_plan(33, 1, 1, 1, p), lib.clt_linear8_rows_plan(1, 1, 1, 1, None)] == [-1] * 3
+    # results whose rows lie more than 2^21 elements apart: small tiles
+    assert lib.clt_gemm8_plan(4096, 12288, 4096, 1, 0, 12288, p) == 0 and p[1] == 768
+    assert lib.clt_gemm8_plan(4096, 12288, 4096, 1, 0, 1 << 22, p) == 0 and p[1] == 0
