@@ -9,7 +9,10 @@
 #include "common.h"
 
 constexpr int B8 = 128;                              // block: columns that share a scale
-constexpr int B8_MIN_EXP = -112;                     // smallest scale exponent: 2^-e and code x 2^e stay normal fp32 numbers
+constexpr int B8_MIN_EXP = -112;                     // smallest scale exponent: 2^-e stays a normal fp32 number, and code x 2^e one of e4m3
+// (e5m2's smallest codes, 2^-16 .. 3 x 2^-16, are subnormal numbers there, in fp32 and bf16: exact as long as subnormals are kept, which
+// the conversions and the bf16 matrix instructions do; tested.)  At the other end 1.9375 x 2^127 (e5m2: 1.875) and more rounds to code x 2^e =
+// 2^128, an infinity in fp32 and bf16.
 
 __host__ __device__ static inline long up128(long n) { return (n + 127) / 128 * 128; }
 

@@ -75,8 +75,9 @@ def _dense(x: torch.Tensor, dims=(2, 3)) -> torch.Tensor:
 class Block8:
     """A batch of matrices [L, rows, cols] in 8 bits.  data: uint8 [L, rows, >= cols rounded up to 128], rows 16-byte aligned,
     codes of `fmt` ("e4m3" / "e5m2"), ZERO behind column `cols` up to the next multiple of 128; scale: uint8 [L, >= blocks of 128
-    columns, >= rows], rows 4-byte aligned, byte e + 127 (1 to 254) for the scale 2^e of a row's block.  The pack functions below make it; one may be built
-    from kept tensors (a checkpoint of packed weights) as well."""
+    columns, >= rows], rows 4-byte aligned, byte e + 127 for the scale 2^e of a row's block.  The pack functions below make it; one may be
+    built from kept tensors (a checkpoint of packed weights) as well, with e from -112 to 119 (e5m2: 112): there 2^e x code is exact in bf16,
+    which products of fp32 or fp16 results and of few tokens rest on."""
     __slots__ = ("data", "scale", "rows", "cols", "fmt")
 
     def __init__(self, data: torch.Tensor, scale: torch.Tensor, rows: int, cols: int, fmt: str = "e4m3"):

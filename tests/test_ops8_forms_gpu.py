@@ -392,3 +392,45 @@ def test_plans_are_refused_for_no_sizes():
     # results whose rows lie more than 2^21 elements apart: small tiles
     assert lib.clt_gemm8_plan(4096, 12288, 4096, 1, 0, 12288, p) == 0 and p[1] == 768
     assert lib.clt_gemm8_plan(4096, 12288, 4096, 1, 0, 1 << 22, p) == 0 and p[1] == 0
+
+
+# ---- the ends of the scales' range -----------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("shape", [(40, 300, 70), (1, 300, 70), (100, 9000, 130), (4096, 200, 8192)])
+def test_smallest_codes_take_part_in_products(shape):
+    """e5m2 at the smallest exponent: codes of 1 to 3 times 2^-16 times 2^-112, subnormal numbers in bf16 and fp32, against weights of 2^110: whole
+    multiples of 2^-18, exact for every type of results."""
+    from crosslayer_transcoder_amd import ops8
+    M, K, N = shape
+    g = torch.Generator().manual_seed(0)
+    few = torch.rand(K, generator=g) < 300 / K                                   # (sums stay below 2^8 in bf16, 2^11 in fp16)
+    i = torch.randint(-1, 2, (M, K), generator=g).float() * few
+    i[:, ::7] *= 3
+    w = torch.randint(-1, 2, (N, K), generator=g).float() * (torch.rand(K, generator=g) < 0.3)
+    a, b = ops8.quantize8((i.double() * 2.0 ** -128).float().cuda(), "e5m2"), ops8.quantize8((w * 2.0 ** 110).cuda(), "e5m2")
+    assert bool((a.scale == 15).all()) and same(ops8.dequantize8(a)[0], i.double() * 2.0 ** -128)
+    ref = i.cuda() @ w.cuda().T.contiguous()                                     # (whole numbers)
+    assert float(ref.abs().max()) <= 256
+    for out in (torch.float32, torch.bfloat16, torch.float16):
+        assert same(ops8.gemm8(a, b, out_dtype=out)[0], ref.cpu().double() * 2.0 ** -18), out
+    x = (w[:M] if M <= N else w[:1].expand(M, K)) * 2.0 ** 110                   # the other way round: kept weights that are tiny
+    want = x.cuda().div(2.0 ** 110) @ i.cuda().T.contiguous()
+    assert same(ops8.linear8(x.cuda(), a), want.cpu().double() * 2.0 ** -18)
+
+
+@gpu
+def test_largest_numbers():
+    """Up to the last magnitude that rounds down, values are finite and products exact; above it they are held as 2^128 and restored as infinities."""
+    from crosslayer_transcoder_amd import ops8
+    for fmt, below, held in (("e4m3", 1.9375 - 2.0 ** -23, 1.875), ("e5m2", 1.875 - 2.0 ** -23, 1.75)):
+        x = torch.zeros(40, 128)
+        x[:, 5], x[1, 5] = below * 2.0 ** 127, -below * 2.0 ** 127
+        q = ops8.quantize8(x.cuda(), fmt)
+        assert float(ops8.dequantize8(q)[0, 0, 5]) == held * 2.0 ** 127
+        w = ops8.quantize8(torch.full((40, 128), 2.0 ** -120).cuda())
+        for out in (torch.float32, torch.bfloat16, torch.float16):
+            y = ops8.gemm8(q, w, out_dtype=out)[0]
+            assert bool((y[0] == held * 128).all()) and bool((y[1] == -held * 128).all()), (fmt, out)
+    x[0, 5] = torch.finfo(torch.float32).max
+    for fmt in ("e4m3", "e5m2"):
+        assert float(ops8.dequantize8(ops8.quantize8(x.cuda(), fmt))[0, 0, 5]) == math.inf
