@@ -259,7 +259,7 @@ extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride,
                                 void* y, int y_dtype, long y_token_stride, long y_layer_stride, int tokens, int layers, int N, int K,
                                 void* workspace, size_t workspace_bytes, void* stream) {
     if (tokens <= 0 || layers <= 0 || N <= 0 || K <= 0 || x_dtype < 0 || x_dtype > 2 || y_dtype < 0 || y_dtype > 2 || (w_format & ~1)) return CLT_ERR_SHAPE;
-    if (tokens > MAX_T) return 1;                                        // the many-token form: clt_pack8 + clt_gemm8
+    if (tokens > MAX_T) return CLT_ERR_RANGE;                            // (more are clt_pack8's and clt_gemm8's)
     if (!x || !w || !w_scale || !y || ldw < up128(K) || ldws < N) return CLT_ERR_SHAPE;
     const size_t xs = x_dtype == CLT_DT_F32 ? 4 : 2, ys = y_dtype == CLT_DT_F32 ? 4 : 2;
     if (!aligned16(w) || ldw % 16 || w_batch % 16 || ((uintptr_t)x & (xs - 1)) || ((uintptr_t)y & (ys - 1)) || ((uintptr_t)bias & 3)) return CLT_ERR_ALIGN;

@@ -573,7 +573,7 @@ int clt_gemm8(const void* a, const void* a_scale, int a_format, long lda, long l
               const void* b, const void* b_scale, int b_format, long ldb, long ldbs, long b_batch, long bs_batch,
               void* c, int c_dtype, long ldc, long c_batch, const float* bias, long bias_batch, int M, int N, int K, int batch,
               int accumulate, void* workspace, size_t workspace_bytes, void* stream);
-/* y[t][l][:] = x[t][l][:] * w[l]^T + bias[l] for few tokens (at most 32; returns 1 for more: clt_pack8 + clt_gemm8), x packed on the
+/* y[t][l][:] = x[t][l][:] * w[l]^T + bias[l] for few tokens (at most 32, else CLT_ERR_RANGE: clt_pack8 + clt_gemm8), x packed on the
  * way (e4m3, blocks along K), exact products, fp32 sums.  x, y: unit stride in K / N, token and layer strides in elements. */
 size_t clt_linear8_rows_workspace_bytes(int tokens, int layers, int N, int K);
 /* plan[5]: how clt_linear8_rows would run (host only): blocks of 128 k a slice, slices, groups of 16 rows a wave holds, chunks of rows a

@@ -434,3 +434,16 @@ def test_largest_numbers():
     x[0, 5] = torch.finfo(torch.float32).max
     for fmt in ("e4m3", "e5m2"):
         assert float(ops8.dequantize8(ops8.quantize8(x.cuda(), fmt))[0, 0, 5]) == math.inf
+
+
+def test_refusals_of_the_few_token_call():
+    from crosslayer_transcoder_amd._lib import lib
+    p = 4096                                                                     # an aligned address nothing reads
+
+    def rows(x=p, dt=0, w=p, ws=p, ldw=128, ldws=128, y=p, T=4, L=1, N=40, K=100, bias=None, buf=None, n=0):
+        return lib.clt_linear8_rows(x, dt, 100, 0, w, ws, 0, ldw, ldws, 0, 0, bias, 0, y, 0, N, 0, T, L, N, K, buf, n, None)
+
+    assert [rows(T=0), rows(L=0), rows(N=0), rows(K=0), rows(dt=3), rows(x=None), rows(w=None), rows(ws=None), rows(y=None), rows(ldw=112), rows(ldws=39)] == [-1] * 11
+    assert [rows(x=p + 2), rows(w=p + 8), rows(ldw=136), rows(y=p + 1), rows(bias=p + 2)] == [-4] * 5
+    assert rows(T=33) == -6                                                      # an error like any other, not a code of its own
+    assert rows(K=40000, ldw=40064, N=40) == -3 and rows(K=40000, ldw=40064, N=40, buf=p, n=16) == -3
