@@ -447,3 +447,116 @@ def test_refusals_of_the_few_token_call():
     assert [rows(x=p + 2), rows(w=p + 8), rows(ldw=136), rows(y=p + 1), rows(bias=p + 2)] == [-4] * 5
     assert rows(T=33) == -6                                                      # an error like any other, not a code of its own
     assert rows(K=40000, ldw=40064, N=40) == -3 and rows(K=40000, ldw=40064, N=40, buf=p, n=16) == -3
+
+
+# ---- the operators together, as a program uses them ---------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("tokens", [1, 5, 40])
+def test_serving_chain_on_packed_weights(tokens):
+    """Encoder layer by layer -> every sparsifier -> both decoders on kept weights, each stage on what the one before it gave (fp32, which the
+    sparsifiers take)."""
+    from crosslayer_transcoder_amd import ops8
+    from crosslayer_transcoder_amd.model import BatchTopK, CrosslayerDecoder, Decoder, Encoder, PerLayerBatchTopK, PerLayerTopK, ReLU
+    L, d, F = 3, 96, 256
+    torch.manual_seed(3)
+    enc, clt, plt = Encoder(d, F, L).cuda(), CrosslayerDecoder(d, F, L).cuda(), Decoder(d, F, L).cuda()
+    pe, pc, pp = enc.pack8(), clt.pack8(), plt.pack8()
+    x = rnd(1, tokens, L, d, seed=4, spread=False)
+    for sparsifier in (ReLU(), PerLayerTopK(k=8), BatchTopK(k=8, e=0.1), PerLayerBatchTopK(k=8, e=0.1, n_layers=L)):
+        feats = []
+        for l in range(L):
+            pre = enc.forward_layer(x[:, :, l], l, packed=pe)
+            feats.append(sparsifier.cuda()(pre, l))
+            assert feats[-1].shape == (1, tokens, F) and feats[-1].dtype == torch.float32
+            stack = torch.stack(feats, 2)
+            y = clt.forward_layer(stack, l, packed=pc)
+            check_large(y, ops8.quantize8(stack.reshape(1, tokens, -1)), pc[l], clt.b[l:l + 1])
+        y = plt.forward_layer(stack, 1, packed=pp)
+        check_large(y, ops8.quantize8(stack[:, :, 1]), pp.of_batch(1), plt.b[1:2])
+
+
+@gpu
+@pytest.mark.parametrize("F,d", [(256, 128), (200, 96)])
+def test_captured_cross_layer_step_equals_eager_on_every_replay(F, d):
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    L, B = 3, 140
+    feat, b, g = torch.relu(rnd(B, L, F, seed=1)).requires_grad_(), rnd(L, d, seed=2).requires_grad_(), rnd(B, L, d, seed=3)
+    Ws = [rnd(l + 1, F, d, seed=4 + l, spread=False).requires_grad_() for l in range(L)]
+
+    def step():
+        y = C.clt_decoder8(feat, b, Ws)
+        return [y] + list(torch.autograd.grad(y, [feat, b] + Ws, g))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        with torch.no_grad():
+            feat.copy_(torch.relu(rnd(B, L, F, seed=10 + k))), g.copy_(rnd(B, L, d, seed=20 + k)), Ws[1].mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.detach().clone() for o in out]
+        assert all(torch.equal(u, v) for u, v in zip(got, step())), k
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_of_16_bits(dtype):
+    """Weights and biases in 16 bits: gradients in their types, each rounded once (bf16 ones from aligned products)."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    T, L, K, N = 150, 2, 256, 128
+    x, dy = rnd(T, L, K, seed=1, spread=False).requires_grad_(), rnd(T, L, N, seed=2, spread=False)
+    W, b = rnd(L, K, N, seed=3, dtype=dtype, spread=False).requires_grad_(), rnd(L, N, seed=4, dtype=dtype, spread=False).requires_grad_()
+    y = C.plt_decoder8(x, W, b)
+    dx, dW, db = torch.autograd.grad(y, (x, W, b), dy)
+    assert (y.dtype, dx.dtype, dW.dtype, db.dtype) == (torch.float32, torch.float32, dtype, dtype)
+    ref, t = reference_training(x, W, b, dy, True), torch.finfo(dtype).eps / 2 + 2.0 ** -12
+    close(y.detach(), ref[0], 2.0 ** -18), close(dx, ref[1], 2.0 ** -18), close(dW, ref[2], t), close(db, ref[3], t)
+    feat, Ws = torch.relu(x.detach()).requires_grad_(), [rnd(l + 1, K, N, seed=5 + l, dtype=dtype, spread=False).requires_grad_() for l in range(L)]
+    y = C.clt_decoder8(feat, b, Ws)
+    grads, ref = torch.autograd.grad(y, [feat, b] + Ws, dy), reference_clt(feat, Ws, b, dy)
+    close(grads[0], ref[1], 2.0 ** -18), close(grads[1], ref[2], t)
+    for dW, want in zip(grads[2:], ref[3:]):
+        assert dW.dtype == dtype
+        close(dW, want, t)
+
+
+@gpu
+@pytest.mark.parametrize("F,d", [(256, 128), (200, 96)])
+def test_cross_layer_decoder_of_views(F, d):
+    """Weights cut out of wider buffers, transposed ones, features and gradients with other strides: the bits of dense tensors."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    L, B = 3, 40
+    feat, g = torch.relu(rnd(L, B, F + 5, seed=1, spread=False)), rnd(B, d, L, seed=2, spread=False)
+    wide = [rnd(l + 2, F + 3, d + 7, seed=4 + l, spread=False) for l in range(L)]
+    views = [wide[0][1:, 2:F + 2, 3:d + 3], wide[1][:2, :F, :d], rnd(3, d, F, seed=9, spread=False).mT]
+    f, h = feat[:, :, 1:F + 1].transpose(0, 1), g.transpose(1, 2)
+    got = []
+    for dense in (False, True):
+        t = [(u.contiguous() if dense else u).detach().requires_grad_() for u in (f, *views)]
+        y = C.clt_decoder8(t[0], None, t[1:])
+        got.append([y] + list(torch.autograd.grad(y, t, h.contiguous() if dense else h)))
+    assert all(torch.equal(u, v) for u, v in zip(*got))
+
+
+@gpu
+def test_the_same_tensor_twice_and_a_stream_of_its_own():
+    """One leaf in two calls of one step, on a stream that is not the current one at the time of the backward pass."""
+    from crosslayer_transcoder_amd import custom_ops8 as C
+    x, W = rnd(70, 2, 128, seed=1, spread=False).requires_grad_(), rnd(2, 128, 128, seed=2, spread=False).requires_grad_()
+    want = [2 * g for g in torch.autograd.grad(C.plt_decoder8(x, W, None).sum(), (x, W))]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        loss = C.plt_decoder8(x, W, None).sum() + C.plt_decoder8(x, W, None).sum()
+    torch.cuda.current_stream().wait_stream(s)
+    got = torch.autograd.grad(loss, (x, W))
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in zip(got, want))
