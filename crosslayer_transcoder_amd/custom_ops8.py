@@ -35,27 +35,25 @@ def _bytes(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def _check(x, W, b, kn):
-    """Refuses what does not fit: the kernels take x's sizes for W's (the op's body, its fake and the eager functions all come here)."""
-    if x.dim() != 3 or W.dim() != 3 or W.shape[0] != x.shape[1] or W.shape[1 if kn else 2] != x.shape[2]:
-        raise ValueError(f"x {tuple(x.shape)} ([tokens, layers, features]) does not match W {tuple(W.shape)}")
-    N = W.shape[2 if kn else 1]
-    if b is not None and (b.numel() != W.shape[0] * N or (b.dim() > 1 and tuple(b.shape) != (W.shape[0], N))):
-        raise ValueError(f"bias {tuple(b.shape)} does not match {W.shape[0]} layers of {N}")
-    if W.device != x.device or (b is not None and b.device != x.device):
-        raise ValueError("x, W and the bias are on different devices")
+def _check(x, W, kn):
+    """Refuses what does not fit: the kernels take x's sizes for W's.  The op's body, its fake and the eager functions all come here
+    (ops8._bias: the bias) -> T, L, K, N."""
+    sx, sw = x.shape, W.shape
+    if len(sx) != 3 or len(sw) != 3 or sw[0] != sx[1] or sw[1 if kn else 2] != sx[2]:
+        raise ValueError(f"x {tuple(sx)} ([tokens, layers, features]) does not match W {tuple(sw)}")
+    if W.device != x.device:
+        raise ValueError("x and W are on different devices")
+    return (*sx, sw[2 if kn else 1])
 
 
 def _forward(x, W, b, kn, keep_x, keep_w):
     """x [T, L, K], W [L, N, K] (kn: [L, K, N]) -> y [T, L, N], the kept buffer."""
-    _check(x, W, b, kn)
+    T, L, K, N = _check(x, W, kn)
+    b = ops8._bias(b, L, N, x.device)
     x, W = ops8._dense(x, (3,)), ops8._dense(W, (3,))
-    T, L, K = x.shape
-    N = W.shape[2] if kn else W.shape[1]
     dev = x.device
     if not (L and K and N):
         raise ValueError(f"empty map: x {tuple(x.shape)}, W {tuple(W.shape)}")
-    b = ops8._bias(b, L, N, dev)
     y = torch.empty((T, L, N), dtype=x.dtype, device=dev)
     kept = _bytes(lib.clt_linear8_kept_bytes(T, L, K, N, keep_x, keep_w), dev)
     nws = lib.clt_linear8_forward_workspace_bytes(T, L, K, N)
@@ -96,9 +94,8 @@ def linear8(x: Tensor, W: Tensor, b: Optional[Tensor], kn: bool, keep_x: bool, k
 
 @linear8.register_fake
 def _(x, W, b, kn, keep_x, keep_w):
-    _check(x, W, b, kn)
-    T, L, K = x.shape
-    N = W.shape[2] if kn else W.shape[1]
+    T, L, K, N = _check(x, W, kn)
+    ops8._bias(b, L, N, x.device)
     return [x.new_empty(T, L, N), x.new_empty(_kept_bytes(T, L, K, N, keep_x, keep_w), dtype=torch.uint8)]
 
 
@@ -143,14 +140,15 @@ def _backward(ctx, grads):
 linear8.register_autograd(_backward, setup_context=_setup)
 
 
-_PLAIN = (Tensor, torch.nn.Parameter)
+_PLAIN = frozenset((Tensor, torch.nn.Parameter, type(None)))
+_transforms = torch._C._functorch.peek_interpreter_stack
 
 
 def _dispatched(*tensors):
     """Whether a call has to be the registered op: something compiles, traces, transforms or watches what runs (none of them would see a
     launch on an address), or a tensor is of a class with its own dispatch."""
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0 or torch._C._get_tracing_state() is not None or
-            torch._C._functorch.peek_interpreter_stack() is not None or any(type(t) not in _PLAIN for t in tensors if t is not None))
+    return (torch.compiler.is_compiling() or ops8._modes() > 0 or ops8._tracing() is not None or _transforms() is not None or
+            not _PLAIN.issuperset(map(type, tensors)))
 
 
 class _Linear8(torch.autograd.Function):

@@ -26,13 +26,13 @@ def _up(n: int) -> int:
     return (n + BLOCK - 1) // BLOCK * BLOCK
 
 
+_tracing, _modes = torch._C._get_tracing_state, torch._C._len_torch_dispatch_stack
 _RECORDERS = (torch._C._TorchDispatchModeKey.PROXY, torch._C._TorchDispatchModeKey.FAKE, torch._C._TorchDispatchModeKey.FUNCTIONAL)
 
 
 def _recorded():
     """Whether a tracer is taking down the calls around this one.  Inside the body of a registered op none is."""
-    return torch._C._get_tracing_state() is not None or (
-        torch._C._len_torch_dispatch_stack() > 0 and any(torch._C._get_dispatch_mode(k) is not None for k in _RECORDERS))
+    return _tracing() is not None or (_modes() > 0 and any(torch._C._get_dispatch_mode(k) is not None for k in _RECORDERS))
 
 
 def _call(fn, *args):
