@@ -16,9 +16,10 @@
 // lanes make 64 / 128 consecutive bytes.  bf16 results pass through a 4 KB slab of LDS a wave, so that 256 bytes of a row leave
 // together, and past the caches, which hold the operands' panels (4096 x 768 x 32768 x 12: 1728 -> 1462 us; without the slab the
 // uncached stores are slower than cached ones, 1765 us).
-// Bound: the matrix units, at what clock the power leaves them (8192^3: 390 .. 437 us from card to card = 2.5 .. 2.8 PFLOP/s; the large library
-// product in 8 bits 2.9); with a short contraction the stores next to them (K = 768, 12 layers, 3.2 GB of results: 1430 us; 1600 us where
-// the rows of a layer lie 786 KB apart).
+// Bound: the matrix units, at what clock the power leaves them (8192^3: 373 .. 437 us from card to card = 2.5 .. 2.9 PFLOP/s; the large library
+// product in 8 bits 2.9); with a short contraction the stores next to them (K = 768, 12 layers, 3.2 GB of results: 1410 .. 1440 us; 1530 us
+// where the rows of a layer lie 786 KB apart; matrix units busy 35 % of the time).  Those are times of a row of launches; the first few of a
+// process take 1.6 .. 1.9 ms.
 #include <type_traits>
 #include "block8_common.h"
 
@@ -253,7 +254,8 @@ __global__ __launch_bounds__(256, 1) void gemm8_large_kernel(Gemm8Args g, int to
 // ---- exact products (fp32 and fp16 results): the codes become bf16 in registers and the products run at the 16-bit rate, so a block of k costs twice the
 // cycles for the same LDS bytes: 8 waves of 128 x 64 (B x A; 192 KB of reads in 4096 cycles), two per SIMD, whose conversions run
 // under each other's matrix instructions.  Tiles, DMA, row order and the stream of blocks as above; A fragments are 4 rows of a
-// 64-row group (row 4 * lane + n).  8192^3: 795 .. 825 us = 1.33 .. 1.38 PFLOP/s, the rate of the large library product in bf16 (1.32).
+// 64-row group (row 4 * lane + n).  8192^3: 770 .. 825 us (fp16 results: 740) = 1.33 .. 1.49 PFLOP/s; the large library product in bf16 1.32.
+// K = 768, 12 layers: 2640 .. 2720 us for the 6.4 GB of fp32 results, 2160 of fp16.
 template <int DT, int FA, int FB>
 __global__ __launch_bounds__(512, 2) void gemm8_large_exact_kernel(Gemm8Args g, int total) {
     typedef typename Elem<DT>::type T;

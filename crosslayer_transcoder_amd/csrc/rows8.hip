@@ -17,7 +17,8 @@ typedef b8_bf16x8 bf16x8;
 constexpr int WAVES = 8, MAX_T = 32;
 constexpr int LDS_CAP = 136 * 1024;                  // packed slice of x at most
 // (beyond 32 tokens packing and the tiled product are faster: 64 tokens, 12 layers of 768 -> 32768 102 against 138 us; 32 tokens: 102 against
-// 78, 4096 -> 4096 20 against 13, 393216 -> 768 107 against 105)
+// 78, 4096 -> 4096 20 against 13, 393216 -> 768 107 against 105.  No one border fits all: with packing, 32 / 33 tokens take 75 / 100 us for the 12
+// layers, 13 / 19 for 4096 -> 4096, but 37 / 32 for 4096 -> 32768)
 
 struct Rows8Args {
     const void* x; long x_token, x_layer;            // strides in elements

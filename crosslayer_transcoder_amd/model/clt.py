@@ -62,7 +62,8 @@ class Encoder(SerializableModule):
     @torch.no_grad()
     def forward_layer(self, acts_norm, layer: int, packed: Optional["ops8.Block8"] = None):
         """Inference: [batch, seq, d_acts] of ONE layer -> [batch, seq, d_features] (clt.py:134-145).  packed: pack8()'s weights, one
-        pass over which gives the features (a byte a weight instead of a cast copy); the result has the activations' type."""
+        pass over which gives the features (a byte a weight instead of a cast copy); the result has the activations' type (the sparsifiers
+        take fp32)."""
         from .. import ops
         shp = acts_norm.shape
         if packed is not None:

@@ -283,7 +283,7 @@ def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: 
 def linear8(x: torch.Tensor, w: Block8, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """y [T, L, N] = x [T, L, K] @ w^T + bias with kept packed weights w [L, N, K] (x [T, K] -> y [T, N] when L == 1): x is packed in
     e4m3 with blocks along K on the way.  out_dtype: x's by default.  Up to FEW_TOKENS the products are exact whatever the type, above
-    that as gemm8's: a token's bf16 results may differ between the two, mostly in the last place."""
+    that as gemm8's (K up to 8 M there): a token's bf16 results may differ between the two, mostly in the last place."""
     x = _dense(x)
     _hip(w)
     two = x.dim() == 2

@@ -54,10 +54,11 @@ _CONTRACTIONS8 = False
 
 
 def set_contractions8(on: bool):
-    """Whether Encoder / Decoder / CrosslayerDecoder.forward contract in 8-bit block-scaled form (custom_ops8.py) and keep their input
-    in 8 bits for the backward pass, instead of in the compute precision.  Off by default: the values differ from the
-    reference's by the rounding to 4 significant bits.  Results have the input's type.  The fused training step does not run
-    the module forward and is unaffected."""
+    """Whether Encoder / Decoder / CrosslayerDecoder.forward over all layers (layer="all") contract in 8-bit block-scaled form
+    (custom_ops8.py) and keep their input in 8 bits for the backward pass, instead of in the compute precision.  Off by default: the values
+    differ from the reference's by the rounding to 4 significant bits.  Results have the input's type; the sparsifiers and standardizers
+    between the maps take fp32, as always.  One layer's forward (layer=k, forward_layer) contracts in 8 bits where it is given
+    packed weights, and the fused training step does not run the module forward: both are unaffected."""
     global _CONTRACTIONS8
     _CONTRACTIONS8 = bool(on)
 
