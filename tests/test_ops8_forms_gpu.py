@@ -560,3 +560,45 @@ def test_the_same_tensor_twice_and_a_stream_of_its_own():
     got = torch.autograd.grad(loss, (x, W))
     torch.cuda.synchronize()
     assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("dec", ["clt", "plt"])
+def test_exported_and_compiled_models(dec):
+    """torch.export of the whole model and torch.compile with batches of changing size, forward and every gradient, to the bit."""
+    import crosslayer_transcoder_amd as cta
+    from crosslayer_transcoder_amd.model import CrosslayerDecoder, CrossLayerTranscoder, Decoder, Encoder, ReLU
+    torch.manual_seed(0)
+    m = CrossLayerTranscoder(ReLU(), Encoder(96, 256, 2), (CrosslayerDecoder if dec == "clt" else Decoder)(96, 256, 2)).cuda()
+    with cta.contractions8():
+        x = rnd(20, 2, 96, seed=1, spread=False)
+        with torch.no_grad():
+            assert torch.equal(torch.export.export(m, (x,)).module()(x)[2], m(x)[2])
+        c = torch.compile(m, backend="aot_eager", dynamic=True)
+        for B in (20, 33, 7, 130):
+            x, g = rnd(B, 2, 96, seed=B, spread=False).requires_grad_(), rnd(B, 2, 96, seed=B + 1, spread=False)
+            leaves = [x] + list(m.parameters())
+            y, z = c(x)[2], m(x)[2]
+            assert torch.equal(y, z)
+            assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(y, leaves, g), torch.autograd.grad(z, leaves, g)))
+
+
+@gpu
+def test_checkpointed_offloaded_and_wrapped_tensors():
+    """Recomputation, saved tensors on the host, a tensor class of its own, inference mode: the bits of a plain call."""
+    from torch.utils.checkpoint import checkpoint
+    from crosslayer_transcoder_amd import custom_ops8 as C
+
+    class Wrapped(torch.Tensor):
+        pass
+
+    x, W, b = rnd(20, 2, 96, seed=1, spread=False), rnd(2, 96, 64, seed=2, spread=False).requires_grad_(), rnd(2, 64, seed=3, spread=False)
+    want = C.plt_decoder8(x, W, b)
+    dW, = torch.autograd.grad(want.sum(), W)
+    assert torch.equal(torch.autograd.grad(checkpoint(lambda x: C.plt_decoder8(x, W, b), x, use_reentrant=False).sum(), W)[0], dW)
+    with torch.autograd.graph.save_on_cpu():
+        y = C.plt_decoder8(x, W, b)
+    assert torch.equal(torch.autograd.grad(y.sum(), W)[0], dW)
+    assert torch.equal(C.plt_decoder8(x.as_subclass(Wrapped), W, b).as_subclass(torch.Tensor), want)
+    with torch.inference_mode():
+        assert torch.equal(C.plt_decoder8(x, W, b), want)
