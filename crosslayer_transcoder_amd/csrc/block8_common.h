@@ -14,6 +14,9 @@ constexpr int B8_MIN_EXP = -112;                     // smallest scale exponent:
 // the conversions and the bf16 matrix instructions do; tested.)  At the other end 1.9375 x 2^127 (e5m2: 1.875) and more rounds to code x 2^e =
 // 2^128, an infinity in fp32 and bf16.
 
+// a launch's threads are counted in 32 bits
+static inline bool b8_fits(long blocks, int threads) { return blocks <= 0xffffffffL / threads; }
+
 __host__ __device__ static inline long up128(long n) { return (n + 127) / 128 * 128; }
 
 // Scale exponent of a block from the bits of its largest finite magnitude: the smallest e >= -112 with amax <= largest * 2^e.

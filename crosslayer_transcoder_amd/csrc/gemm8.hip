@@ -278,7 +278,7 @@ template <int DT, int FA, int FB> int launch_fmt(const Gemm8Args& g, long blocks
 template <int DT> int fold(const Gemm8Args& g, hipStream_t st) {
     const int quads = (g.N - 1) / 4 + 1;
     const long total = (long)g.batch * g.M * quads, fold = (total + 255) / 256;
-    if (fold > 0x7fffffffL) return CLT_ERR_RANGE;
+    if (!b8_fits(fold, 256)) return CLT_ERR_RANGE;
     gemm8_fold_kernel<DT><<<dim3((unsigned)fold), dim3(256), 0, st>>>(g, quads, total);
     CLT_LAUNCH_CHECK();
     return CLT_OK;
@@ -339,7 +339,7 @@ extern "C" int clt_gemm8(const void* a, const void* a_scale, int a_format, long 
         g.first = (int)plan.large;
         blocks = 4 * (tiles - plan.large);
     }
-    if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
+    if (!b8_fits(blocks, 256)) return CLT_ERR_RANGE;
     return c_dtype == CLT_DT_F32 ? launch<CLT_DT_F32>(g, a_format, b_format, blocks, st)
            : c_dtype == CLT_DT_BF16 ? launch<CLT_DT_BF16>(g, a_format, b_format, blocks, st)
                                     : launch<CLT_DT_F16>(g, a_format, b_format, blocks, st);

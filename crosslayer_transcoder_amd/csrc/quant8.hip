@@ -244,15 +244,15 @@ extern "C" int clt_pack8_into(const void* x, int dtype, long row_stride, long ba
     const size_t need = clt_pack8_sums_workspace_bytes(batch, rows, cols);
     if (column_sums && need && (!workspace || workspace_bytes < need)) return CLT_ERR_WORKSPACE;
     a.sums = !column_sums ? nullptr : need ? static_cast<float*>(workspace) : column_sums;
-    const long blocks = (long)batch * a.tiles_r * a.tiles_c;
-    if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
+    const long blocks = (long)batch * a.tiles_r * a.tiles_c, sums = ((long)batch * cols + 255) / 256;
+    if (!b8_fits(blocks, 256) || (column_sums && need && !b8_fits(sums, 256))) return CLT_ERR_RANGE;
     const hipStream_t hs = as_stream(stream);
     const int rc = dtype == CLT_DT_F32 ? launch_pack<CLT_DT_F32>(a, format, tiles != 0, blocks, hs)
                    : dtype == CLT_DT_BF16 ? launch_pack<CLT_DT_BF16>(a, format, tiles != 0, blocks, hs)
                                           : launch_pack<CLT_DT_F16>(a, format, tiles != 0, blocks, hs);
     if (rc != CLT_OK || !column_sums || !need) return rc;
     const long n = (long)batch * cols;
-    fold_sums_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, hs>>>(a.sums, column_sums, a.tiles_r, cols, n);
+    fold_sums_kernel<<<dim3((unsigned)sums), dim3(256), 0, hs>>>(a.sums, column_sums, a.tiles_r, cols, n);
     CLT_LAUNCH_CHECK();
     return CLT_OK;
 }
@@ -265,7 +265,7 @@ extern "C" int clt_unpack8(const void* q, const void* s, int format, int batch, 
     if (!aligned16(q) || pitch % 16 || q_batch_stride % 16 || ((uintptr_t)out & (es - 1))) return CLT_ERR_ALIGN;
     const int chunks = (cols - 1) / 16 + 1;
     const long total = (long)batch * rows * chunks, blocks = (total + 255) / 256;
-    if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
+    if (!b8_fits(blocks, 256)) return CLT_ERR_RANGE;
     const dim3 g((unsigned)blocks), t(256);
     const hipStream_t hs = as_stream(stream);
     const uint8_t *qp = static_cast<const uint8_t*>(q), *sp = static_cast<const uint8_t*>(s);

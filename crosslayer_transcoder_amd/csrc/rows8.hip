@@ -276,7 +276,7 @@ extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride,
     a.part = c.slices > 1 ? static_cast<float*>(workspace) : nullptr;
     a.T = tokens; a.N = N; a.K = K; a.KB = KB; a.slice_kb = c.slice_kb; a.slices = c.slices; a.chunks = c.chunks; a.row_blocks = c.row_blocks; a.layers = layers;
     const long blocks = (long)layers * c.slices * c.row_blocks;
-    if (blocks > 0x7fffffffL) return CLT_ERR_RANGE;
+    if (!b8_fits(blocks, WAVES * 64)) return CLT_ERR_RANGE;
     const int lds = tokens * (c.slice_kb * 256 + 16);
     const hipStream_t st = as_stream(stream);
     int rc;
@@ -284,7 +284,7 @@ extern "C" int clt_linear8_rows(const void* x, int x_dtype, long x_token_stride,
     else rc = launch_rows<2, 1>(a, w_format, blocks, lds, st);
     if (rc != CLT_OK || c.slices == 1) return rc;
     const long n = (long)layers * tokens * N, fold = (n + 255) / 256;
-    if (fold > 0x7fffffffL) return CLT_ERR_RANGE;
+    if (!b8_fits(fold, 256)) return CLT_ERR_RANGE;
     rows8_fold_kernel<<<dim3((unsigned)fold), dim3(256), 0, st>>>(a, n);
     CLT_LAUNCH_CHECK();
     return CLT_OK;

@@ -535,7 +535,8 @@ int clt_sparse_scatter_dense_f32(const uint32_t* col_start, const int32_t* tok, 
  * [up128(cols) / 128][up128(rows)]: byte e + 127 is the scale 2^e of a row's block of 128 columns.  e is the smallest integer
  * >= -112 with amax <= largest * 2^e, amax over the block's finite values; code = x * 2^-e rounded to nearest, ties to even.
  * NaN stays NaN; an infinity becomes NaN (e4m3, which has none) or stays (e5m2); a magnitude of 1.9375 * 2^127 (e5m2: 1.875) and more is held as 2^128,
- * an infinity once restored or multiplied in bf16.  q, s and their pitches: 16-byte aligned.
+ * an infinity once restored or multiplied in bf16.  q, s and their pitches: 16-byte aligned.  A call that would need more than 2^32 threads
+ * (packing 2.7e11 elements, restoring 6.8e10) is CLT_ERR_RANGE.
  */
 #define CLT_F8_E4M3 0 /* 4 exponent bits, 3 mantissa bits, largest 448   */
 #define CLT_F8_E5M2 1 /* 5 exponent bits, 2 mantissa bits, largest 57344 */

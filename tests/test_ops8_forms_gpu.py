@@ -602,3 +602,15 @@ def test_checkpointed_offloaded_and_wrapped_tensors():
     assert torch.equal(C.plt_decoder8(x.as_subclass(Wrapped), W, b).as_subclass(torch.Tensor), want)
     with torch.inference_mode():
         assert torch.equal(C.plt_decoder8(x, W, b), want)
+
+
+def test_more_threads_than_a_launch_counts_are_refused():
+    """Grids of more than 2^32 threads: errors before any launch (fewer blocks than 2^31, the count alone)."""
+    from crosslayer_transcoder_amd._lib import lib
+    p = 4096                                                                     # an aligned address nothing reads
+    rows = 1 << 27
+    assert lib.clt_unpack8(p, p, 0, 1, rows, 4096, 4096, rows, 0, 0, p, 1, None) == -6
+    assert lib.clt_pack8(p, 1, 4096, 0, 1, rows, 4096, 0, 0, p, p, None, None, None, None, 0, None) == -6
+    # results 2^23 elements apart, where only small tiles run: 2^13 x 2^13 of them
+    n = 1 << 20
+    assert lib.clt_gemm8(p, p, 0, 128, n, 0, 0, p, p, 0, 128, n, 0, 0, p, 1, 1 << 23, 0, None, 0, n, n, 128, 1, 0, None, 0, None) == -6
