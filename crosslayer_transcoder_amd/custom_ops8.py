@@ -9,8 +9,10 @@ the same two forms: dx = g8 W8^T, dW = X8t g8t^T, db = the sum of g itself, take
 straight-through gradients: rounding to 8 bits counts as the identity.
 
 y and dx have x's type, dW has W's, db has b's.  A product with a bf16 result uses the 8-bit matrix instructions, which align products
-to about 14 bits (`ops8.gemm8`), one with an fp32 or fp16 result is exact up to fp32 sums: x in fp32 or fp16 asks for that.  A training step can be captured into a graph, forward and backward, as long as no
-eager graph of the same leaves is alive then (torch's own rule: the engine would wait for the stream that graph was made on)."""
+to about 14 bits (`ops8.gemm8`), one with an fp32 or fp16 result is exact up to fp32 sums: x in fp32 or fp16 asks for that.
+
+A training step can be captured into a graph, forward and backward, as long as no eager graph of the same leaves is alive then (torch's
+own rule: the engine would wait for the stream that graph was made on)."""
 from typing import List, Optional
 
 import torch

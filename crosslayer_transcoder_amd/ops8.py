@@ -251,8 +251,8 @@ def gemm8(a: Block8, b: Block8, bias: Optional[torch.Tensor] = None, out_dtype: 
     """out [L, M, N] (+)= a [L, M, K] @ b [L, N, K]^T + bias [L, N].  fp32 and fp16 results: exact products, fp32 sums, one rounding; bf16
     results: the 8-bit matrix instructions, at twice the rate.  These align the products of a group of 16 k to about 14 bits below the
     largest one: off by less than 2^-9 of the sum of |a b|, by about 1e-5 of the result's norm on normal data (rounding: 1.7e-3), more
-    where large products cancel.  `out`: an [L, M, N] tensor or view with a dense last dimension to write into (its dtype counts), sharing nothing with the operands; accumulate: add to it (fp32
-    only).  The codes of a row of a or b take at most 8 MB."""
+    where large products cancel.  `out`: an [L, M, N] tensor or view with a dense last dimension to write into (its dtype counts), sharing
+    nothing with the operands; accumulate: add to it (fp32 only).  The codes of a row of a or b take at most 8 MB."""
     _hip(a), _hip(b)
     L, M, N, K = a.batch, a.rows, b.rows, a.cols
     if b.batch != L or b.cols != K or b.device != a.device:
